@@ -50,6 +50,22 @@ class CompactOut(ctypes.Structure):
     ]
 
 
+class KvCache(ctypes.Structure):
+    _fields_ = [
+        ("k", c_void_p),
+        ("v", c_void_p),
+        ("k_scale", c_void_p),
+        ("v_scale", c_void_p),
+        ("slots", c_int64),
+        ("slot_stride", c_int64),
+        ("head_stride", c_int64),
+        ("scale_stride", c_int64),
+        ("heads", c_int32),
+        ("dim", c_int32),
+        ("dtype", c_int32),
+    ]
+
+
 # argument types of every entry point (restype is int unless listed in _RESTYPES)
 _SIGNATURES = {
     "dsv_version": [],
@@ -115,6 +131,19 @@ _SIGNATURES = {
                          c_void_p],
     "dsv_serial_chain": [c_int32, c_int32, c_int32, c_void_p, c_void_p, c_void_p, c_void_p,
                          c_void_p, c_void_p],
+    "dsv_kv_write": [c_int64, c_int32, c_void_p, c_int64, c_int64, c_void_p, c_int64, c_int64,
+                     c_void_p, c_int32, ctypes.POINTER(KvCache), c_void_p, c_void_p],
+    "dsv_kv_read": [c_int64, c_void_p, c_int32, ctypes.POINTER(KvCache), c_int32, c_void_p,
+                    c_void_p, c_void_p, c_void_p],
+    "dsv_tree_attention_workspace_size": [c_int32, c_int32, c_int32, c_int32,
+                                          ctypes.POINTER(c_size_t)],
+    "dsv_tree_attention": [c_int32, c_int64, c_int32, c_int32, c_void_p, c_int64, c_int64,
+                           ctypes.POINTER(KvCache), c_void_p, c_int64, c_int32, c_int32, c_void_p,
+                           c_void_p, c_int32, c_void_p, ctypes.c_float, c_void_p, c_int64, c_int64,
+                           c_void_p, c_void_p, c_void_p, c_size_t, c_void_p],
+    "dsv_accept_tree": [c_int32, c_int64, c_void_p, c_void_p, c_void_p, c_void_p, c_int32,
+                        c_void_p, c_void_p, c_int32, c_void_p, c_void_p, c_void_p, c_void_p,
+                        c_void_p, c_void_p, c_void_p, c_void_p],
     "dsv_verify_logits_noalloc": [c_int32, c_int32, c_int32, c_void_p, c_void_p, c_void_p,
                                   c_int64, c_void_p, c_void_p, c_int64, c_int64, c_void_p,
                                   c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p,

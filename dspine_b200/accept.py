@@ -1,18 +1,21 @@
-"""Host API of the per-request accept steps (C ABI: dsv_accept_greedy, dsv_accept_compact).
+"""Host API of the per-request accept steps (C ABI: dsv_accept_greedy, dsv_accept_compact,
+dsv_accept_tree).
 
 `accept_greedy` is verification/caps.py:32-59 `_accept_capped` on the GPU: the five accept
 outputs of a greedy (argmax) verification from the target's top-1 ids.  `accept_compact`
 packs accepted tokens and KV slots after any accept step (SGLang's `_commit_accept`, wrapped
-at runtime/worker.py:745-777).  Argument errors raise ValueError before launch.
+at runtime/worker.py:745-777).  `accept_tree` is the greedy accept for draft trees.  Argument errors raise ValueError before launch.
 """
 
 from __future__ import annotations
 
 import ctypes
+from dataclasses import dataclass
 
 import torch
 
 from . import _lib
+from .kvcache import on_device
 from .verify import CompactOutputs, Workspace, new_outputs, workspace_for  # noqa: F401
 
 T = 16
@@ -73,3 +76,77 @@ def accept_compact(commit, verify_lens, output, slots, slot_rows, *, compact=Non
               output.contiguous().data_ptr(), ctypes.byref(c), workspace.buf.data_ptr(),
               _stream(dev))
     return compact
+
+
+@dataclass
+class TreeAccept:
+    """Outputs of accept_tree (see there)."""
+
+    accept: torch.Tensor
+    commit: torch.Tensor
+    bonus: torch.Tensor
+    output: torch.Tensor
+    path: torch.Tensor
+    kept_slots: torch.Tensor | None
+    new_seq: torch.Tensor
+
+    @staticmethod
+    def allocate(batch: int, width: int, device, *, slots=True) -> "TreeAccept":
+        def empty(*shape, dtype=torch.int32):
+            return torch.empty(shape, dtype=dtype, device=device)
+
+        return TreeAccept(empty(batch), empty(batch), empty(batch, dtype=torch.int64),
+                          empty(batch, width, dtype=torch.int64), empty(batch, width),
+                          empty(batch, width) if slots else None, empty(batch))
+
+
+def accept_tree(tokens, top1, tree_mask, *, q_indptr=None, prefix_lens=None, slots=None, width=None, outputs=None):
+    """Greedy acceptance over draft trees (C ABI: dsv_accept_tree), the tree form of accept_greedy.
+
+    tokens, top1, tree_mask [rows] int64: each drafted node's token, the target's top-1 token at
+    it and its ancestor bits (`attention.tree_mask`); node 0 of a request is the root, its last
+    committed token.  Request b owns rows [q_indptr[b], q_indptr[b+1]) (int32 [B+1]; None: tokens
+    is [B, nodes], and so are top1, tree_mask and slots).  A node is accepted when its token and those of all its ancestors are
+    the top-1 token of their parent; the deepest accepted node, the first among equals, ends the
+    path.  Returns TreeAccept: accept [B] (drafted nodes on the path), commit = accept + 1, bonus
+    [B] int64 (the top-1 token after the path), output [B, width] int64 (the path's tokens after
+    the root, the bonus, then 0), path [B, width] int32 (its nodes, then -1), kept_slots [B,
+    width] int32 (slots of its nodes, then -1; None without slots), new_seq = prefix_lens (zeros
+    when None) + commit.  At most the first `width` (<= 64, default 64 or nodes) rows of a request
+    are looked at; a request without rows gets commit 0 and bonus -1."""
+    dev = tokens.device
+    if q_indptr is None:
+        _check(tokens.dim() == 2, "without q_indptr tokens must be [requests, nodes]")
+        B, nodes = tokens.shape
+        width = max(1, nodes) if width is None else int(width)
+        _check(nodes <= width, "width must hold every node")
+    else:
+        _check(tokens.dim() == 1, "with q_indptr tokens must be [rows]")
+        _check(q_indptr.dim() == 1 and q_indptr.shape[0] >= 1 and q_indptr.dtype == torch.int32 and q_indptr.device == dev
+               and q_indptr.is_contiguous(), "q_indptr must be contiguous int32 [requests + 1]")
+        B, nodes = q_indptr.shape[0] - 1, 0
+        width = 64 if width is None else int(width)
+    _check(1 <= width <= 64, "a draft tree has at most 64 nodes")
+    for name, x in (("tokens", tokens), ("top1", top1), ("tree_mask", tree_mask)):
+        _check(x.shape == tokens.shape and x.dtype == torch.int64 and x.is_contiguous() and x.device == dev,
+               f"{name} must be contiguous int64, one value a node")
+    _check(prefix_lens is None or (prefix_lens.shape == (B,) and prefix_lens.dtype == torch.int32 and prefix_lens.device == dev
+                                   and prefix_lens.is_contiguous()), "prefix_lens must be contiguous int32 [requests]")
+    _check(slots is None or (slots.shape == tokens.shape and slots.dtype == torch.int32 and slots.device == dev
+                             and slots.is_contiguous()), "slots must be contiguous int32, one value a node")
+    if outputs is None:
+        outputs = TreeAccept.allocate(B, width, dev, slots=slots is not None)
+    o = outputs
+    for x, shape, dtype in ((o.accept, (B,), torch.int32), (o.commit, (B,), torch.int32), (o.bonus, (B,), torch.int64),
+                            (o.output, (B, width), torch.int64), (o.path, (B, width), torch.int32),
+                            (o.new_seq, (B,), torch.int32)) + (((o.kept_slots, (B, width), torch.int32),) if slots is not None else ()):
+        _check(x is not None and x.shape == shape and x.dtype == dtype and x.device == dev and x.is_contiguous(),
+               "outputs must be as TreeAccept.allocate gives them")
+    _check(dev.type == "cuda", "tensors must be on a CUDA device")
+    if B:
+        with on_device(dev) as stream:
+            _lib.call("dsv_accept_tree", B, tokens.numel(), tokens.data_ptr(), top1.data_ptr(), tree_mask.data_ptr(),
+                      _lib.ptr(q_indptr), nodes, _lib.ptr(prefix_lens), _lib.ptr(slots), width, o.accept.data_ptr(),
+                      o.commit.data_ptr(), o.bonus.data_ptr(), o.output.data_ptr(), o.path.data_ptr(),
+                      o.kept_slots.data_ptr() if slots is not None else None, o.new_seq.data_ptr(), stream)
+    return outputs

@@ -46,6 +46,25 @@ void* noalloc_scratch() {
     return g_noalloc_addr[dev];
 }
 
+// a KV cache that the kernels can address, as the kernels take it
+int check_cache(const dsv_kv_cache* c, int max_dim, dsv::KvCache* out) {
+    if (c == nullptr) return DSV_BAD_POINTER;
+    if (c->dtype != DSV_BF16 && c->dtype != DSV_F16 && c->dtype != DSV_E4M3) return DSV_BAD_DTYPE;
+    if (c->slots < 1 || c->slots > 0x7fffffff || c->heads < 1 || c->dim < 16 || c->dim > max_dim ||
+        c->dim % 16 != 0 || c->head_stride < c->dim || c->slot_stride < c->dim ||
+        (c->dtype == DSV_E4M3 && c->scale_stride < c->heads))
+        return DSV_BAD_SHAPE;
+    const bool codes = c->dtype == DSV_E4M3;
+    if (!c->k || !c->v || (codes && (!c->k_scale || !c->v_scale))) return DSV_BAD_POINTER;
+    const int64_t step = codes ? 16 : 8;  // elements in 16 bytes
+    if (!aligned(c->k, 16) || !aligned(c->v, 16) || c->slot_stride % step != 0 ||
+        c->head_stride % step != 0 || (codes && (!aligned(c->k_scale, 4) || !aligned(c->v_scale, 4))))
+        return DSV_BAD_ALIGNMENT;
+    *out = {c->k, c->v, c->k_scale, c->v_scale, c->slots, c->slot_stride, c->head_stride,
+            c->scale_stride, c->heads, c->dim, c->dtype};
+    return DSV_OK;
+}
+
 }  // namespace
 
 extern "C" {
@@ -554,6 +573,145 @@ int dsv_target_probs(int64_t rows, int32_t vocab, int32_t rows_per_request, cons
     return dsv_target_probs_ex(rows, vocab, DSV_BF16, rows_per_request, logits, row_stride,
                                temperature, top_k, top_p, nullptr, DSV_FILTER_JOINT, probs,
                                workspace, workspace_bytes, stream);
+}
+
+int dsv_kv_write(int64_t tokens, int32_t dtype, const void* k, int64_t k_token_stride,
+                 int64_t k_head_stride, const void* v, int64_t v_token_stride,
+                 int64_t v_head_stride, const void* slots, int32_t slots_int64,
+                 const dsv_kv_cache* cache, uint32_t* err, dsv_stream_t stream) {
+    if (tokens < 0) return DSV_BAD_SHAPE;
+    if (dtype != DSV_BF16 && dtype != DSV_F16 && dtype != DSV_F32) return DSV_BAD_DTYPE;
+    dsv::KvRowsArgs a = {};
+    const int st = check_cache(cache, 256, &a.c);
+    if (st != DSV_OK) return st;
+    if (a.c.dtype != DSV_E4M3 && a.c.dtype != dtype) return DSV_BAD_DTYPE;
+    if (tokens == 0) return DSV_OK;
+    if (tokens > 0x7fffffff / a.c.heads) return DSV_BAD_SHAPE;
+    if (!k || !v || !slots) return DSV_BAD_POINTER;
+    const int64_t step = dtype == DSV_F32 ? 4 : 8;
+    if (!aligned(k, 16) || !aligned(v, 16) || k_token_stride % step || k_head_stride % step ||
+        v_token_stride % step || v_head_stride % step || !aligned(slots, slots_int64 ? 8 : 4) ||
+        !aligned(err, 4))
+        return DSV_BAD_ALIGNMENT;
+    a.tokens = tokens;
+    a.slots = slots;
+    a.slots64 = slots_int64 != 0;
+    a.k = k;
+    a.v = v;
+    a.k_token_stride = k_token_stride;
+    a.k_head_stride = k_head_stride;
+    a.v_token_stride = v_token_stride;
+    a.v_head_stride = v_head_stride;
+    a.err = err;
+    return counted(dsv::launch_kv_write(a, dtype, (cudaStream_t)stream), 1);
+}
+
+int dsv_kv_read(int64_t tokens, const void* slots, int32_t slots_int64, const dsv_kv_cache* cache,
+                int32_t out_dtype, void* k, void* v, uint32_t* err, dsv_stream_t stream) {
+    if (tokens < 0) return DSV_BAD_SHAPE;
+    if (out_dtype != DSV_BF16 && out_dtype != DSV_F16 && out_dtype != DSV_F32) return DSV_BAD_DTYPE;
+    dsv::KvRowsArgs a = {};
+    const int st = check_cache(cache, 256, &a.c);
+    if (st != DSV_OK) return st;
+    if (tokens == 0) return DSV_OK;
+    if (tokens > 0x7fffffff / a.c.heads) return DSV_BAD_SHAPE;
+    if (!k || !v || !slots) return DSV_BAD_POINTER;
+    if (!aligned(k, 16) || !aligned(v, 16) || !aligned(slots, slots_int64 ? 8 : 4) || !aligned(err, 4))
+        return DSV_BAD_ALIGNMENT;
+    a.tokens = tokens;
+    a.slots = slots;
+    a.slots64 = slots_int64 != 0;
+    a.k = k;
+    a.v = v;
+    a.err = err;
+    return counted(dsv::launch_kv_read(a, out_dtype, (cudaStream_t)stream), 1);
+}
+
+int dsv_tree_attention_workspace_size(int32_t q_heads, int32_t kv_heads, int32_t dim,
+                                      int32_t width, size_t* bytes) {
+    if (bytes == nullptr) return DSV_BAD_POINTER;
+    if (kv_heads < 1 || q_heads < kv_heads || q_heads % kv_heads != 0 || dim < 16 || dim > 128 ||
+        dim % 16 != 0 || width < 1)
+        return DSV_BAD_SHAPE;
+    *bytes = dsv::tree_attn_workspace_bytes(q_heads, kv_heads, dim, width);
+    return DSV_OK;
+}
+
+int dsv_tree_attention(int32_t batch, int64_t rows, int32_t q_heads, int32_t dtype, const void* q,
+                       int64_t q_token_stride, int64_t q_head_stride, const dsv_kv_cache* cache,
+                       const int32_t* page_table, int64_t table_stride, int32_t max_pages,
+                       int32_t page_size, const int32_t* kv_lens, const int32_t* q_indptr,
+                       int32_t width, const int64_t* tree_mask, float scale, void* out,
+                       int64_t out_token_stride, int64_t out_head_stride, float* lse,
+                       uint32_t* err, void* workspace, size_t workspace_bytes,
+                       dsv_stream_t stream) {
+    if (dtype != DSV_BF16 && dtype != DSV_F16) return DSV_BAD_DTYPE;
+    dsv::TreeAttnArgs a = {};
+    const int st = check_cache(cache, 128, &a.c);
+    if (st != DSV_OK) return st;
+    if (a.c.dtype != DSV_E4M3 && a.c.dtype != dtype) return DSV_BAD_DTYPE;
+    if (batch < 0 || rows < 0 || rows > 0x7fffffff || q_heads < 1 || q_heads % a.c.heads != 0 ||
+        page_size < 1 || a.c.slots % page_size != 0 || max_pages < 0 || table_stride < max_pages ||
+        width < 1 || (int64_t)max_pages * page_size > 0x7fffffff)
+        return DSV_BAD_SHAPE;
+    if (q_indptr == nullptr && rows != (int64_t)batch * width) return DSV_BAD_SHAPE;
+    if (tree_mask != nullptr && q_indptr == nullptr && width > 64) return DSV_BAD_SHAPE;
+    if (!(scale > 0.f) || !(scale < 3.4e38f)) return DSV_UNSUPPORTED;
+    if (batch == 0 || rows == 0) return DSV_OK;
+    if (!q || !out || !kv_lens || (max_pages > 0 && !page_table)) return DSV_BAD_POINTER;
+    if (!aligned(q, 16) || !aligned(out, 16) || q_token_stride % 8 || q_head_stride % 8 ||
+        out_token_stride % 8 || out_head_stride % 8 || !aligned(page_table, 4) ||
+        !aligned(kv_lens, 4) || !aligned(q_indptr, 4) || !aligned(tree_mask, 8) ||
+        !aligned(lse, 4) || !aligned(err, 4))
+        return DSV_BAD_ALIGNMENT;
+    if (workspace_bytes < dsv::tree_attn_workspace_bytes(q_heads, a.c.heads, a.c.dim, width))
+        return DSV_WORKSPACE_TOO_SMALL;
+    if (workspace_bytes > 0 && !workspace) return DSV_BAD_POINTER;
+    if (!aligned(workspace, 16)) return DSV_BAD_ALIGNMENT;
+    a.batch = batch;
+    a.q_heads = q_heads;
+    a.group = q_heads / a.c.heads;
+    a.rows = rows;
+    a.q = q;
+    a.q_token_stride = q_token_stride;
+    a.q_head_stride = q_head_stride;
+    a.out = out;
+    a.out_token_stride = out_token_stride;
+    a.out_head_stride = out_head_stride;
+    a.lse = lse;
+    a.table = page_table;
+    a.table_stride = table_stride;
+    a.max_pages = max_pages;
+    a.page_size = page_size;
+    a.lens = kv_lens;
+    a.indptr = q_indptr;
+    a.width = width;
+    a.mask = tree_mask;
+    a.scale = scale;
+    a.err = err;
+    a.ws = workspace;
+    return counted(dsv::launch_tree_attn(a, dtype, (cudaStream_t)stream), 1);
+}
+
+int dsv_accept_tree(int32_t batch, int64_t rows, const int64_t* tokens, const int64_t* top1,
+                    const int64_t* tree_mask, const int32_t* q_indptr, int32_t nodes,
+                    const int32_t* prefix, const int32_t* slots, int32_t width, int32_t* accept,
+                    int32_t* commit, int64_t* bonus, int64_t* output, int32_t* path, int32_t* kept,
+                    int32_t* new_seq, dsv_stream_t stream) {
+    if (batch < 0 || rows < 0 || width < 1 || width > 64) return DSV_BAD_SHAPE;
+    if (q_indptr == nullptr && (nodes < 0 || nodes > width || rows != (int64_t)batch * nodes))
+        return DSV_BAD_SHAPE;
+    if (batch == 0) return DSV_OK;
+    if ((rows > 0 && (!tokens || !top1 || !tree_mask || (kept && !slots))) || !accept || !commit || !bonus || !output ||
+        !path || !new_seq)
+        return DSV_BAD_POINTER;
+    if (!aligned(tokens, 8) || !aligned(top1, 8) || !aligned(tree_mask, 8) || !aligned(q_indptr, 4) ||
+        !aligned(prefix, 4) || !aligned(slots, 4) || !aligned(bonus, 8) || !aligned(output, 8))
+        return DSV_BAD_ALIGNMENT;
+    dsv::TreeAcceptArgs t = {batch, rows, tokens, top1, tree_mask, q_indptr, nodes, prefix, slots,
+                             width, accept, commit, bonus, output, path, kept,
+                             new_seq};
+    return counted(dsv::launch_tree_accept(t, (cudaStream_t)stream), 1);
 }
 
 int dsv_topk_ids(int64_t rows, int32_t vocab, int64_t row_stride, int32_t dtype,

@@ -389,4 +389,78 @@ int launch_compact(int B, const int32_t* commit, const int32_t* lens, const int6
                    int64_t* tok_out, int32_t* slot_out, int32_t* offsets, int32_t* free_out,
                    int32_t* free_offsets, unsigned int* err, cudaStream_t stream);
 
+// ---- slot-addressed KV cache (kvcache.cu, attention.cu) -----------------------------------
+enum Dtype : int { kBf16 = 0, kF32 = 1, kF16 = 2, kE4m3 = 3 };
+
+struct KvCache {
+    void* k;                   // [slots, heads, dim], strides below (elements)
+    void* v;
+    float* k_scale;            // [slots, heads] (e4m3 only), rows scale_stride apart
+    float* v_scale;
+    long long slots;
+    long long slot_stride, head_stride;
+    long long scale_stride;
+    int heads, dim, dtype;     // Dtype
+};
+
+struct KvRowsArgs {
+    KvCache c;
+    long long tokens;
+    const void* slots;         // [tokens] int32 or int64; negative: no slot
+    int slots64;
+    const void* k;             // rows [tokens, heads, dim]; read: outputs, packed
+    const void* v;
+    long long k_token_stride, k_head_stride, v_token_stride, v_head_stride;
+    unsigned int* err;         // or null; bit 0: a slot past the cache
+    int lanes;                 // set by the launcher
+};
+int launch_kv_write(KvRowsArgs a, int dtype, cudaStream_t stream);
+int launch_kv_read(KvRowsArgs a, int dtype, cudaStream_t stream);
+
+// ---- attention of drafted tokens over the cache (attention.cu) ----------------------------
+struct TreeAttnArgs {
+    KvCache c;
+    int batch, q_heads, group; // group = q_heads / kv heads
+    long long rows;            // rows of q, out, lse
+    const void* q;             // [rows, q_heads, dim]
+    long long q_token_stride, q_head_stride;
+    void* out;
+    long long out_token_stride, out_head_stride;
+    float* lse;                // [rows, q_heads] or null
+    const int32_t* table;      // [batch, max_pages], rows table_stride apart
+    long long table_stride;
+    int max_pages, page_size;
+    const int32_t* lens;       // [batch]
+    const int32_t* indptr;     // [batch + 1] or null: `width` rows each
+    int width;
+    const int64_t* mask;       // [rows] ancestor bits or null: a chain
+    float scale;
+    unsigned int* err;         // or null
+    void* ws;
+};
+size_t tree_attn_workspace_bytes(int q_heads, int kv_heads, int dim, int width);
+int launch_tree_attn(const TreeAttnArgs& a, int dtype, cudaStream_t stream);
+
+// ---- greedy acceptance over draft trees (tree.cu) -----------------------------------------
+struct TreeAcceptArgs {
+    int batch;
+    long long rows;
+    const int64_t* tokens;     // [rows]
+    const int64_t* top1;       // [rows]
+    const int64_t* mask;       // [rows] ancestor bits
+    const int32_t* indptr;     // [batch + 1] or null: `nodes` rows each
+    int nodes;
+    const int32_t* prefix;     // [batch] or null
+    const int32_t* slots;      // [rows] or null
+    int width;                 // columns of output, path, kept
+    int32_t* accept;
+    int32_t* commit;
+    int64_t* bonus;
+    int64_t* output;           // [batch, width]
+    int32_t* path;             // [batch, width]
+    int32_t* kept;             // [batch, width] or null
+    int32_t* new_seq;
+};
+int launch_tree_accept(const TreeAcceptArgs& a, cudaStream_t stream);
+
 }  // namespace dsv

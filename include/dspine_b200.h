@@ -33,7 +33,7 @@ typedef enum {
     DSV_UNSUPPORTED = 8
 } dsv_status;
 
-typedef enum { DSV_BF16 = 0, DSV_F32 = 1 } dsv_dtype;
+typedef enum { DSV_BF16 = 0, DSV_F32 = 1, DSV_F16 = 2, DSV_E4M3 = 3 } dsv_dtype;
 
 /* Filter modes of the target distribution (runtime/worker.py:473-508 filter_target_probs):
  * JOINT  flashinfer backend, no min-p in the batch: rank < top_k and mass ranked ahead <= top_p,
@@ -409,6 +409,98 @@ int dsv_rescore_select16(int32_t rows, int32_t cands, int32_t hidden, int32_t vo
                          const void* weight, int64_t w_stride, const int64_t* ids,
                          const void* hidden_rows, int64_t h_stride, int32_t hidden_dtype,
                          void* scores, int32_t scores_f32, int64_t* out16, dsv_stream_t stream);
+
+/* ---- slot-addressed KV cache ---------------------------------------------------------------
+ * The cache that the KV slots of the accept step (dsv_compact_out, SGLang's out_cache_loc) point
+ * into: per slot and KV head one K row and one V row of `dim` elements.  dtype DSV_BF16 or
+ * DSV_F16 holds the rows as they are; DSV_E4M3 holds codes with one fp32 scale per (slot, head),
+ * value = code * scale, quantised by the rule of dsv_fp8_quantize_rows applied to each head's row
+ * (scale = amax / 448, 1 for a row of zeros or with a NaN).  No counterpart in the reference
+ * (SGLang owns the cache).  K and V have the same strides; dim is a multiple of 16, at most 256;
+ * rows start on 16-byte boundaries. */
+typedef struct {
+    void* k;                  /* [slots, heads, dim] */
+    void* v;
+    float* k_scale;           /* [slots, heads], DSV_E4M3 only */
+    float* v_scale;
+    int64_t slots;
+    int64_t slot_stride;      /* elements between slots, and between a slot's heads */
+    int64_t head_stride;
+    int64_t scale_stride;     /* scales between slots; a slot's heads are adjacent */
+    int32_t heads;
+    int32_t dim;
+    int32_t dtype;            /* DSV_BF16, DSV_F16 or DSV_E4M3 */
+} dsv_kv_cache;
+
+/* Writes token n's K and V rows (dtype DSV_BF16, DSV_F16 or, into an e4m3 cache, DSV_F32;
+ * strides in elements, rows on 16-byte boundaries) to slot slots[n] (int32, or int64 where
+ * slots_int64).  A negative slot is skipped; one past the cache is skipped and sets bit 0 of
+ * *err (a device word, may be NULL).  Of tokens that share a slot any may be kept, or a mixture
+ * of them: the slots of one call should differ.  A cache that is not e4m3 takes rows of its own
+ * type only.  tokens * heads < 2^31. */
+int dsv_kv_write(int64_t tokens, int32_t dtype, const void* k, int64_t k_token_stride,
+                 int64_t k_head_stride, const void* v, int64_t v_token_stride,
+                 int64_t v_head_stride, const void* slots, int32_t slots_int64,
+                 const dsv_kv_cache* cache, uint32_t* err, dsv_stream_t stream);
+
+/* Reads the rows of slots[n] back into k and v, packed [tokens, heads, dim] of out_dtype
+ * (DSV_BF16, DSV_F16 or DSV_F32): code * scale in fp32, rounded once.  A negative slot gives
+ * rows of zeros, one past the cache too and bit 0 of *err. */
+int dsv_kv_read(int64_t tokens, const void* slots, int32_t slots_int64, const dsv_kv_cache* cache,
+                int32_t out_dtype, void* k, void* v, uint32_t* err, dsv_stream_t stream);
+
+/* ---- attention of drafted tokens over the cache --------------------------------------------
+ * The target's attention on the verified block (behind the logits that dsv_verify_logits
+ * takes).  No counterpart in the reference (SGLang's attention backends).
+ * Request b owns rows [q_indptr[b], q_indptr[b+1]) of q (q_indptr NULL: `width` rows each,
+ * rows == batch * width); rows outside every request are left as they were.  kv_lens[b] counts
+ * its cached tokens with the drafted ones as the last, so drafted token j is cached at position
+ * p0 + j, p0 = kv_lens[b] - (rows of b); a negative position does not exist.  Position p is slot
+ * page_table[b][p / page_size] * page_size + p % page_size.
+ * Row i sees the positions before p0 and drafted token j where bit j of tree_mask[row] is set
+ * (drafted tokens from 64 on: never), or, with tree_mask NULL, where j <= i.
+ * out[row, head] = sum softmax(scale * q . k) v over those, rounded once to dtype; lse [rows,
+ * q_heads] fp32 (may be NULL) the natural logsumexp of the scaled scores.  A row that sees
+ * nothing gets zeros and -inf.  Query head hq reads KV head hq / (q_heads / heads).
+ * dtype (q and out) DSV_BF16 or DSV_F16; the cache has the same type or is e4m3; dim a multiple
+ * of 16, at most 128; cache->slots a multiple of page_size; scale positive and finite.  `width`
+ * is with q_indptr a bound on the rows of a request, by which the work is laid out (a request
+ * with more rows is computed all the same).
+ * Bits of *err (a device word, may be NULL): bit 1: a page outside the cache, or a length above
+ * max_pages * page_size (those positions are unseen); bit 2: a wait inside the kernel timed out
+ * (outputs not valid).  The workspace needs no initialisation; calls that may overlap need one
+ * each. */
+int dsv_tree_attention_workspace_size(int32_t q_heads, int32_t kv_heads, int32_t dim,
+                                      int32_t width, size_t* bytes);
+int dsv_tree_attention(int32_t batch, int64_t rows, int32_t q_heads, int32_t dtype, const void* q,
+                       int64_t q_token_stride, int64_t q_head_stride, const dsv_kv_cache* cache,
+                       const int32_t* page_table, int64_t table_stride, int32_t max_pages,
+                       int32_t page_size, const int32_t* kv_lens, const int32_t* q_indptr,
+                       int32_t width, const int64_t* tree_mask, float scale, void* out,
+                       int64_t out_token_stride, int64_t out_head_stride, float* lse,
+                       uint32_t* err, void* workspace, size_t workspace_bytes,
+                       dsv_stream_t stream);
+
+/* ---- greedy acceptance over draft trees ----------------------------------------------------
+ * The tree form of dsv_accept_greedy (verification/caps.py:32-59 _accept_capped).  Request b owns
+ * rows [q_indptr[b], q_indptr[b+1]) (q_indptr NULL: `nodes` rows each) of tokens, top1,
+ * tree_mask and slots; row 0 is the root, the last committed token, and a parent comes before its
+ * children.  tree_mask as for dsv_tree_attention: bit j of row i set where j is i or an ancestor
+ * (bits above i are not read, bit i counts as set); the parent is the highest bit below i.
+ * Node i agrees where tokens[i] == top1[parent]; it is accepted where it and all its ancestors
+ * agree and the root is one of them.  The path to the deepest accepted node, the first among
+ * equals:
+ *   accept = its drafted nodes, commit = accept + 1, bonus = top1 of its last node,
+ *   path [batch, width] its node indices then -1, output [batch, width] the tokens of its nodes
+ *   after the root, then the bonus, then 0; kept [batch, width] the slots of its nodes then -1
+ *   (NULL: not wanted, slots not read), new_seq = prefix (NULL: 0) + commit.
+ * A request without rows gets accept = commit = 0 and bonus -1.  At most the first
+ * min(64, width) rows of a request are looked at; width 1..64. */
+int dsv_accept_tree(int32_t batch, int64_t rows, const int64_t* tokens, const int64_t* top1,
+                    const int64_t* tree_mask, const int32_t* q_indptr, int32_t nodes,
+                    const int32_t* prefix, const int32_t* slots, int32_t width, int32_t* accept,
+                    int32_t* commit, int64_t* bonus, int64_t* output, int32_t* path, int32_t* kept,
+                    int32_t* new_seq, dsv_stream_t stream);
 
 /* ---- the same verification without a caller workspace ------------------------------------
  * No counterpart in the reference: for callers that cannot allocate device memory (or hand out
