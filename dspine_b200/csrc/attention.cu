@@ -1,4 +1,5 @@
-// attention.cu -- attention of drafted tokens over a slot-addressed, paged KV cache (sm_100a).
+// attention.cu -- attention of drafted tokens over a slot-addressed, paged KV cache (sm_100a:
+// tcgen05 + TMEM).
 //
 // Request b has t_b drafted tokens (rows of q) and lens[b] cached ones, the drafted among them as
 // its last t_b: drafted token j is cached at position p0 + j, p0 = lens[b] - t_b.  Its row i sees
@@ -8,11 +9,46 @@
 // A row that sees nothing gets zeros and -inf.  Position p lives in slot
 // table[b][p / page_size] * page_size + p % page_size; a page outside the cache makes its
 // positions unseen and sets bit 1 of the error word.
+//
+//   attn_kernel     persistent, one CTA per SM.  The rows of one (request, KV head), t_b tokens x
+//                   `group` query heads, are the M = 128 rows of the matrix instructions, so a key
+//                   is read once for all of them.  The tiles of 128 keys of all (request, KV head,
+//                   row block) items form one line that is cut into equal pieces, one per CTA:
+//                   every SM streams the same number of tiles however ragged the lengths are.
+//                     warps 0-7    two softmax warpgroups, one TMEM lane (row) per thread
+//                     warp 8       TMEM allocation and the MMA issuer
+//                     warps 9..    producers: K and V rows of a tile, slot by slot, into a ring of
+//                                  128-byte-swizzled shared-memory stages
+//                   S = Q K^T (kind::f16, both operands in shared memory) and O += P V (P from
+//                   TMEM, written over S; V as a matrix with rows of keys, "MN-major").
+//                   Two streams keep the tensor core and the exponentials busy at once: with more
+//                   than 128 rows each warpgroup owns 128 of them and both use every tile, else
+//                   both own the same rows and take every other tile, with an accumulator each,
+//                   joined at the end.
+//   combine_kernel  joins the partial results of items that a cut went through.
+//
+// Softmax: weights are 2^(s c - ref), c = scale log2(e), ref a running reference that follows the
+// row's maximum but moves only when the maximum has outgrown it by more than 2^8: the accumulator
+// is then rescaled (a TMEM round trip), else left alone.  Any reference gives the same quotient;
+// 2^8 keeps fp16 weights below 2^14.  Sums and the accumulator are fp32; the weights are rounded
+// once to the operand type.
+//
+// e4m3 caches: codes are exact in fp16, so the producers convert them on the way into shared
+// memory and the matrix instructions run on fp16.  q goes to fp16 with a power of two per row.  K
+// scales multiply the scores; V scales multiply the weights, and the reference moves by the running
+// maximum of the V scales (a power of two) so that weight x scale stays within fp16.
+//
+// Masked positions: scores of unseen keys are replaced by -inf, rows of unreadable positions are
+// zeros in shared memory.  A V element of a drafted token that is not finite would reach rows that
+// do not see it through 0 x inf; tiles with drafted tokens are scanned, such elements zeroed and
+// added back to the rows that do see them.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_fp8.h>
 #include <cuda_runtime.h>
 #include <stdint.h>
+
+#include <type_traits>
 
 #include "dsv_common.cuh"
 #include "dsv_kernels.h"
@@ -20,109 +56,1156 @@
 namespace dsv {
 namespace attn {
 
-constexpr int kThreads = 128;
-constexpr int kMaxDim = 128;
+constexpr int kRows = 128;                 // rows of a Q tile (MMA M)
+constexpr int kTile = 128;                 // keys of a tile
+constexpr int kBlock = kTile * 128;        // bytes of a [128 rows][128 bytes] swizzled block
+constexpr int kMaxCtas = 148;              // SMs of a B200; partial results are laid out for these
+constexpr int kInfo = 8;                   // tiles whose validity and scales are held at once
+constexpr int kSoftmaxThreads = 256;
+constexpr int kMinTiles = 2;               // tiles per CTA below which fewer CTAs take part
+constexpr float kSlack = 8.0f;             // log2 by which a maximum may outgrow the reference
+constexpr float kL2E = 1.4426950408889634f;
+constexpr float kLn2 = 0.6931471805599453f;
 
-__device__ __forceinline__ float elem(const void* p, long long i, int dtype) {
-    if (dtype == kBf16) return __bfloat162float(static_cast<const __nv_bfloat16*>(p)[i]);
-    if (dtype == kF16) return __half2float(static_cast<const __half*>(p)[i]);
-    const __half_raw h = __nv_cvt_fp8_to_halfraw(static_cast<const uint8_t*>(p)[i], __NV_E4M3);
-    return __half2float(*reinterpret_cast<const __half*>(&h));
-}
+template <bool kFp8> constexpr int producer_warps() { return kFp8 ? 8 : 4; }
+template <bool kFp8> constexpr int threads() { return kSoftmaxThreads + 32 + 32 * producer_warps<kFp8>(); }
 
-__device__ __forceinline__ void rows_of(const TreeAttnArgs& a, int b, long long& lo, long long& hi) {
+// one slot of the tile ring beside the stages
+struct TileInfo {
+    uint32_t valid[4];        // positions of the tile that exist and can be read
+    float vmax[8];            // e4m3: largest finite V scale, per producer warp
+    float ks[kTile];          // e4m3: K scale x scale x log2(e)
+    float vs[kTile];          // e4m3: V scale
+};
+struct TileInfoPlain {
+    uint32_t valid[4];
+};
+template <bool kFp8> struct InfoOf { using type = TileInfoPlain; };
+template <> struct InfoOf<true> { using type = TileInfo; };
+
+constexpr int kMaxStages = 12;
+
+struct alignas(16) Shared {
+    uint64_t full[kMaxStages];   // stage holds a K or V tile
+    uint64_t empty[kMaxStages];  // the matrix instructions that read it are done
+    uint64_t info[kInfo];        // TileInfo written
+    uint64_t q_full;             // Q of the segment in shared memory, last segment's TMEM read
+    uint64_t s_full[2];          // scores of a stream's tile in TMEM
+    uint64_t p_full[2];          // weights of a stream's tile in TMEM
+    uint64_t o_full;             // the segment's accumulators are complete
+    uint64_t joined;             // both warpgroups have written what the other reads
+    uint64_t drain;
+    uint32_t tmem;
+    int abort;
+    int odd[2];                  // a drafted V element was not finite (by segment parity)
+    // where this CTA starts on the line of tiles
+    int start_b;
+    long long start_in_b;
+    long long scan[32];
+};
+
+template <int DP, bool kFp8> struct Layout {
+    static constexpr int kStage = (DP / 64) * kBlock;      // bytes of a K or V stage
+    static __host__ __device__ constexpr int stages(int qt) {
+        return DP == 128 ? (kFp8 ? 6 - qt : 7 - qt) : (kFp8 ? 8 : 12);
+    }
+    // stages whose copies are in flight before the oldest is waited for.  At least two below the
+    // ring: a K tile of two streams is freed only after the V tile behind it has been handed over.
+    static constexpr int kLag = DP == 128 ? 4 : 10;         // one Q tile
+    static constexpr int kLag2 = DP == 128 ? 3 : 10;        // two Q tiles
+    static_assert(kFp8 || (kLag + 2 <= stages(1) && kLag2 + 2 <= stages(2)), "the ring would lock");
+    static constexpr size_t info_bytes = sizeof(typename InfoOf<kFp8>::type) * kInfo;
+    static constexpr size_t smem(int qt) {
+        return (size_t)(qt + stages(qt)) * kStage + sizeof(Shared) + info_bytes + (kFp8 ? 1024 : 0) + 1024;
+    }
+};
+static_assert(Layout<128, false>::smem(1) <= 232448 && Layout<128, false>::smem(2) <= 232448 &&
+                  Layout<128, true>::smem(1) <= 232448 && Layout<128, true>::smem(2) <= 232448 &&
+                  Layout<64, false>::smem(2) <= 232448 && Layout<64, true>::smem(2) <= 232448,
+              "shared memory of one CTA");
+
+// ---- partial results ------------------------------------------------------------------------
+// CTA c has two slots: 2c for a segment that continues an item, 2c + 1 for one that begins an item
+// and does not finish it.
+struct Split {          // written by CTA c for the item that reaches into it from CTA c - 1
+    int valid;
+    int b, h, block;
+    int first, last;    // CTAs that hold parts of it
+    int pad[2];
+};
+
+struct KernelArgs {
+    TreeAttnArgs t;
+    int qt;                 // Q tiles of a row block
+    Split* splits;          // [kMaxCtas]
+    float2* part_ml;        // [2 * kMaxCtas][128 qt] (reference, sum)
+    float* part_o;          // [2 * kMaxCtas][128 qt][DP], not normalised
+};
+
+// ---- requests, items, segments ---------------------------------------------------------------
+
+struct Request {
+    int lo, n;              // rows of q
+    int len, p0;            // cached positions, the first drafted one
+    int rows, blocks;       // n x group, row blocks
+};
+
+__device__ __forceinline__ Request request_of(const TreeAttnArgs& a, int qt, int b) {
+    Request r;
+    long long lo, hi;
     if (a.indptr) {
-        lo = a.indptr[b];
-        hi = a.indptr[b + 1];
+        lo = __ldg(a.indptr + b);
+        hi = __ldg(a.indptr + b + 1);
         lo = lo < 0 ? 0 : (lo > a.rows ? a.rows : lo);
         hi = hi < lo ? lo : (hi > a.rows ? a.rows : hi);
     } else {
         lo = (long long)b * a.width;
         hi = lo + a.width;
     }
+    const int cap = a.max_pages * a.page_size;
+    const int len = __ldg(a.lens + b);
+    r.lo = (int)lo;
+    r.n = (int)(hi - lo);
+    r.len = len < 0 ? 0 : (len > cap ? cap : len);
+    r.p0 = r.len - r.n;
+    r.rows = r.n * a.group;
+    r.blocks = (r.rows + kRows * qt - 1) / (kRows * qt);
+    return r;
 }
 
-// one block per (query head, request); its rows one after the other, 128 keys at a time
-__global__ void __launch_bounds__(kThreads) rows_kernel(TreeAttnArgs a, int dtype) {
-    __shared__ float q[kMaxDim], p[kThreads], red[kThreads / 32];
-    __shared__ long long at[kThreads];
-    const int tid = threadIdx.x, lane = tid & 31, wid = tid >> 5;
-    const int hq = blockIdx.x, b = blockIdx.y, h = hq / a.group, dim = a.c.dim;
-    const bool scaled = a.c.dtype == kE4m3;
-    long long lo, hi;
-    rows_of(a, b, lo, hi);
-    const long long cap = (long long)a.max_pages * a.page_size;
-    long long len = a.lens[b] < 0 ? 0 : a.lens[b];
-    if (len > cap) {
-        len = cap;
-        if (tid == 0 && a.err) atomicOr(a.err, 2u);
+// tiles of keys that a row block needs: up to the last position its last row sees, one at least
+__device__ __forceinline__ int tiles_of(const TreeAttnArgs& a, int qt, const Request& r, int block) {
+    int end = r.len;
+    if (!a.mask) {
+        const int past = min(r.rows, (block + 1) * kRows * qt);
+        end = min(end, r.p0 + (past - 1) / a.group + 1);
     }
-    const long long p0 = len - (hi - lo), pages = a.c.slots / a.page_size;
-    for (long long r = lo; r < hi; ++r) {
-        const int i = (int)(r - lo);
+    return end <= kTile ? 1 : (end + kTile - 1) / kTile;
+}
+
+__device__ __forceinline__ long long tiles_of_head(const TreeAttnArgs& a, int qt, const Request& r) {
+    if (r.blocks <= 1 || a.mask) return r.blocks == 0 ? 0 : (long long)r.blocks * tiles_of(a, qt, r, r.blocks - 1);
+    long long n = 0;
+    for (int i = 0; i < r.blocks; ++i) n += tiles_of(a, qt, r, i);
+    return n;
+}
+
+__device__ __forceinline__ long long first_tile(long long c, long long total, int ctas) { return c * total / ctas; }
+// the CTA whose piece holds tile x
+__device__ __forceinline__ int cta_of(long long x, long long total, int ctas) {
+    return (int)(((x + 1) * ctas - 1) / total);
+}
+
+// The segments (runs of tiles of one item) of a CTA, in order.  Every warp walks them by itself.
+struct Walk {
+    Request r;
+    int b, h, block;
+    int tiles;              // of the item
+    int k0, k1;             // this segment's tiles
+    long long left;         // tiles of this CTA after this segment
+    int next_k0;            // where the item goes on
+
+    __device__ __forceinline__ void begin(const KernelArgs& a, int b0, long long in_b, long long count) {
+        b = b0;
+        r = request_of(a.t, a.qt, b);
+        const long long per_head = tiles_of_head(a.t, a.qt, r);
+        h = (int)(in_b / per_head);
+        long long at = in_b - h * per_head;
+        block = 0;
+        tiles = tiles_of(a.t, a.qt, r, 0);
+        while (at >= tiles) {
+            at -= tiles;
+            ++block;
+            tiles = tiles_of(a.t, a.qt, r, block);
+        }
+        k0 = (int)at;
+        left = count;
+        take();
+    }
+    __device__ __forceinline__ void take() {
+        k1 = (long long)(tiles - k0) < left ? tiles : k0 + (int)left;
+        left -= k1 - k0;
+    }
+    // the next segment; false at the end of the CTA's piece
+    __device__ __forceinline__ bool advance(const KernelArgs& a) {
+        if (left <= 0) return false;
+        if (++block >= r.blocks) {
+            block = 0;
+            if (++h >= a.t.c.heads) {
+                h = 0;
+                do {
+                    ++b;
+                    r = request_of(a.t, a.qt, b);
+                } while (r.rows == 0);
+            }
+        }
+        tiles = tiles_of(a.t, a.qt, r, block);
+        k0 = 0;
+        take();
+        return true;
+    }
+    __device__ __forceinline__ int count() const { return k1 - k0; }
+    __device__ __forceinline__ int first_row(int qt) const { return block * kRows * qt; }
+    __device__ __forceinline__ int rows(int qt) const { return min(r.rows - first_row(qt), kRows * qt); }
+    __device__ __forceinline__ bool shared_rows(int qt) const { return rows(qt) <= kRows; }
+};
+
+// ---- PTX helpers ------------------------------------------------------------------------------
+
+__device__ __forceinline__ uint64_t smem_desc(uint32_t saddr, uint32_t lead_bytes) {
+    uint64_t d = 0;
+    d |= (uint64_t)((saddr >> 4) & 0x3FFFu);
+    d |= (uint64_t)((lead_bytes >> 4) & 0x3FFFu) << 16;
+    d |= (uint64_t)(1024u >> 4) << 32;              // 8 rows of 128 bytes
+    d |= (uint64_t)1u << 46;                        // descriptor version (sm100)
+    d |= (uint64_t)2u << 61;                        // 128-byte swizzle
+    return d;
+}
+
+__device__ __forceinline__ void tc_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void tc_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
+
+__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d), "l"(a), "l"(b), "r"(idesc),
+        "r"(accumulate)
+        : "memory");
+}
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d), "r"(a), "l"(b), "r"(idesc),
+        "r"(accumulate)
+        : "memory");
+}
+__device__ __forceinline__ void mma_commit(uint64_t* bar) {
+    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(bar))
+                 : "memory");
+}
+__device__ __forceinline__ void mbar_arrive(uint64_t* bar) {
+    asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(bar)) : "memory");
+}
+
+#define DSV_R16(x, o)                                                                                             \
+    x(r[o + 0]), x(r[o + 1]), x(r[o + 2]), x(r[o + 3]), x(r[o + 4]), x(r[o + 5]), x(r[o + 6]), x(r[o + 7]),        \
+        x(r[o + 8]), x(r[o + 9]), x(r[o + 10]), x(r[o + 11]), x(r[o + 12]), x(r[o + 13]), x(r[o + 14]), x(r[o + 15])
+
+// 32 columns of this thread's TMEM lane
+__device__ __forceinline__ void tmem_ld32(uint32_t taddr, uint32_t (&r)[32]) {
+#define DSV_OUT(y) "=r"(y)
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, "
+        "%15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
+        : DSV_R16(DSV_OUT, 0), DSV_R16(DSV_OUT, 16)
+        : "r"(taddr));
+#undef DSV_OUT
+}
+__device__ __forceinline__ void tmem_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t (&r)[32]) {
+#define DSV_IN(y) "r"(y)
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x32.b32 [%32], {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, "
+        "%14, %15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31};" ::DSV_R16(DSV_IN, 0),
+        DSV_R16(DSV_IN, 16), "r"(taddr)
+        : "memory");
+}
+__device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&r)[16]) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x16.b32 [%16], {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, "
+        "%14, %15};" ::DSV_R16(DSV_IN, 0),
+        "r"(taddr)
+        : "memory");
+#undef DSV_IN
+}
+#undef DSV_R16
+
+__device__ __forceinline__ float ex2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
+__device__ __forceinline__ uint32_t pack2(float a, float b, __nv_bfloat16) {
+    const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&h);
+}
+__device__ __forceinline__ uint32_t pack2(float a, float b, __half) {
+    const __half2 h = __floats2half2_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&h);
+}
+__device__ __forceinline__ void unpack2(uint32_t w, float& a, float& b, __nv_bfloat16) {
+    a = __uint_as_float(w << 16);
+    b = __uint_as_float(w & 0xFFFF0000u);
+}
+__device__ __forceinline__ void unpack2(uint32_t w, float& a, float& b, __half) {
+    const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w));
+    a = f.x;
+    b = f.y;
+}
+
+// 16 bytes global -> shared, zeros where !ok (nothing is read then)
+__device__ __forceinline__ void cp16(uint32_t dst, const void* src, bool ok) {
+    asm volatile("cp.async.cg.shared.global.L2::128B [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(ok ? 16 : 0)
+                 : "memory");
+}
+__device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N> __device__ __forceinline__ void cp_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+
+// bounded wait that also gives up when another warp of the CTA has given up
+__device__ __forceinline__ bool wait_or_abort(uint64_t* bar, uint32_t parity, volatile int* abort) {
+    if (mbar_try_wait(bar, parity)) return true;
+    const uint64_t t0 = globaltimer_ns();
+    for (;;) {
+        if (mbar_try_wait(bar, parity)) return true;
+        if (*abort) return false;
+        if (globaltimer_ns() - t0 > 2000000000ull) {
+            *abort = 1;
+            return false;
+        }
+    }
+}
+
+// 16-byte chunk c of row `row` in a tile of 128-byte-swizzled blocks
+__device__ __forceinline__ uint32_t chunk_at(int row, int c) {
+    return (uint32_t)((c >> 3) * kBlock + row * 128 + (((c ^ row) & 7) << 4));
+}
+
+// ---- the tiles of a CTA, in the order they are loaded -------------------------------------------
+// per segment of n tiles: K0, K1, V0, K2, V1, ..., K(n-1), V(n-2), V(n-1): the order in which the
+// matrix instructions use them (the scores of a tile are computed one tile ahead of its V).
+__device__ __forceinline__ uint32_t item_of_k(uint32_t base, int t) { return base + (t == 0 ? 0 : 2 * t - 1); }
+__device__ __forceinline__ uint32_t item_of_v(uint32_t base, int t, int n) { return base + (t == n - 1 ? 2 * n - 1 : 2 * t + 2); }
+
+// A producer warp's view: which tile comes next, and the slot of the lane's token in it.
+template <int kTokens>  // tokens of a tile that one warp loads (lane l looks after token l % kTokens)
+struct Tiles {
+    Walk w;
+    int i, n;                 // item of the segment, tiles of the segment
+    int token;
+    int cur, prev, ahead;     // slots: the newest tile's, the one before, the one after (-1: none)
+    uint32_t tile;            // tiles begun so far
+    bool is_k;
+
+    __device__ __forceinline__ int slot_of(const KernelArgs& a, int t) const {
+        const int pos = (w.k0 + t) * kTile + token;
+        if (t >= n || pos >= w.r.len) return -1;
+        const int page = pos / a.t.page_size;
+        const int entry = __ldg(a.t.table + (long long)w.b * a.t.table_stride + page);
+        const int pages = (int)(a.t.c.slots / a.t.page_size);
+        if (entry < 0 || entry >= pages) {
+            if (a.t.err) atomicOr(a.t.err, 2u);
+            return -1;
+        }
+        return entry * a.t.page_size + (pos - page * a.t.page_size);
+    }
+    __device__ __forceinline__ void begin(const KernelArgs& a, const Walk& from, int tok) {
+        w = from;
+        token = tok;
+        i = -1;
+        n = w.count();
+        tile = 0;
+        cur = prev = -1;
+        ahead = slot_of(a, 0);
+    }
+    // the next item; false at the end
+    __device__ __forceinline__ bool next(const KernelArgs& a) {
+        if (++i == 2 * n) {
+            if (!w.advance(a)) return false;
+            i = 0;
+            n = w.count();
+            ahead = slot_of(a, 0);
+        }
+        is_k = i == 0 || ((i & 1) && i != 2 * n - 1);
+        if (is_k) {
+            prev = cur;
+            cur = ahead;
+            ahead = slot_of(a, ((i + 1) >> 1) + 1);
+            ++tile;
+        }
+        return true;
+    }
+    // slot of the lane's token in this item
+    __device__ __forceinline__ int slot() const { return is_k || i == 2 * n - 1 ? cur : prev; }
+};
+
+// ---- the kernel ---------------------------------------------------------------------------------
+
+template <typename TQ, bool kFp8, int DP>
+__global__ void __launch_bounds__(threads<kFp8>(), 1) attn_kernel(const __grid_constant__ KernelArgs a) {
+    using L = Layout<DP, kFp8>;
+    using Info = typename InfoOf<kFp8>::type;
+    using TO = typename std::conditional<kFp8, __half, TQ>::type;   // operands of the matrix instructions
+    constexpr int kThreads = threads<kFp8>();
+    constexpr int kProducers = producer_warps<kFp8>();
+    extern __shared__ uint8_t smem_raw[];
+    const int qt = a.qt, stages = L::stages(qt);
+    uint8_t* base = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
+    uint8_t* sq = base;                                    // [qt][kStage]
+    uint8_t* ring = base + qt * L::kStage;                 // [stages][kStage]
+    Shared* sh = reinterpret_cast<Shared*>(ring + stages * L::kStage);
+    Info* info = reinterpret_cast<Info*>(sh + 1);
+    float* row_mul = reinterpret_cast<float*>(info + kInfo);        // e4m3: [128 qt] power of two of a row of q
+    volatile int* abort = &sh->abort;
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const TreeAttnArgs& t = a.t;
+
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+
+    // ---- this CTA's piece of the line of tiles
+    long long total = 0;
+    for (int b0 = 0; b0 < t.batch; b0 += kThreads) {
+        const int b = b0 + tid;
+        long long c = 0;
+        if (b < t.batch) {
+            const Request r = request_of(t, qt, b);
+            c = tiles_of_head(t, qt, r) * t.c.heads;
+            if (t.err && blockIdx.x == 0 && __ldg(t.lens + b) > t.max_pages * t.page_size) atomicOr(t.err, 2u);
+        }
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) c += __shfl_xor_sync(0xffffffffu, c, o);
+        if (lane == 0) sh->scan[warp] = c;
         __syncthreads();
-        if (tid < dim) q[tid] = elem(a.q, r * a.q_token_stride + hq * a.q_head_stride + tid, dtype);
-        const uint64_t bits = a.mask ? (uint64_t)a.mask[r] : 0;
-        float m = -INFINITY, l = 0.f, o = 0.f;
-        for (long long base = 0; base < len; base += kThreads) {
-            __syncthreads();
-            const long long pos = base + tid, j = pos - p0;
-            long long slot = -1;
-            if (pos < len && (j < 0 || (a.mask ? (j < 64 && ((bits >> j) & 1)) : j <= i))) {
-                const long long page = a.table[b * a.table_stride + pos / a.page_size];
-                if (page >= 0 && page < pages)
-                    slot = page * a.page_size + pos % a.page_size;
-                else if (a.err)
-                    atomicOr(a.err, 2u);
-            }
-            float s = -INFINITY;
-            if (slot >= 0) {
-                s = 0.f;
-                const long long k = slot * a.c.slot_stride + h * a.c.head_stride;
-                for (int d = 0; d < dim; ++d) s = fmaf(q[d], elem(a.c.k, k + d, a.c.dtype), s);
-                s *= a.scale * (scaled ? a.c.k_scale[slot * a.c.scale_stride + h] : 1.0f);
-            }
-            float t = s;
-            for (int k = 16; k > 0; k >>= 1) t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, k));
-            if (lane == 0) red[wid] = t;
-            __syncthreads();
-            const float mn = fmaxf(fmaxf(m, fmaxf(red[0], red[1])), fmaxf(red[2], red[3]));
-            const float ref = mn == -INFINITY ? 0.f : mn;
-            at[tid] = slot;
-            p[tid] = slot >= 0 ? expf(s - ref) : 0.f;
-            __syncthreads();
-            const float f = expf(m - ref);
-            l *= f;
-            o *= f;
-            for (int k = 0; k < kThreads; ++k) {
-                const long long sk = at[k];
-                if (sk < 0) continue;
-                l += p[k];
-                if (tid < dim)
-                    o = fmaf(p[k] * (scaled ? a.c.v_scale[sk * a.c.scale_stride + h] : 1.0f),
-                             elem(a.c.v, sk * a.c.slot_stride + h * a.c.head_stride + tid, a.c.dtype), o);
-            }
-            m = mn;
-        }
-        if (tid < dim) {
-            const float x = l == 0.f ? 0.f : o / l;
-            const long long w = r * a.out_token_stride + hq * a.out_head_stride + tid;
-            if (dtype == kBf16)
-                static_cast<__nv_bfloat16*>(a.out)[w] = __float2bfloat16_rn(x);
-            else
-                static_cast<__half*>(a.out)[w] = __float2half_rn(x);
-        }
-        if (tid == 0 && a.lse) a.lse[r * a.q_heads + hq] = l == 0.f ? -INFINITY : m + logf(l);
+        for (int i = 0; i < kThreads / 32; ++i) total += sh->scan[i];
+        __syncthreads();
     }
+    long long want = total / kMinTiles;
+    const int ctas = (int)(want < 1 ? 1 : (want < (long long)gridDim.x ? want : (long long)gridDim.x));
+    if (tid == 0) a.splits[blockIdx.x].valid = 0;
+    if (total == 0 || (int)blockIdx.x >= ctas) return;
+    const long long mine = first_tile(blockIdx.x, total, ctas);
+    const long long count = first_tile(blockIdx.x + 1, total, ctas) - mine;
+    {
+        long long before = 0;
+        for (int b0 = 0; b0 < t.batch; b0 += kThreads) {
+            const int b = b0 + tid;
+            long long c = 0;
+            if (b < t.batch) c = tiles_of_head(t, qt, request_of(t, qt, b)) * t.c.heads;
+            long long s = c;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const long long up = __shfl_up_sync(0xffffffffu, s, o);
+                if (lane >= o) s += up;
+            }
+            if (lane == 31) sh->scan[warp] = s;
+            __syncthreads();
+            long long add = before;
+            for (int i = 0; i < warp; ++i) add += sh->scan[i];
+            for (int i = 0; i < kThreads / 32; ++i) before += sh->scan[i];
+            s += add;
+            if (c > 0 && mine >= s - c && mine < s) {
+                sh->start_b = b;
+                sh->start_in_b = mine - (s - c);
+            }
+            __syncthreads();
+        }
+    }
+
+    if (tid == 0) {
+        for (int s = 0; s < stages; ++s) {
+            mbar_init(&sh->full[s], kProducers);
+            mbar_init(&sh->empty[s], 1);
+        }
+        for (int i = 0; i < kInfo; ++i) mbar_init(&sh->info[i], kProducers);
+        mbar_init(&sh->q_full, 8);
+        for (int i = 0; i < 2; ++i) {
+            mbar_init(&sh->s_full[i], 1);
+            mbar_init(&sh->p_full[i], 4);
+        }
+        mbar_init(&sh->o_full, 1);
+        mbar_init(&sh->joined, 8);
+        mbar_init(&sh->drain, 1);
+        sh->abort = 0;
+        sh->odd[0] = sh->odd[1] = 0;
+        fence_mbar_init();
+    }
+    if (warp == 8) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_u32(&sh->tmem))
+                     : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = sh->tmem;
+    Walk w;
+    w.begin(a, sh->start_b, sh->start_in_b, count);
+    if (tid == 0 && w.k0 > 0) {
+        const long long i0 = mine - w.k0;
+        Split s = {1, w.b, w.h, w.block, cta_of(i0, total, ctas), cta_of(i0 + w.tiles - 1, total, ctas), {0, 0}};
+        a.splits[blockIdx.x] = s;
+    }
+
+    if (warp > 8) {
+        // ---------------- producers ----------------
+        const int pw = warp - 9;
+        constexpr int kTokens = kTile / kProducers;             // tokens of a tile per warp
+        Tiles<kTokens> g;
+        g.begin(a, w, pw * kTokens + (lane & (kTokens - 1)));
+        uint32_t n = 0;
+        bool ok = true;
+        if constexpr (!kFp8) {
+            constexpr int kLanes = DP / 8;                      // lanes of a row (16-byte chunks)
+            const int sub = lane % kLanes, dr = lane / kLanes;
+            const bool live = sub * 8 < t.c.dim;
+            const int lag = qt == 1 ? L::kLag : L::kLag2;
+            uint32_t told = 0;                                  // stages handed over
+            while (ok && g.next(a)) {
+                if (g.is_k) {
+                    const uint32_t valid = __ballot_sync(0xffffffffu, g.cur >= 0);
+                    if (lane == 0) {
+                        Info* inf = info + (g.tile - 1) % kInfo;
+                        inf->valid[pw] = valid;
+                        mbar_arrive(&sh->info[(g.tile - 1) % kInfo]);
+                    }
+                }
+                const uint32_t s = n % stages, ph = (n / stages) & 1u;
+                ok = __all_sync(0xffffffffu, wait_or_abort(&sh->empty[s], ph ^ 1u, abort));
+                if (!ok) break;
+                const uint8_t* src = static_cast<const uint8_t*>(g.is_k ? t.c.k : t.c.v) +
+                                     2 * (g.w.h * t.c.head_stride + sub * 8);
+                const uint32_t dst = smem_u32(ring + s * L::kStage);
+                const int mine_slot = g.slot();
+#pragma unroll
+                for (int i = 0; i < kTokens; i += 32 / kLanes) {
+                    const int tok = i + dr;
+                    const int slot = __shfl_sync(0xffffffffu, mine_slot, tok);
+                    const bool get = live && slot >= 0;
+                    cp16(dst + chunk_at(pw * kTokens + tok, sub), src + (get ? 2 * (slot * t.c.slot_stride) : 0), get);
+                }
+                cp_commit();
+                ++n;
+                if (n > (uint32_t)lag) {
+                    if (qt == 1)
+                        cp_wait<L::kLag>();
+                    else
+                        cp_wait<L::kLag2>();
+                    fence_proxy_async_smem();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(&sh->full[told % stages]);
+                    ++told;
+                }
+            }
+            cp_wait<0>();
+            fence_proxy_async_smem();
+            __syncwarp();
+            for (; told < n; ++told)
+                if (lane == 0) mbar_arrive(&sh->full[told % stages]);
+        } else {
+            constexpr int kLanes = DP / 16;                     // lanes of a row (16 codes each)
+            constexpr int kSteps = kTokens * kLanes / 32;
+            constexpr int kAhead = 3;                           // items whose loads are in flight
+            const int sub = lane % kLanes, dr = lane / kLanes;
+            const bool live = sub * 16 < t.c.dim;
+            uint4 buf[kAhead][kSteps];
+            auto issue = [&](uint4 (&x)[kSteps]) -> bool {
+                if (!g.next(a)) return false;
+                const int mine_slot = g.slot();
+                if (g.is_k) {
+                    Info* inf = info + (g.tile - 1) % kInfo;
+                    const uint32_t valid = __ballot_sync(0xffffffffu, mine_slot >= 0) & ((1u << kTokens) - 1u);
+                    float ks = 0.f, vs = 0.f;
+                    if (mine_slot >= 0) {
+                        const long long at = mine_slot * t.c.scale_stride + g.w.h;
+                        ks = __ldg(t.c.k_scale + at);
+                        vs = __ldg(t.c.v_scale + at);
+                    }
+                    float top = fabsf(vs) < __int_as_float(0x7f800000) ? fabsf(vs) : 0.f;
+#pragma unroll
+                    for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+                    if (lane < kTokens) {
+                        inf->ks[pw * kTokens + lane] = ks * (t.scale * kL2E);
+                        inf->vs[pw * kTokens + lane] = vs;
+                    }
+                    if (lane == 0) {
+                        reinterpret_cast<uint16_t*>(inf->valid)[pw] = (uint16_t)valid;
+                        inf->vmax[pw] = top;
+                    }
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(&sh->info[(g.tile - 1) % kInfo]);
+                }
+                const uint8_t* src = static_cast<const uint8_t*>(g.is_k ? t.c.k : t.c.v) +
+                                     (g.w.h * t.c.head_stride + sub * 16);
+#pragma unroll
+                for (int i = 0; i < kSteps; ++i) {
+                    const int slot = __shfl_sync(0xffffffffu, mine_slot, i * (32 / kLanes) + dr);
+                    x[i] = make_uint4(0, 0, 0, 0);
+                    if (live && slot >= 0) x[i] = __ldg(reinterpret_cast<const uint4*>(src + slot * t.c.slot_stride));
+                }
+                return true;
+            };
+            auto finish = [&](const uint4 (&x)[kSteps]) {
+                const uint32_t s = n % stages, ph = (n / stages) & 1u;
+                ok = __all_sync(0xffffffffu, wait_or_abort(&sh->empty[s], ph ^ 1u, abort));
+                if (!ok) return;
+                uint8_t* dst = ring + s * L::kStage;
+#pragma unroll
+                for (int i = 0; i < kSteps; ++i) {
+                    const int row = pw * kTokens + i * (32 / kLanes) + dr;
+                    const uint32_t c[4] = {x[i].x, x[i].y, x[i].z, x[i].w};
+                    uint32_t o[8];
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) {
+                        const __half2_raw h =
+                            __nv_cvt_fp8x2_to_halfraw2((uint16_t)(c[j >> 1] >> (16 * (j & 1))), __NV_E4M3);
+                        o[j] = (uint32_t)h.x | ((uint32_t)h.y << 16);
+                    }
+                    *reinterpret_cast<uint4*>(dst + chunk_at(row, 2 * sub)) = make_uint4(o[0], o[1], o[2], o[3]);
+                    *reinterpret_cast<uint4*>(dst + chunk_at(row, 2 * sub + 1)) = make_uint4(o[4], o[5], o[6], o[7]);
+                }
+                fence_proxy_async_smem();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&sh->full[s]);
+                ++n;
+            };
+            int held = 0;                                       // items loaded and not handed over
+            bool more = true;
+#pragma unroll
+            for (int i = 0; i < kAhead; ++i)
+                if (more && (more = issue(buf[i]))) ++held;
+            while (ok && held > 0) {
+#pragma unroll
+                for (int i = 0; i < kAhead; ++i) {
+                    if (ok && held > 0) {
+                        finish(buf[i]);
+                        --held;
+                        if (ok && more && (more = issue(buf[i]))) ++held;
+                    }
+                }
+            }
+        }
+    } else if (warp == 8) {
+        // ---------------- MMA issuer ----------------
+        if (lane == 0) {
+            constexpr uint32_t kFormat = std::is_same<TO, __nv_bfloat16>::value ? 1u : 0u;
+            constexpr uint32_t kCommon = (1u << 4) | (kFormat << 7) | (kFormat << 10) | ((uint32_t)(kRows >> 4) << 24);
+            constexpr uint32_t kIdescS = kCommon | ((uint32_t)(kTile >> 3) << 17);
+            const uint32_t idesc_o = kCommon | (1u << 16) | ((uint32_t)(t.c.dim >> 3) << 17);  // B: MN-major
+            const int ksteps = t.c.dim / 16;
+            const uint32_t q0 = smem_u32(sq), r0 = smem_u32(ring);
+            uint32_t item = 0, seg = 0, su[2] = {0, 0};  // items before the segment, segments, units per stream
+            bool ok = true;
+            do {
+                const bool both = !w.shared_rows(qt);    // both streams use every tile
+                const int nt = w.count(), units = both ? 2 * nt : nt;
+                ok = wait_or_abort(&sh->q_full, seg & 1u, abort);
+                tc_fence_after();
+                auto scores = [&](int u) {
+                    const int s = u & 1, tl = both ? u >> 1 : u;
+                    const uint32_t it = item_of_k(item, tl), st = it % stages;
+                    if (!both || s == 0) {
+                        ok = wait_or_abort(&sh->full[st], (it / stages) & 1u, abort);
+                        if (!ok) return;
+                        fence_proxy_async_smem();
+                        tc_fence_after();
+                    }
+                    const uint32_t qa = q0 + (both ? s * L::kStage : 0), kb = r0 + st * L::kStage;
+                    for (int k = 0; k < ksteps; ++k) {
+                        const uint32_t off = (k >> 2) * kBlock + (k & 3) * 32;
+                        mma_ss(tmem + s * kTile, smem_desc(qa + off, 16), smem_desc(kb + off, 16), kIdescS, k != 0);
+                    }
+                    if (!both || s == 1) mma_commit(&sh->empty[st]);
+                    mma_commit(&sh->s_full[s]);
+                };
+                for (int u = 0; ok && u < 2 && u < units; ++u) scores(u);
+                for (int u = 0; ok && u < units; ++u) {
+                    const int s = u & 1, tl = both ? u >> 1 : u;
+                    ok = wait_or_abort(&sh->p_full[s], su[s] & 1u, abort);
+                    if (!ok) break;
+                    ++su[s];
+                    const uint32_t it = item_of_v(item, tl, nt), st = it % stages;
+                    if (!both || s == 0) {
+                        ok = wait_or_abort(&sh->full[st], (it / stages) & 1u, abort);
+                        if (!ok) break;
+                        fence_proxy_async_smem();
+                    }
+                    tc_fence_after();
+                    const uint32_t vb = r0 + st * L::kStage;
+#pragma unroll
+                    for (int k = 0; k < kTile / 16; ++k)
+                        mma_ts(tmem + 256 + s * 128, tmem + s * kTile + k * 8, smem_desc(vb + k * 2048, kBlock), idesc_o,
+                               u >= 2 || k != 0);
+                    if (!both || s == 1) mma_commit(&sh->empty[st]);
+                    if (u + 2 < units) scores(u + 2);
+                }
+                if (ok) mma_commit(&sh->o_full);
+                item += 2 * nt;
+                ++seg;
+            } while (ok && w.advance(a));
+            // every instruction issued here is done before TMEM is released
+            mma_commit(&sh->drain);
+            if (!mbar_wait_bounded(&sh->drain, 0)) *abort = 1;
+        }
+        __syncwarp();
+    } else {
+        // ---------------- softmax and epilogue: one row per thread ----------------
+        const int s = warp >> 2, quarter = warp & 3, row = quarter * 32 + lane;
+        const uint32_t lanes = (uint32_t)(quarter * 32) << 16;
+        const uint32_t ts = tmem + lanes + s * kTile, to = tmem + lanes + 256 + s * 128;
+        uint32_t seg = 0, su = 0, tile0 = 0, item = 0;
+        bool ok = true;
+        do {
+            const bool both = !w.shared_rows(qt);
+            const int nt = w.count(), nrows = w.rows(qt), row0 = w.first_row(qt);
+            const int my = both ? s * kRows + row : row;        // row of the block
+            // ---- Q into shared memory
+            {
+                constexpr int kLanes = DP / 8;
+                const int sub = tid % kLanes, tiles_q = both ? 2 : 1;
+                const int filled = (nrows + 31) & ~31;          // whole warps of rows: zeros past the last
+#pragma unroll 4
+                for (int r = tid / kLanes; r < tiles_q * kRows; r += kSoftmaxThreads / kLanes) {
+                    uint4 x = make_uint4(0, 0, 0, 0);
+                    if (r < nrows && sub * 8 < t.c.dim) {
+                        const int i = (row0 + r) / t.group, gq = (row0 + r) - i * t.group;
+                        x = __ldg(reinterpret_cast<const uint4*>(
+                            static_cast<const TQ*>(t.q) + (long long)(w.r.lo + i) * t.q_token_stride +
+                            (long long)(w.h * t.group + gq) * t.q_head_stride + sub * 8));
+                    }
+                    if constexpr (kFp8) {
+                        float f[8];
+                        unpack2(x.x, f[0], f[1], TQ());
+                        unpack2(x.y, f[2], f[3], TQ());
+                        unpack2(x.z, f[4], f[5], TQ());
+                        unpack2(x.w, f[6], f[7], TQ());
+                        float m = 0.f;
+#pragma unroll
+                        for (int i = 0; i < 8; ++i) m = fmaxf(m, fabsf(f[i]));
+#pragma unroll
+                        for (int o = kLanes / 2; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+                        // a power of two that brings the row's largest value to [2^13, 2^14): products stay
+                        // exact, and values down to 2^-37 of the largest keep a place in fp16
+                        int e = (int)(__float_as_uint(m) >> 23) - 127;
+                        e = m > 0.f && e < 128 ? max(e, -100) : 13;
+                        const float up = __uint_as_float((uint32_t)(13 - e + 127) << 23);
+                        if (sub == 0) row_mul[r] = __uint_as_float((uint32_t)(e - 13 + 127) << 23);
+                        x = make_uint4(pack2(f[0] * up, f[1] * up, __half()), pack2(f[2] * up, f[3] * up, __half()),
+                                       pack2(f[4] * up, f[5] * up, __half()), pack2(f[6] * up, f[7] * up, __half()));
+                    }
+                    if (r < filled)
+                        *reinterpret_cast<uint4*>(sq + (r >> 7) * L::kStage + chunk_at(r & 127, sub)) = x;
+                }
+                fence_proxy_async_smem();
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&sh->q_full);
+                if constexpr (kFp8) {
+                    // row_mul comes from all eight warps
+                    ok = ok && wait_or_abort(&sh->q_full, seg & 1u, abort);
+                    ok = __all_sync(0xffffffffu, ok);
+                }
+            }
+            const bool any_row = (both ? s * kRows : 0) + quarter * 32 < nrows;  // this warp has rows
+            const float cm = kFp8 ? row_mul[my] : t.scale * kL2E;
+            int token = 0;                                      // this row's drafted token
+            uint64_t bits = 0;
+            if (my < nrows) {
+                token = (row0 + my) / t.group;
+                if (t.mask) bits = (uint64_t)__ldg(reinterpret_cast<const long long*>(t.mask) + w.r.lo + token);
+            }
+            float ref = -INFINITY, sum = 0.f, vmax = 0.f;
+            const int step = both ? 1 : 2;
+            for (int tl = both ? 0 : s; ok && tl < nt; tl += step, ++su) {
+                const uint32_t ti = tile0 + tl;
+                const Info* inf = info + ti % kInfo;
+                ok = wait_or_abort(&sh->info[ti % kInfo], (ti / kInfo) & 1u, abort) &&
+                     wait_or_abort(&sh->s_full[s], su & 1u, abort);
+                ok = __all_sync(0xffffffffu, ok);
+                if (!ok) break;
+                tc_fence_after();
+                const int kb = (w.k0 + tl) * kTile;             // first position of the tile
+                const bool drafted = kb + kTile > w.r.p0;
+                if (any_row) {
+                    uint32_t vis[4] = {~0u, ~0u, ~0u, ~0u};
+                    const uint4 valid = *reinterpret_cast<const uint4*>(inf->valid);
+                    const bool masked = drafted || (valid.x & valid.y & valid.z & valid.w) != ~0u;
+                    if (masked) {
+                        const uint32_t vw[4] = {valid.x, valid.y, valid.z, valid.w};
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            const int pos = kb + 32 * i;
+                            const int n = (t.mask ? w.r.p0 : w.r.p0 + token + 1) - pos;
+                            uint32_t m = n >= 32 ? ~0u : (n <= 0 ? 0u : (1u << n) - 1u);
+                            if (t.mask) {
+                                const int d = pos - w.r.p0;     // drafted token of the word's first bit
+                                if (d >= 0)
+                                    m |= d < 64 ? (uint32_t)(bits >> d) : 0u;
+                                else if (d > -32)
+                                    m |= (uint32_t)(bits << -d);
+                            }
+                            vis[i] = m & vw[i];
+                        }
+                    }
+                    // the row's largest score of this tile
+                    float mx = -INFINITY;
+#pragma unroll
+                    for (int c = 0; c < 4; ++c) {
+                        uint32_t v[32];
+                        tmem_ld32(ts + c * 32, v);
+                        tmem_wait_ld();
+                        if constexpr (kFp8) {
+#pragma unroll
+                            for (int j = 0; j < 32; j += 4) {
+                                const float4 k4 = *reinterpret_cast<const float4*>(&inf->ks[c * 32 + j]);
+                                v[j] = __float_as_uint(__uint_as_float(v[j]) * k4.x);
+                                v[j + 1] = __float_as_uint(__uint_as_float(v[j + 1]) * k4.y);
+                                v[j + 2] = __float_as_uint(__uint_as_float(v[j + 2]) * k4.z);
+                                v[j + 3] = __float_as_uint(__uint_as_float(v[j + 3]) * k4.w);
+                            }
+                        }
+                        if (masked) {
+#pragma unroll
+                            for (int j = 0; j < 32; ++j)
+                                if (!((vis[c] >> j) & 1u)) v[j] = 0xFF800000u;
+                        }
+#pragma unroll
+                        for (int j = 0; j < 32; ++j) mx = fmaxf(mx, __uint_as_float(v[j]));
+                    }
+                    float target = mx * cm;
+                    if constexpr (kFp8) {
+#pragma unroll
+                        for (int i = 0; i < 8; ++i) vmax = fmaxf(vmax, inf->vmax[i]);
+                        // 2^ev is the first power of two above the V scales so far
+                        const int ev = max(-90, min(120, (int)(__float_as_uint(vmax) >> 23) - 126));
+                        target += (float)(ev - 6);
+                    } else if constexpr (std::is_same<TO, __half>::value) {
+                        target -= 6.0f;
+                    }
+                    if (__any_sync(0xffffffffu, target > ref + kSlack)) {
+                        const float to_ref = fmaxf(ref, target);
+                        if (tl >= step) {                       // the accumulator holds something
+                            const float f = ref == -INFINITY ? 1.0f : ex2(ref - to_ref);
+                            sum *= f;
+#pragma unroll 1
+                            for (int c = 0; c < t.c.dim; c += 32) {
+                                uint32_t v[32];
+                                tmem_ld32(to + c, v);
+                                tmem_wait_ld();
+#pragma unroll
+                                for (int j = 0; j < 32; ++j) v[j] = __float_as_uint(__uint_as_float(v[j]) * f);
+                                tmem_st32(to + c, v);
+                            }
+                        }
+                        ref = to_ref;
+                    }
+                    const float nref = ref == -INFINITY ? 0.f : -ref;
+                    float part[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                    for (int c = 0; c < 4; ++c) {
+                        uint32_t v[32], p[16];
+                        tmem_ld32(ts + c * 32, v);
+                        tmem_wait_ld();
+#pragma unroll
+                        for (int j = 0; j < 32; j += 4) {
+                            float x[4] = {__uint_as_float(v[j]), __uint_as_float(v[j + 1]), __uint_as_float(v[j + 2]),
+                                          __uint_as_float(v[j + 3])};
+                            if constexpr (kFp8) {
+                                const float4 k4 = *reinterpret_cast<const float4*>(&inf->ks[c * 32 + j]);
+                                x[0] *= k4.x;
+                                x[1] *= k4.y;
+                                x[2] *= k4.z;
+                                x[3] *= k4.w;
+                            }
+#pragma unroll
+                            for (int i = 0; i < 4; ++i) {
+                                x[i] = ex2(fmaf(x[i], cm, nref));
+                                if (masked && !((vis[c] >> (j + i)) & 1u)) x[i] = 0.f;
+                                part[i] += x[i];
+                            }
+                            if constexpr (kFp8) {
+                                const float4 v4 = *reinterpret_cast<const float4*>(&inf->vs[c * 32 + j]);
+                                x[0] = masked && !((vis[c] >> j) & 1u) ? 0.f : x[0] * v4.x;
+                                x[1] = masked && !((vis[c] >> (j + 1)) & 1u) ? 0.f : x[1] * v4.y;
+                                x[2] = masked && !((vis[c] >> (j + 2)) & 1u) ? 0.f : x[2] * v4.z;
+                                x[3] = masked && !((vis[c] >> (j + 3)) & 1u) ? 0.f : x[3] * v4.w;
+                            }
+                            p[j / 2] = pack2(x[0], x[1], TO());
+                            p[j / 2 + 1] = pack2(x[2], x[3], TO());
+                        }
+                        tmem_st16(ts + c * 16, p);              // over scores that have been read
+                    }
+                    sum += (part[0] + part[1]) + (part[2] + part[3]);
+                }
+                if (drafted) {
+                    // V elements of drafted tokens that are not finite: zeroed for the matrix
+                    // instructions, added to the rows that see them at the end
+                    const uint32_t it = item_of_v(item, tl, nt), st = it % stages;
+                    ok = __all_sync(0xffffffffu, wait_or_abort(&sh->full[st], (it / stages) & 1u, abort));
+                    if (!ok) break;
+                    if (kb + row >= w.r.p0 && kb + row < w.r.len) {
+                        uint8_t* v = ring + st * L::kStage;
+                        constexpr uint32_t kExp = std::is_same<TO, __nv_bfloat16>::value ? 0x7F80u : 0x7C00u;
+                        bool found = false;
+                        for (int c = 0; c < t.c.dim / 8; ++c) {
+                            uint4* at = reinterpret_cast<uint4*>(v + chunk_at(row, c));
+                            uint4 x = *at;
+                            uint32_t* xw = &x.x;
+                            bool here = false;
+#pragma unroll
+                            for (int i = 0; i < 4; ++i) {
+                                if ((xw[i] & kExp) == kExp) {
+                                    xw[i] &= 0xFFFF0000u;
+                                    here = true;
+                                }
+                                if ((xw[i] & (kExp << 16)) == (kExp << 16)) {
+                                    xw[i] &= 0xFFFFu;
+                                    here = true;
+                                }
+                            }
+                            if (here) *at = x;
+                            found |= here;
+                        }
+                        if (found) *(volatile int*)&sh->odd[seg & 1] = 1;
+                    }
+                    fence_proxy_async_smem();
+                }
+                tmem_wait_st();
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&sh->p_full[s]);
+            }
+            // ---- the segment's result
+            if (tid == 0) sh->odd[(seg + 1) & 1] = 0;
+            ok = ok && wait_or_abort(&sh->o_full, seg & 1u, abort);
+            ok = __all_sync(0xffffffffu, ok);
+            if (!ok) break;
+            tc_fence_after();
+            float2* swap = reinterpret_cast<float2*>(sq);       // [2][128]: Q has been used
+            if (!both) swap[s * kRows + row] = make_float2(ref, sum);
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&sh->joined);
+            ok = __all_sync(0xffffffffu, wait_or_abort(&sh->joined, 0u, abort));
+            if (!ok) break;
+            float f0 = 1.f, f1 = 0.f;                           // factors of the two accumulators
+            if (!both && nt > 1) {
+                const float2 x = swap[row], y = swap[kRows + row];
+                const float top = fmaxf(x.x, y.x);
+                f0 = top == -INFINITY ? 1.f : ex2(x.x - top);
+                f1 = top == -INFINITY ? 1.f : ex2(y.x - top);
+                ref = top;
+                sum = x.y * f0 + y.y * f1;
+            } else if (!both) {
+                const float2 x = swap[row];
+                ref = x.x;
+                sum = x.y;
+            }
+            const bool odd = *(volatile int*)&sh->odd[seg & 1] != 0;
+            // the exchange area is Q's: nobody overwrites it before everyone has read it
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&sh->joined);
+            ok = __all_sync(0xffffffffu, wait_or_abort(&sh->joined, 1u, abort));
+            if (!ok) break;
+            if (any_row) {
+                const bool whole = w.k0 == 0 && w.k1 == w.tiles;
+                const int slot = 2 * blockIdx.x + (w.k0 == 0 ? 1 : 0);
+                const int gq = (row0 + my) - token * t.group;
+                const long long qrow = w.r.lo + token;
+                const int hq = w.h * t.group + gq;
+                TQ* out = static_cast<TQ*>(t.out) + qrow * t.out_token_stride + hq * t.out_head_stride;
+                float* po = a.part_o + ((long long)slot * (kRows * qt) + my) * DP;
+                const float inv = sum == 0.f ? 0.f : 1.0f / sum;
+                const int c0 = both ? 0 : s * (DP / 2), c1 = both ? DP : c0 + DP / 2;
+#pragma unroll 1
+                for (int c = c0; c < c1 && c < t.c.dim; c += 32) {
+                    uint32_t v[32];
+                    tmem_ld32(tmem + lanes + 256 + (both ? s * 128 : 0) + c, v);
+                    tmem_wait_ld();
+                    if (!both && nt > 1) {
+                        uint32_t y[32];
+                        tmem_ld32(tmem + lanes + 256 + 128 + c, y);
+                        tmem_wait_ld();
+#pragma unroll
+                        for (int j = 0; j < 32; ++j)
+                            v[j] = __float_as_uint(__uint_as_float(v[j]) * f0 + __uint_as_float(y[j]) * f1);
+                    }
+                    if (my < nrows) {
+                        if (odd) {
+                            const int pages = (int)(t.c.slots / t.page_size);
+                            const int n0 = max(0, w.k0 * kTile - w.r.p0), n1 = min(w.r.len, w.k1 * kTile) - w.r.p0;
+                            for (int j = max(n0, -w.r.p0); j < n1; ++j) {
+                                if (!(t.mask ? j < 64 && ((bits >> j) & 1) : j <= token)) continue;
+                                const int pos = w.r.p0 + j, page = __ldg(t.table + (long long)w.b * t.table_stride + pos / t.page_size);
+                                if (page < 0 || page >= pages) continue;
+                                const long long at = (long long)(page * t.page_size + pos % t.page_size) * t.c.slot_stride +
+                                                     (long long)w.h * t.c.head_stride + c;
+#pragma unroll
+                                for (int d = 0; d < 32; ++d) {
+                                    if (c + d >= t.c.dim) break;
+                                    float x;
+                                    if constexpr (kFp8) {
+                                        const uint8_t q8 = static_cast<const uint8_t*>(t.c.v)[at + d];
+                                        x = (q8 & 0x7F) == 0x7F ? __int_as_float(0x7fffffff) : 0.f;
+                                    } else {
+                                        x = (float)static_cast<const TQ*>(t.c.v)[at + d];
+                                        if (fabsf(x) < __int_as_float(0x7f800000)) x = 0.f;
+                                    }
+                                    v[d] = __float_as_uint(__uint_as_float(v[d]) + x);
+                                }
+                            }
+                        }
+                        if (whole) {
+#pragma unroll
+                            for (int j = 0; j < 32; j += 8) {
+                                if (c + j >= t.c.dim) break;
+                                uint32_t p[4];
+#pragma unroll
+                                for (int i = 0; i < 4; ++i)
+                                    p[i] = pack2(__uint_as_float(v[j + 2 * i]) * inv, __uint_as_float(v[j + 2 * i + 1]) * inv, TQ());
+                                *reinterpret_cast<uint4*>(out + c + j) = make_uint4(p[0], p[1], p[2], p[3]);
+                            }
+                        } else {
+#pragma unroll
+                            for (int j = 0; j < 32; j += 4)
+                                *reinterpret_cast<uint4*>(po + c + j) = make_uint4(v[j], v[j + 1], v[j + 2], v[j + 3]);
+                        }
+                    }
+                }
+                if (my < nrows && (both || s == 0)) {
+                    if (!whole)
+                        a.part_ml[(long long)slot * (kRows * qt) + my] = make_float2(ref, sum);
+                    else if (t.lse)
+                        t.lse[qrow * t.q_heads + hq] = sum == 0.f ? -INFINITY : (ref + log2f(sum)) * kLn2;
+                }
+            }
+            tc_fence_before();
+            tile0 += nt;
+            item += 2 * nt;
+            ++seg;
+        } while (w.advance(a));
+    }
+
+    __syncthreads();
+    if (tid == 0 && *abort && t.err) atomicOr(t.err, 4u);
+    if (warp == 8) {
+        tc_fence_after();
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem) : "memory");
+    }
+}
+
+// ---- joining the parts of an item ------------------------------------------------------------
+// CTAs first..last hold parts of an item; the blocks first + 1..last share its rows, a warp a row.
+constexpr int kCombineThreads = 128;
+
+template <typename TQ, int DP>
+__global__ void __launch_bounds__(kCombineThreads) combine_kernel(const __grid_constant__ KernelArgs a) {
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    const Split sp = a.splits[blockIdx.x];
+    if (!sp.valid) return;
+    const TreeAttnArgs& t = a.t;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const Request r = request_of(t, a.qt, sp.b);
+    const int row0 = sp.block * kRows * a.qt, nrows = min(r.rows - row0, kRows * a.qt);
+    const int parts = sp.last - sp.first + 1, per = kRows * a.qt;
+    constexpr int kCols = DP / 32;
+    constexpr int kWarps = kCombineThreads / 32;
+    for (int row = ((int)blockIdx.x - sp.first - 1) * kWarps + warp; row < nrows; row += (parts - 1) * kWarps) {
+        float top = -INFINITY;
+        for (int p = lane; p < parts; p += 32) {
+            const int slot = 2 * (sp.first + p) + (p == 0);
+            top = fmaxf(top, __ldcg(&a.part_ml[(long long)slot * per + row]).x);
+        }
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+        float sum = 0.f, acc[kCols];
+#pragma unroll
+        for (int i = 0; i < kCols; ++i) acc[i] = 0.f;
+#pragma unroll 4
+        for (int p = 0; p < parts; ++p) {
+            const long long at = (long long)(2 * (sp.first + p) + (p == 0)) * per + row;
+            const float2 ml = __ldcg(&a.part_ml[at]);
+            const float f = top == -INFINITY ? 1.f : ex2(ml.x - top);
+            sum += ml.y * f;
+            float x[kCols];
+            if constexpr (kCols == 4) {
+                const float4 v = __ldcg(reinterpret_cast<const float4*>(a.part_o + at * DP) + lane);
+                x[0] = v.x;
+                x[1] = v.y;
+                x[2] = v.z;
+                x[3] = v.w;
+            } else {
+                const float2 v = __ldcg(reinterpret_cast<const float2*>(a.part_o + at * DP) + lane);
+                x[0] = v.x;
+                x[1] = v.y;
+            }
+#pragma unroll
+            for (int i = 0; i < kCols; ++i) acc[i] = fmaf(x[i], f, acc[i]);
+        }
+        const int token = (row0 + row) / t.group;
+        const long long qrow = r.lo + token;
+        const int hq = sp.h * t.group + (row0 + row) - token * t.group;
+        const float inv = sum == 0.f ? 0.f : 1.0f / sum;
+        TQ* out = static_cast<TQ*>(t.out) + qrow * t.out_token_stride + hq * t.out_head_stride + lane * kCols;
+        if (lane * kCols < t.c.dim) {
+#pragma unroll
+            for (int i = 0; i < kCols; i += 2)
+                *reinterpret_cast<uint32_t*>(out + i) = pack2(acc[i] * inv, acc[i + 1] * inv, TQ());
+        }
+        if (lane == 0 && t.lse)
+            t.lse[qrow * t.q_heads + hq] = sum == 0.f ? -INFINITY : (top + log2f(sum)) * kLn2;
+    }
+}
+
+// ---- host side ---------------------------------------------------------------------------------
+
+int q_tiles(int group, int width) { return (long long)group * width > kRows ? 2 : 1; }
+int padded_dim(int dim) { return dim <= 64 ? 64 : 128; }
+
+constexpr size_t kSplitBytes = sizeof(Split) * kMaxCtas;
+constexpr size_t kMlBytes(int qt) { return sizeof(float2) * 2 * kMaxCtas * kRows * qt; }
+
+template <typename TQ, bool kFp8, int DP>
+int launch(const KernelArgs& a, int sms, cudaStream_t st) {
+    using L = Layout<DP, kFp8>;
+    auto kern = attn_kernel<TQ, kFp8, DP>;
+    const size_t smem = L::smem(a.qt);
+    if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess)
+        return kLaunchFailed;
+    const int grid = sms < kMaxCtas ? sms : kMaxCtas;
+    kern<<<grid, threads<kFp8>(), smem, st>>>(a);
+    if (cudaGetLastError() != cudaSuccess) return kLaunchFailed;
+    // items of one tile are never cut
+    if ((long long)a.t.max_pages * a.t.page_size <= kTile) return kOk;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(grid);
+    cfg.blockDim = dim3(kCombineThreads);
+    cfg.stream = st;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    return cudaLaunchKernelEx(&cfg, combine_kernel<TQ, DP>, a) == cudaSuccess ? kOk : kLaunchFailed;
 }
 
 }  // namespace attn
 
-size_t tree_attn_workspace_bytes(int, int, int, int) { return 0; }
+size_t tree_attn_workspace_bytes(int q_heads, int kv_heads, int dim, int width) {
+    const int qt = attn::q_tiles(q_heads / kv_heads, width);
+    return attn::kSplitBytes + attn::kMlBytes(qt) +
+           sizeof(float) * 2 * attn::kMaxCtas * attn::kRows * qt * attn::padded_dim(dim);
+}
 
-int launch_tree_attn(const TreeAttnArgs& a, int dtype, cudaStream_t st) {
-    attn::rows_kernel<<<dim3(a.q_heads, a.batch), attn::kThreads, 0, st>>>(a, dtype);
-    return cudaGetLastError() == cudaSuccess ? kOk : kLaunchFailed;
+int launch_tree_attn(const TreeAttnArgs& t, int dtype, cudaStream_t st) {
+    using namespace attn;
+    KernelArgs a = {};
+    a.t = t;
+    a.qt = q_tiles(t.group, t.width);
+    char* ws = static_cast<char*>(t.ws);
+    a.splits = reinterpret_cast<Split*>(ws);
+    a.part_ml = reinterpret_cast<float2*>(ws + kSplitBytes);
+    a.part_o = reinterpret_cast<float*>(ws + kSplitBytes + kMlBytes(a.qt));
+    int dev = 0, sms = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess ||
+        cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess)
+        return kLaunchFailed;
+    const bool fp8 = t.c.dtype == kE4m3, wide = padded_dim(t.c.dim) == 128;
+    if (dtype == kBf16) {
+        if (fp8) return wide ? launch<__nv_bfloat16, true, 128>(a, sms, st) : launch<__nv_bfloat16, true, 64>(a, sms, st);
+        return wide ? launch<__nv_bfloat16, false, 128>(a, sms, st) : launch<__nv_bfloat16, false, 64>(a, sms, st);
+    }
+    if (fp8) return wide ? launch<__half, true, 128>(a, sms, st) : launch<__half, true, 64>(a, sms, st);
+    return wide ? launch<__half, false, 128>(a, sms, st) : launch<__half, false, 64>(a, sms, st);
 }
 
 }  // namespace dsv
