@@ -81,7 +81,8 @@ def tree_attention(q, k_cache, v_cache, page_table, kv_lens, *, page_size=1, q_i
     rows, q_heads, dim = q.shape
     dtype = _DTYPES[q.dtype]
     _check(dim == c.dim and dim <= MAX_DIM, f"q and the cache must have one dim, at most {MAX_DIM}")
-    _check(q_heads >= 1 and q_heads % c.heads == 0, "q_heads must be a multiple of the cache's heads")
+    _check(q_heads >= 1 and q_heads % c.heads == 0 and q_heads <= 4096 * c.heads,
+           "q_heads must be a multiple of the cache's heads, at most 4096 of them each")
     _check(c.dtype == 3 or c.dtype == dtype, "the cache must have q's type or be e4m3")
     _check(page_table.dim() == 2 and page_table.dtype == torch.int32, "page_table must be int32 [requests, pages]")
     batch, pages = page_table.shape

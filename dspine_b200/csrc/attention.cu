@@ -15,9 +15,10 @@
 //                   is read once for all of them.  The tiles of 128 keys of all (request, KV head,
 //                   row block) items form one line that is cut into equal pieces, one per CTA:
 //                   every SM streams the same number of tiles however ragged the lengths are.
-//                     warps 0-7    two softmax warpgroups, one TMEM lane (row) per thread
-//                     warp 8       TMEM allocation and the MMA issuer
-//                     warps 9..    producers: K and V rows of a tile, slot by slot, into a ring of
+//                     warps 0-7    two softmax warpgroups, one TMEM lane (row) per thread, its 128
+//                                  scores in registers
+//                     warp 8       TMEM allocation and the MMA issuer (its warpgroup is else idle)
+//                     warps 12-15  producers: K and V rows of a tile, slot by slot, into a ring of
 //                                  128-byte-swizzled shared-memory stages
 //                   S = Q K^T (kind::f16, both operands in shared memory) and O += P V (P from
 //                   TMEM, written over S; V as a matrix with rows of keys, "MN-major").
@@ -67,13 +68,13 @@ constexpr float kSlack = 8.0f;             // log2 by which a maximum may outgro
 constexpr float kL2E = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
 
-template <bool kFp8> constexpr int producer_warps() { return kFp8 ? 8 : 4; }
-template <bool kFp8> constexpr int threads() { return kSoftmaxThreads + 32 + 32 * producer_warps<kFp8>(); }
+constexpr int kProducers = 4;              // producer warps
+constexpr int kThreads = 512;              // four warpgroups: softmax, softmax, MMA issuer, producers
 
 // one slot of the tile ring beside the stages
 struct TileInfo {
     uint32_t valid[4];        // positions of the tile that exist and can be read
-    float vmax[8];            // e4m3: largest finite V scale, per producer warp
+    float vmax[kProducers];   // e4m3: largest finite V scale, per producer warp
     float ks[kTile];          // e4m3: K scale x scale x log2(e)
     float vs[kTile];          // e4m3: V scale
 };
@@ -91,7 +92,7 @@ struct alignas(16) Shared {
     uint64_t info[kInfo];        // TileInfo written
     uint64_t q_full;             // Q of the segment in shared memory, last segment's TMEM read
     uint64_t s_full[2];          // scores of a stream's tile in TMEM
-    uint64_t p_full[2];          // weights of a stream's tile in TMEM
+    uint64_t p_full[2][2];       // weights of a stream's tile in TMEM: its first and second 64 keys
     uint64_t o_full;             // the segment's accumulators are complete
     uint64_t joined;             // both warpgroups have written what the other reads
     uint64_t drain;
@@ -109,11 +110,6 @@ template <int DP, bool kFp8> struct Layout {
     static __host__ __device__ constexpr int stages(int qt) {
         return DP == 128 ? (kFp8 ? 6 - qt : 7 - qt) : (kFp8 ? 8 : 12);
     }
-    // stages whose copies are in flight before the oldest is waited for.  At least two below the
-    // ring: a K tile of two streams is freed only after the V tile behind it has been handed over.
-    static constexpr int kLag = DP == 128 ? 4 : 10;         // one Q tile
-    static constexpr int kLag2 = DP == 128 ? 3 : 10;        // two Q tiles
-    static_assert(kFp8 || (kLag + 2 <= stages(1) && kLag2 + 2 <= stages(2)), "the ring would lock");
     static constexpr size_t info_bytes = sizeof(typename InfoOf<kFp8>::type) * kInfo;
     static constexpr size_t smem(int qt) {
         return (size_t)(qt + stages(qt)) * kStage + sizeof(Shared) + info_bytes + (kFp8 ? 1024 : 0) + 1024;
@@ -139,7 +135,8 @@ struct KernelArgs {
     int qt;                 // Q tiles of a row block
     Split* splits;          // [kMaxCtas]
     float2* part_ml;        // [2 * kMaxCtas][128 qt] (reference, sum)
-    float* part_o;          // [2 * kMaxCtas][128 qt][DP], not normalised
+    float4* part_o;         // [2 * kMaxCtas][DP / 4][128 qt], not normalised: columns in fours, rows
+                            // adjacent, so that the threads of a warp (a row each) write in one run
 };
 
 // ---- requests, items, segments ---------------------------------------------------------------
@@ -252,15 +249,19 @@ struct Walk {
 
 // ---- PTX helpers ------------------------------------------------------------------------------
 
-__device__ __forceinline__ uint64_t smem_desc(uint32_t saddr, uint32_t lead_bytes) {
-    uint64_t d = 0;
-    d |= (uint64_t)((saddr >> 4) & 0x3FFFu);
-    d |= (uint64_t)((lead_bytes >> 4) & 0x3FFFu) << 16;
-    d |= (uint64_t)(1024u >> 4) << 32;              // 8 rows of 128 bytes
-    d |= (uint64_t)1u << 46;                        // descriptor version (sm100)
-    d |= (uint64_t)2u << 61;                        // 128-byte swizzle
-    return d;
+// Order between the threads' writes to shared memory and the matrix instructions' reads (another
+// proxy): the issuing thread runs the proxy fence, after it has seen the writers' barrier.  A fence
+// in the producers would do as well, but there it waits for their loads in flight: measured, it
+// left one tile in flight (64x1 bf16 455 us).
+
+// shared-memory matrix descriptors: the low word holds the address and the distance between
+// 128-byte column blocks (of an MN-major operand), both in 16-byte units, and takes offsets by
+// addition; the high word is the same for all: 8 rows 1024 bytes apart, sm100 version, 128-byte swizzle
+constexpr uint32_t kDescHigh = (1024u >> 4) | (1u << 14) | (2u << 29);
+__device__ __forceinline__ uint32_t desc_low(uint32_t saddr, uint32_t lead_bytes) {
+    return ((saddr >> 4) & 0x3FFFu) | ((lead_bytes >> 4) << 16);
 }
+__device__ __forceinline__ uint64_t desc(uint32_t low) { return ((uint64_t)kDescHigh << 32) | low; }
 
 __device__ __forceinline__ void tc_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void tc_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
@@ -301,7 +302,12 @@ __device__ __forceinline__ void tmem_ld32(uint32_t taddr, uint32_t (&r)[32]) {
         : "r"(taddr));
 #undef DSV_OUT
 }
-__device__ __forceinline__ void tmem_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+// the loads issued so far are complete; `r` is in the operands so that no use of it moves ahead
+__device__ __forceinline__ void tmem_wait_ld(uint32_t (&r)[32]) {
+#define DSV_IO(y) "+r"(y)
+    asm volatile("tcgen05.wait::ld.sync.aligned;" : DSV_R16(DSV_IO, 0), DSV_R16(DSV_IO, 16)::"memory");
+#undef DSV_IO
+}
 __device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t (&r)[32]) {
 #define DSV_IN(y) "r"(y)
@@ -350,15 +356,19 @@ __device__ __forceinline__ void cp16(uint32_t dst, const void* src, bool ok) {
     asm volatile("cp.async.cg.shared.global.L2::128B [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(ok ? 16 : 0)
                  : "memory");
 }
-__device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int N> __device__ __forceinline__ void cp_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+// arrives at `bar` once this thread's copies so far have landed
+__device__ __forceinline__ void cp_arrive(uint64_t* bar) {
+    asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
+}
+__device__ __forceinline__ void cp_wait_all() { asm volatile("cp.async.wait_all;" ::: "memory"); }
 
 // bounded wait that also gives up when another warp of the CTA has given up
 __device__ __forceinline__ bool wait_or_abort(uint64_t* bar, uint32_t parity, volatile int* abort) {
     if (mbar_try_wait(bar, parity)) return true;
     const uint64_t t0 = globaltimer_ns();
-    for (;;) {
+    for (uint32_t i = 1;; ++i) {
         if (mbar_try_wait(bar, parity)) return true;
+        if (i % 32 != 0) continue;
         if (*abort) return false;
         if (globaltimer_ns() - t0 > 2000000000ull) {
             *abort = 1;
@@ -366,6 +376,9 @@ __device__ __forceinline__ bool wait_or_abort(uint64_t* bar, uint32_t parity, vo
         }
     }
 }
+
+template <int N> __device__ __forceinline__ void regs_down() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N)); }
+template <int N> __device__ __forceinline__ void regs_up() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N)); }
 
 // 16-byte chunk c of row `row` in a tile of 128-byte-swizzled blocks
 __device__ __forceinline__ uint32_t chunk_at(int row, int c) {
@@ -433,12 +446,10 @@ struct Tiles {
 // ---- the kernel ---------------------------------------------------------------------------------
 
 template <typename TQ, bool kFp8, int DP>
-__global__ void __launch_bounds__(threads<kFp8>(), 1) attn_kernel(const __grid_constant__ KernelArgs a) {
+__global__ void __launch_bounds__(kThreads, 1) attn_kernel(const __grid_constant__ KernelArgs a) {
     using L = Layout<DP, kFp8>;
     using Info = typename InfoOf<kFp8>::type;
     using TO = typename std::conditional<kFp8, __half, TQ>::type;   // operands of the matrix instructions
-    constexpr int kThreads = threads<kFp8>();
-    constexpr int kProducers = producer_warps<kFp8>();
     extern __shared__ uint8_t smem_raw[];
     const int qt = a.qt, stages = L::stages(qt);
     uint8_t* base = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
@@ -453,65 +464,70 @@ __global__ void __launch_bounds__(threads<kFp8>(), 1) attn_kernel(const __grid_c
 
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
 
-    // ---- this CTA's piece of the line of tiles
-    long long total = 0;
-    for (int b0 = 0; b0 < t.batch; b0 += kThreads) {
-        const int b = b0 + tid;
-        long long c = 0;
-        if (b < t.batch) {
-            const Request r = request_of(t, qt, b);
-            c = tiles_of_head(t, qt, r) * t.c.heads;
-            if (t.err && blockIdx.x == 0 && __ldg(t.lens + b) > t.max_pages * t.page_size) atomicOr(t.err, 2u);
-        }
-#pragma unroll
-        for (int o = 16; o > 0; o >>= 1) c += __shfl_xor_sync(0xffffffffu, c, o);
-        if (lane == 0) sh->scan[warp] = c;
-        __syncthreads();
-        for (int i = 0; i < kThreads / 32; ++i) total += sh->scan[i];
-        __syncthreads();
-    }
-    long long want = total / kMinTiles;
-    const int ctas = (int)(want < 1 ? 1 : (want < (long long)gridDim.x ? want : (long long)gridDim.x));
     if (tid == 0) a.splits[blockIdx.x].valid = 0;
+
+    // ---- this CTA's piece of the line of tiles: a block scan over the requests' tiles, a second
+    // one (another round over the requests) only where they are more than the threads
+    long long total = 0, c = 0, upto = 0;                 // of all; of this thread's request; up to it
+    auto scan = [&](int b0) {
+        const int b = b0 + tid;
+        c = 0;
+        if (b < t.batch) c = tiles_of_head(t, qt, request_of(t, qt, b)) * t.c.heads;
+        upto = c;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const long long up = __shfl_up_sync(0xffffffffu, upto, o);
+            if (lane >= o) upto += up;
+        }
+        if (lane == 31) sh->scan[warp] = upto;
+        __syncthreads();
+        long long all = 0;
+#pragma unroll
+        for (int i = 0; i < kThreads / 32; ++i) {
+            const long long x = sh->scan[i];
+            if (i < warp) upto += x;
+            all += x;
+        }
+        return all;
+    };
+    for (int b0 = 0; b0 < t.batch; b0 += kThreads) {
+        if (b0 > 0) __syncthreads();
+        total += scan(b0);
+        if (t.err && blockIdx.x == 0 && b0 + tid < t.batch && __ldg(t.lens + b0 + tid) > t.max_pages * t.page_size)
+            atomicOr(t.err, 2u);
+    }
+    const long long want = total / kMinTiles;
+    const int ctas = (int)(want < 1 ? 1 : (want < (long long)gridDim.x ? want : (long long)gridDim.x));
     if (total == 0 || (int)blockIdx.x >= ctas) return;
     const long long mine = first_tile(blockIdx.x, total, ctas);
     const long long count = first_tile(blockIdx.x + 1, total, ctas) - mine;
     {
         long long before = 0;
         for (int b0 = 0; b0 < t.batch; b0 += kThreads) {
-            const int b = b0 + tid;
-            long long c = 0;
-            if (b < t.batch) c = tiles_of_head(t, qt, request_of(t, qt, b)) * t.c.heads;
-            long long s = c;
-#pragma unroll
-            for (int o = 1; o < 32; o <<= 1) {
-                const long long up = __shfl_up_sync(0xffffffffu, s, o);
-                if (lane >= o) s += up;
+            if (t.batch > kThreads) {
+                __syncthreads();
+                const long long all = scan(b0);
+                upto += before;
+                before += all;
             }
-            if (lane == 31) sh->scan[warp] = s;
-            __syncthreads();
-            long long add = before;
-            for (int i = 0; i < warp; ++i) add += sh->scan[i];
-            for (int i = 0; i < kThreads / 32; ++i) before += sh->scan[i];
-            s += add;
-            if (c > 0 && mine >= s - c && mine < s) {
-                sh->start_b = b;
-                sh->start_in_b = mine - (s - c);
+            if (c > 0 && mine >= upto - c && mine < upto) {
+                sh->start_b = b0 + tid;
+                sh->start_in_b = mine - (upto - c);
             }
-            __syncthreads();
         }
     }
 
     if (tid == 0) {
         for (int s = 0; s < stages; ++s) {
-            mbar_init(&sh->full[s], kProducers);
+            mbar_init(&sh->full[s], kFp8 ? kProducers : kProducers * 32);
             mbar_init(&sh->empty[s], 1);
         }
         for (int i = 0; i < kInfo; ++i) mbar_init(&sh->info[i], kProducers);
         mbar_init(&sh->q_full, 8);
         for (int i = 0; i < 2; ++i) {
             mbar_init(&sh->s_full[i], 1);
-            mbar_init(&sh->p_full[i], 4);
+            mbar_init(&sh->p_full[i][0], 4);
+            mbar_init(&sh->p_full[i][1], 4);
         }
         mbar_init(&sh->o_full, 1);
         mbar_init(&sh->joined, 8);
@@ -537,9 +553,10 @@ __global__ void __launch_bounds__(threads<kFp8>(), 1) attn_kernel(const __grid_c
         a.splits[blockIdx.x] = s;
     }
 
-    if (warp > 8) {
+    if (warp >= 12) {
         // ---------------- producers ----------------
-        const int pw = warp - 9;
+        if constexpr (!kFp8) regs_down<56>();
+        const int pw = warp - 12;
         constexpr int kTokens = kTile / kProducers;             // tokens of a tile per warp
         Tiles<kTokens> g;
         g.begin(a, w, pw * kTokens + (lane & (kTokens - 1)));
@@ -549,8 +566,6 @@ __global__ void __launch_bounds__(threads<kFp8>(), 1) attn_kernel(const __grid_c
             constexpr int kLanes = DP / 8;                      // lanes of a row (16-byte chunks)
             const int sub = lane % kLanes, dr = lane / kLanes;
             const bool live = sub * 8 < t.c.dim;
-            const int lag = qt == 1 ? L::kLag : L::kLag2;
-            uint32_t told = 0;                                  // stages handed over
             while (ok && g.next(a)) {
                 if (g.is_k) {
                     const uint32_t valid = __ballot_sync(0xffffffffu, g.cur >= 0);
@@ -574,122 +589,119 @@ __global__ void __launch_bounds__(threads<kFp8>(), 1) attn_kernel(const __grid_c
                     const bool get = live && slot >= 0;
                     cp16(dst + chunk_at(pw * kTokens + tok, sub), src + (get ? 2 * (slot * t.c.slot_stride) : 0), get);
                 }
-                cp_commit();
+                cp_arrive(&sh->full[s]);
                 ++n;
-                if (n > (uint32_t)lag) {
-                    if (qt == 1)
-                        cp_wait<L::kLag>();
-                    else
-                        cp_wait<L::kLag2>();
-                    fence_proxy_async_smem();
-                    __syncwarp();
-                    if (lane == 0) mbar_arrive(&sh->full[told % stages]);
-                    ++told;
-                }
             }
-            cp_wait<0>();
-            fence_proxy_async_smem();
-            __syncwarp();
-            for (; told < n; ++told)
-                if (lane == 0) mbar_arrive(&sh->full[told % stages]);
+            cp_wait_all();
         } else {
             constexpr int kLanes = DP / 16;                     // lanes of a row (16 codes each)
-            constexpr int kSteps = kTokens * kLanes / 32;
-            constexpr int kAhead = 3;                           // items whose loads are in flight
+            constexpr int kSteps = kTokens * kLanes / 64;       // 16-byte loads of half an item, per lane
+            constexpr int kAhead = 5;                           // half items whose loads are in flight
             const int sub = lane % kLanes, dr = lane / kLanes;
             const bool live = sub * 16 < t.c.dim;
             uint4 buf[kAhead][kSteps];
-            auto issue = [&](uint4 (&x)[kSteps]) -> bool {
-                if (!g.next(a)) return false;
-                const int mine_slot = g.slot();
-                if (g.is_k) {
-                    Info* inf = info + (g.tile - 1) % kInfo;
-                    const uint32_t valid = __ballot_sync(0xffffffffu, mine_slot >= 0) & ((1u << kTokens) - 1u);
-                    float ks = 0.f, vs = 0.f;
-                    if (mine_slot >= 0) {
-                        const long long at = mine_slot * t.c.scale_stride + g.w.h;
-                        ks = __ldg(t.c.k_scale + at);
-                        vs = __ldg(t.c.v_scale + at);
-                    }
-                    float top = fabsf(vs) < __int_as_float(0x7f800000) ? fabsf(vs) : 0.f;
+            uint32_t issued = 0, done = 0;                      // half items
+            int item_slot = -1;
+            const uint8_t* src = nullptr;
+            bool more = true;
+            auto issue = [&](uint4 (&x)[kSteps]) {
+                if (!(issued & 1u)) {
+                    more = g.next(a);
+                    if (!more) return;
+                    item_slot = g.slot();
+                    src = static_cast<const uint8_t*>(g.is_k ? t.c.k : t.c.v) + (g.w.h * t.c.head_stride + sub * 16);
+                    if (g.is_k) {
+                        const int at_info = (g.tile - 1) % kInfo;
+                        Info* inf = info + at_info;
+                        const uint32_t valid = __ballot_sync(0xffffffffu, item_slot >= 0);
+                        float ks = 0.f, vs = 0.f;
+                        if (item_slot >= 0) {
+                            const long long at = item_slot * t.c.scale_stride + g.w.h;
+                            ks = __ldg(t.c.k_scale + at);
+                            vs = __ldg(t.c.v_scale + at);
+                        }
+                        float top = fabsf(vs) < __int_as_float(0x7f800000) ? fabsf(vs) : 0.f;
 #pragma unroll
-                    for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-                    if (lane < kTokens) {
+                        for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
                         inf->ks[pw * kTokens + lane] = ks * (t.scale * kL2E);
                         inf->vs[pw * kTokens + lane] = vs;
+                        if (lane == 0) {
+                            inf->valid[pw] = valid;
+                            inf->vmax[pw] = top;
+                        }
+                        __syncwarp();
+                        if (lane == 0) mbar_arrive(&sh->info[at_info]);
                     }
-                    if (lane == 0) {
-                        reinterpret_cast<uint16_t*>(inf->valid)[pw] = (uint16_t)valid;
-                        inf->vmax[pw] = top;
-                    }
-                    __syncwarp();
-                    if (lane == 0) mbar_arrive(&sh->info[(g.tile - 1) % kInfo]);
                 }
-                const uint8_t* src = static_cast<const uint8_t*>(g.is_k ? t.c.k : t.c.v) +
-                                     (g.w.h * t.c.head_stride + sub * 16);
+                const int first = (issued & 1u) * (kTokens / 2) + dr;
 #pragma unroll
                 for (int i = 0; i < kSteps; ++i) {
-                    const int slot = __shfl_sync(0xffffffffu, mine_slot, i * (32 / kLanes) + dr);
+                    const int slot = __shfl_sync(0xffffffffu, item_slot, first + i * (32 / kLanes));
                     x[i] = make_uint4(0, 0, 0, 0);
                     if (live && slot >= 0) x[i] = __ldg(reinterpret_cast<const uint4*>(src + slot * t.c.slot_stride));
                 }
-                return true;
+                ++issued;
             };
             auto finish = [&](const uint4 (&x)[kSteps]) {
                 const uint32_t s = n % stages, ph = (n / stages) & 1u;
-                ok = __all_sync(0xffffffffu, wait_or_abort(&sh->empty[s], ph ^ 1u, abort));
-                if (!ok) return;
+                if (!(done & 1u)) {
+                    ok = __all_sync(0xffffffffu, wait_or_abort(&sh->empty[s], ph ^ 1u, abort));
+                    if (!ok) return;
+                }
                 uint8_t* dst = ring + s * L::kStage;
+                const int first = pw * kTokens + (done & 1u) * (kTokens / 2) + dr;
 #pragma unroll
                 for (int i = 0; i < kSteps; ++i) {
-                    const int row = pw * kTokens + i * (32 / kLanes) + dr;
-                    const uint32_t c[4] = {x[i].x, x[i].y, x[i].z, x[i].w};
+                    const int row = first + i * (32 / kLanes);
+                    const uint32_t c8[4] = {x[i].x, x[i].y, x[i].z, x[i].w};
                     uint32_t o[8];
 #pragma unroll
                     for (int j = 0; j < 8; ++j) {
                         const __half2_raw h =
-                            __nv_cvt_fp8x2_to_halfraw2((uint16_t)(c[j >> 1] >> (16 * (j & 1))), __NV_E4M3);
+                            __nv_cvt_fp8x2_to_halfraw2((uint16_t)(c8[j >> 1] >> (16 * (j & 1))), __NV_E4M3);
                         o[j] = (uint32_t)h.x | ((uint32_t)h.y << 16);
                     }
                     *reinterpret_cast<uint4*>(dst + chunk_at(row, 2 * sub)) = make_uint4(o[0], o[1], o[2], o[3]);
                     *reinterpret_cast<uint4*>(dst + chunk_at(row, 2 * sub + 1)) = make_uint4(o[4], o[5], o[6], o[7]);
                 }
-                fence_proxy_async_smem();
-                __syncwarp();
-                if (lane == 0) mbar_arrive(&sh->full[s]);
-                ++n;
+                if (done & 1u) {
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(&sh->full[s]);
+                    ++n;
+                }
+                ++done;
             };
-            int held = 0;                                       // items loaded and not handed over
-            bool more = true;
 #pragma unroll
             for (int i = 0; i < kAhead; ++i)
-                if (more && (more = issue(buf[i]))) ++held;
-            while (ok && held > 0) {
+                if (more) issue(buf[i]);
+            while (ok && done < issued) {
 #pragma unroll
                 for (int i = 0; i < kAhead; ++i) {
-                    if (ok && held > 0) {
+                    if (ok && done < issued) {
                         finish(buf[i]);
-                        --held;
-                        if (ok && more && (more = issue(buf[i]))) ++held;
+                        if (ok && more) issue(buf[i]);
                     }
                 }
             }
         }
-    } else if (warp == 8) {
+    } else if (warp >= 8) {
         // ---------------- MMA issuer ----------------
-        if (lane == 0) {
+        regs_down<kFp8 ? 40 : 56>();
+        if (warp == 8 && lane == 0) {
             constexpr uint32_t kFormat = std::is_same<TO, __nv_bfloat16>::value ? 1u : 0u;
             constexpr uint32_t kCommon = (1u << 4) | (kFormat << 7) | (kFormat << 10) | ((uint32_t)(kRows >> 4) << 24);
             constexpr uint32_t kIdescS = kCommon | ((uint32_t)(kTile >> 3) << 17);
             const uint32_t idesc_o = kCommon | (1u << 16) | ((uint32_t)(t.c.dim >> 3) << 17);  // B: MN-major
             const int ksteps = t.c.dim / 16;
-            const uint32_t q0 = smem_u32(sq), r0 = smem_u32(ring);
+            const uint32_t q0 = desc_low(smem_u32(sq), 16), k0 = desc_low(smem_u32(ring), 16),
+                           v0 = desc_low(smem_u32(ring), kBlock);
             uint32_t item = 0, seg = 0, su[2] = {0, 0};  // items before the segment, segments, units per stream
             bool ok = true;
             do {
                 const bool both = !w.shared_rows(qt);    // both streams use every tile
                 const int nt = w.count(), units = both ? 2 * nt : nt;
                 ok = wait_or_abort(&sh->q_full, seg & 1u, abort);
+                fence_proxy_async_smem();
                 tc_fence_after();
                 auto scores = [&](int u) {
                     const int s = u & 1, tl = both ? u >> 1 : u;
@@ -700,10 +712,12 @@ __global__ void __launch_bounds__(threads<kFp8>(), 1) attn_kernel(const __grid_c
                         fence_proxy_async_smem();
                         tc_fence_after();
                     }
-                    const uint32_t qa = q0 + (both ? s * L::kStage : 0), kb = r0 + st * L::kStage;
-                    for (int k = 0; k < ksteps; ++k) {
-                        const uint32_t off = (k >> 2) * kBlock + (k & 3) * 32;
-                        mma_ss(tmem + s * kTile, smem_desc(qa + off, 16), smem_desc(kb + off, 16), kIdescS, k != 0);
+                    const uint32_t qa = q0 + (both && s ? L::kStage >> 4 : 0), kb = k0 + st * (L::kStage >> 4);
+                    const uint32_t d = tmem + s * kTile;
+#pragma unroll
+                    for (int k = 0; k < DP / 16; ++k) {
+                        const uint32_t off = (k >> 2) * (kBlock >> 4) + (k & 3) * 2;
+                        if (k < ksteps) mma_ss(d, desc(qa + off), desc(kb + off), kIdescS, k != 0);
                     }
                     if (!both || s == 1) mma_commit(&sh->empty[st]);
                     mma_commit(&sh->s_full[s]);
@@ -711,21 +725,24 @@ __global__ void __launch_bounds__(threads<kFp8>(), 1) attn_kernel(const __grid_c
                 for (int u = 0; ok && u < 2 && u < units; ++u) scores(u);
                 for (int u = 0; ok && u < units; ++u) {
                     const int s = u & 1, tl = both ? u >> 1 : u;
-                    ok = wait_or_abort(&sh->p_full[s], su[s] & 1u, abort);
-                    if (!ok) break;
-                    ++su[s];
                     const uint32_t it = item_of_v(item, tl, nt), st = it % stages;
                     if (!both || s == 0) {
                         ok = wait_or_abort(&sh->full[st], (it / stages) & 1u, abort);
                         if (!ok) break;
                         fence_proxy_async_smem();
                     }
-                    tc_fence_after();
-                    const uint32_t vb = r0 + st * L::kStage;
+                    const uint32_t vb = v0 + st * (L::kStage >> 4), d = tmem + 256 + s * 128, p = tmem + s * kTile;
 #pragma unroll
-                    for (int k = 0; k < kTile / 16; ++k)
-                        mma_ts(tmem + 256 + s * 128, tmem + s * kTile + k * 8, smem_desc(vb + k * 2048, kBlock), idesc_o,
-                               u >= 2 || k != 0);
+                    for (int half = 0; half < 2; ++half) {
+                        ok = ok && wait_or_abort(&sh->p_full[s][half], su[s] & 1u, abort);
+                        if (!ok) break;
+                        tc_fence_after();
+#pragma unroll
+                        for (int k = 4 * half; k < 4 * half + 4; ++k)
+                            mma_ts(d, p + k * 8, desc(vb + k * (2048 >> 4)), idesc_o, u >= 2 || k != 0);
+                    }
+                    if (!ok) break;
+                    ++su[s];
                     if (!both || s == 1) mma_commit(&sh->empty[st]);
                     if (u + 2 < units) scores(u + 2);
                 }
@@ -740,68 +757,93 @@ __global__ void __launch_bounds__(threads<kFp8>(), 1) attn_kernel(const __grid_c
         __syncwarp();
     } else {
         // ---------------- softmax and epilogue: one row per thread ----------------
+        regs_up<kFp8 ? 168 : 200>();
         const int s = warp >> 2, quarter = warp & 3, row = quarter * 32 + lane;
         const uint32_t lanes = (uint32_t)(quarter * 32) << 16;
         const uint32_t ts = tmem + lanes + s * kTile, to = tmem + lanes + 256 + s * 128;
-        uint32_t seg = 0, su = 0, tile0 = 0, item = 0;
+        constexpr int kLanes = DP / 8;                          // 16-byte chunks of a row
+        constexpr int kStep = kSoftmaxThreads / kLanes;         // rows that the 256 threads move at once
+        const int sub = tid % kLanes, r_first = tid / kLanes;
+        const bool sub_live = sub * 8 < t.c.dim;
+        const uint32_t group_inv = (0xFFFFFFFFu / (uint32_t)t.group) + 1u;  // ceil(2^32 / group), 0 for 1
+        uint32_t seg = 0, su = 0, tile0 = 0, item = 0, jp = 0;  // jp: phases of `joined`
         bool ok = true;
+        auto join = [&]() {                                     // both warpgroups have come here
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&sh->joined);
+            ok = __all_sync(0xffffffffu, ok && wait_or_abort(&sh->joined, jp & 1u, abort));
+            ++jp;
+        };
         do {
             const bool both = !w.shared_rows(qt);
             const int nt = w.count(), nrows = w.rows(qt), row0 = w.first_row(qt);
             const int my = both ? s * kRows + row : row;        // row of the block
-            // ---- Q into shared memory
+            const int token0 = row0 / t.group, rem0 = row0 - token0 * t.group;
+            // drafted token (from token0) and query head of the block's row r
+            auto token_of = [&](int r, int& gq) {
+                const uint32_t x = rem0 + r;
+                const int i = t.group == 1 ? (int)x : (int)__umulhi(x, group_inv);
+                gq = (int)x - i * t.group;
+                return i;
+            };
+            auto q_offset = [&](int r, long long ts_, long long hs) {
+                int gq;
+                const int i = token_of(r, gq);
+                return (long long)(w.r.lo + token0 + i) * ts_ + (long long)(w.h * t.group + gq) * hs;
+            };
+            // ---- Q into shared memory: whole warps of rows, zeros past the last
             {
-                constexpr int kLanes = DP / 8;
-                const int sub = tid % kLanes, tiles_q = both ? 2 : 1;
-                const int filled = (nrows + 31) & ~31;          // whole warps of rows: zeros past the last
-#pragma unroll 4
-                for (int r = tid / kLanes; r < tiles_q * kRows; r += kSoftmaxThreads / kLanes) {
-                    uint4 x = make_uint4(0, 0, 0, 0);
-                    if (r < nrows && sub * 8 < t.c.dim) {
-                        const int i = (row0 + r) / t.group, gq = (row0 + r) - i * t.group;
-                        x = __ldg(reinterpret_cast<const uint4*>(
-                            static_cast<const TQ*>(t.q) + (long long)(w.r.lo + i) * t.q_token_stride +
-                            (long long)(w.h * t.group + gq) * t.q_head_stride + sub * 8));
-                    }
-                    if constexpr (kFp8) {
-                        float f[8];
-                        unpack2(x.x, f[0], f[1], TQ());
-                        unpack2(x.y, f[2], f[3], TQ());
-                        unpack2(x.z, f[4], f[5], TQ());
-                        unpack2(x.w, f[6], f[7], TQ());
-                        float m = 0.f;
+                const int filled = (nrows + 31) & ~31;
+                const TQ* q = static_cast<const TQ*>(t.q) + sub * 8;
+#pragma unroll 1
+                for (int r0 = r_first; r0 - r_first < filled; r0 += 8 * kStep) {
+                    uint4 x[8];
 #pragma unroll
-                        for (int i = 0; i < 8; ++i) m = fmaxf(m, fabsf(f[i]));
-#pragma unroll
-                        for (int o = kLanes / 2; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-                        // a power of two that brings the row's largest value to [2^13, 2^14): products stay
-                        // exact, and values down to 2^-37 of the largest keep a place in fp16
-                        int e = (int)(__float_as_uint(m) >> 23) - 127;
-                        e = m > 0.f && e < 128 ? max(e, -100) : 13;
-                        const float up = __uint_as_float((uint32_t)(13 - e + 127) << 23);
-                        if (sub == 0) row_mul[r] = __uint_as_float((uint32_t)(e - 13 + 127) << 23);
-                        x = make_uint4(pack2(f[0] * up, f[1] * up, __half()), pack2(f[2] * up, f[3] * up, __half()),
-                                       pack2(f[4] * up, f[5] * up, __half()), pack2(f[6] * up, f[7] * up, __half()));
+                    for (int i = 0; i < 8; ++i) {
+                        const int r = r0 + i * kStep;
+                        x[i] = make_uint4(0, 0, 0, 0);
+                        if (r < nrows && sub_live)
+                            x[i] = __ldg(reinterpret_cast<const uint4*>(q + q_offset(r, t.q_token_stride, t.q_head_stride)));
                     }
-                    if (r < filled)
-                        *reinterpret_cast<uint4*>(sq + (r >> 7) * L::kStage + chunk_at(r & 127, sub)) = x;
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) {
+                        const int r = r0 + i * kStep;
+                        if constexpr (kFp8) {
+                            float f[8];
+                            unpack2(x[i].x, f[0], f[1], TQ());
+                            unpack2(x[i].y, f[2], f[3], TQ());
+                            unpack2(x[i].z, f[4], f[5], TQ());
+                            unpack2(x[i].w, f[6], f[7], TQ());
+                            float m = 0.f;
+#pragma unroll
+                            for (int j = 0; j < 8; ++j) m = fmaxf(m, fabsf(f[j]));
+#pragma unroll
+                            for (int o = kLanes / 2; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+                            // a power of two that brings the row's largest value to [2^13, 2^14): products
+                            // stay exact, and values down to 2^-37 of the largest keep a place in fp16
+                            int e = (int)(__float_as_uint(m) >> 23) - 127;
+                            e = m > 0.f && e < 128 ? max(e, -100) : 13;
+                            const float up = __uint_as_float((uint32_t)(13 - e + 127) << 23);
+                            if (sub == 0 && r < filled) row_mul[r] = __uint_as_float((uint32_t)(e - 13 + 127) << 23);
+                            x[i] = make_uint4(pack2(f[0] * up, f[1] * up, __half()), pack2(f[2] * up, f[3] * up, __half()),
+                                              pack2(f[4] * up, f[5] * up, __half()), pack2(f[6] * up, f[7] * up, __half()));
+                        }
+                        if (r < filled)
+                            *reinterpret_cast<uint4*>(sq + (r >> 7) * L::kStage + chunk_at(r & 127, sub)) = x[i];
+                    }
                 }
-                fence_proxy_async_smem();
                 tc_fence_before();
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&sh->q_full);
-                if constexpr (kFp8) {
-                    // row_mul comes from all eight warps
-                    ok = ok && wait_or_abort(&sh->q_full, seg & 1u, abort);
-                    ok = __all_sync(0xffffffffu, ok);
-                }
+                if constexpr (kFp8)                             // row_mul comes from all eight warps
+                    ok = __all_sync(0xffffffffu, ok && wait_or_abort(&sh->q_full, seg & 1u, abort));
             }
             const bool any_row = (both ? s * kRows : 0) + quarter * 32 < nrows;  // this warp has rows
-            const float cm = kFp8 ? row_mul[my] : t.scale * kL2E;
-            int token = 0;                                      // this row's drafted token
+            const float cm = kFp8 ? (any_row ? row_mul[my] : 1.f) : t.scale * kL2E;
+            int token = 0, gq = 0;                              // this row's drafted token and head
             uint64_t bits = 0;
             if (my < nrows) {
-                token = (row0 + my) / t.group;
+                token = token0 + token_of(my, gq);
                 if (t.mask) bits = (uint64_t)__ldg(reinterpret_cast<const long long*>(t.mask) + w.r.lo + token);
             }
             float ref = -INFINITY, sum = 0.f, vmax = 0.f;
@@ -816,10 +858,47 @@ __global__ void __launch_bounds__(threads<kFp8>(), 1) attn_kernel(const __grid_c
                 tc_fence_after();
                 const int kb = (w.k0 + tl) * kTile;             // first position of the tile
                 const bool drafted = kb + kTile > w.r.p0;
+                if (drafted) {
+                    // V elements of drafted tokens that are not finite: zeroed for the matrix
+                    // instructions, added to the rows that see them at the end
+                    const uint32_t it = item_of_v(item, tl, nt), st = it % stages;
+                    ok = __all_sync(0xffffffffu, wait_or_abort(&sh->full[st], (it / stages) & 1u, abort));
+                    if (!ok) break;
+                    if (kb + row >= w.r.p0 && kb + row < w.r.len) {
+                        uint8_t* v = ring + st * L::kStage;
+                        constexpr uint32_t kExp = std::is_same<TO, __nv_bfloat16>::value ? 0x7F80u : 0x7C00u;
+                        bool found = false;
+                        for (int c = 0; c < t.c.dim / 8; ++c) {
+                            uint4* at = reinterpret_cast<uint4*>(v + chunk_at(row, c));
+                            const uint4 x = *at;
+                            uint32_t xw[4] = {x.x, x.y, x.z, x.w};
+                            bool here = false;
+#pragma unroll
+                            for (int i = 0; i < 4; ++i) {
+                                if ((xw[i] & kExp) == kExp) {
+                                    xw[i] &= 0xFFFF0000u;
+                                    here = true;
+                                }
+                                if ((xw[i] & (kExp << 16)) == (kExp << 16)) {
+                                    xw[i] &= 0xFFFFu;
+                                    here = true;
+                                }
+                            }
+                            if (here) *at = make_uint4(xw[0], xw[1], xw[2], xw[3]);
+                            found |= here;
+                        }
+                        if (found) *(volatile int*)&sh->odd[seg & 1] = 1;
+                    }
+                    fence_proxy_async_smem();
+                }
                 if (any_row) {
-                    uint32_t vis[4] = {~0u, ~0u, ~0u, ~0u};
+                    // this row's 128 scores stay in registers: one read of TMEM
+                    uint32_t v[4][32];
+#pragma unroll
+                    for (int c = 0; c < 4; ++c) tmem_ld32(ts + c * 32, v[c]);
                     const uint4 valid = *reinterpret_cast<const uint4*>(inf->valid);
                     const bool masked = drafted || (valid.x & valid.y & valid.z & valid.w) != ~0u;
+                    uint32_t vis[4] = {~0u, ~0u, ~0u, ~0u};
                     if (masked) {
                         const uint32_t vw[4] = {valid.x, valid.y, valid.z, valid.w};
 #pragma unroll
@@ -837,35 +916,41 @@ __global__ void __launch_bounds__(threads<kFp8>(), 1) attn_kernel(const __grid_c
                             vis[i] = m & vw[i];
                         }
                     }
-                    // the row's largest score of this tile
-                    float mx = -INFINITY;
+                    float mx[4];
 #pragma unroll
                     for (int c = 0; c < 4; ++c) {
-                        uint32_t v[32];
-                        tmem_ld32(ts + c * 32, v);
-                        tmem_wait_ld();
+                        tmem_wait_ld(v[c]);
                         if constexpr (kFp8) {
 #pragma unroll
                             for (int j = 0; j < 32; j += 4) {
                                 const float4 k4 = *reinterpret_cast<const float4*>(&inf->ks[c * 32 + j]);
-                                v[j] = __float_as_uint(__uint_as_float(v[j]) * k4.x);
-                                v[j + 1] = __float_as_uint(__uint_as_float(v[j + 1]) * k4.y);
-                                v[j + 2] = __float_as_uint(__uint_as_float(v[j + 2]) * k4.z);
-                                v[j + 3] = __float_as_uint(__uint_as_float(v[j + 3]) * k4.w);
+                                const float2 lo = __fmul2_rn(make_float2(__uint_as_float(v[c][j]), __uint_as_float(v[c][j + 1])),
+                                                             make_float2(k4.x, k4.y));
+                                const float2 hi = __fmul2_rn(make_float2(__uint_as_float(v[c][j + 2]), __uint_as_float(v[c][j + 3])),
+                                                             make_float2(k4.z, k4.w));
+                                v[c][j] = __float_as_uint(lo.x);
+                                v[c][j + 1] = __float_as_uint(lo.y);
+                                v[c][j + 2] = __float_as_uint(hi.x);
+                                v[c][j + 3] = __float_as_uint(hi.y);
                             }
                         }
                         if (masked) {
 #pragma unroll
                             for (int j = 0; j < 32; ++j)
-                                if (!((vis[c] >> j) & 1u)) v[j] = 0xFF800000u;
+                                if (!((vis[c] >> j) & 1u)) v[c][j] = 0xFF800000u;
                         }
+                        float a0 = -INFINITY, a1 = -INFINITY;
 #pragma unroll
-                        for (int j = 0; j < 32; ++j) mx = fmaxf(mx, __uint_as_float(v[j]));
+                        for (int j = 0; j < 32; j += 4) {
+                            a0 = fmaxf(a0, fmaxf(__uint_as_float(v[c][j]), __uint_as_float(v[c][j + 1])));
+                            a1 = fmaxf(a1, fmaxf(__uint_as_float(v[c][j + 2]), __uint_as_float(v[c][j + 3])));
+                        }
+                        mx[c] = fmaxf(a0, a1);
                     }
-                    float target = mx * cm;
+                    float target = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * cm;
                     if constexpr (kFp8) {
-#pragma unroll
-                        for (int i = 0; i < 8; ++i) vmax = fmaxf(vmax, inf->vmax[i]);
+                        const float4 vm = *reinterpret_cast<const float4*>(inf->vmax);
+                        vmax = fmaxf(vmax, fmaxf(fmaxf(vm.x, vm.y), fmaxf(vm.z, vm.w)));
                         // 2^ev is the first power of two above the V scales so far
                         const int ev = max(-90, min(120, (int)(__float_as_uint(vmax) >> 23) - 126));
                         target += (float)(ev - 6);
@@ -879,193 +964,167 @@ __global__ void __launch_bounds__(threads<kFp8>(), 1) attn_kernel(const __grid_c
                             sum *= f;
 #pragma unroll 1
                             for (int c = 0; c < t.c.dim; c += 32) {
-                                uint32_t v[32];
-                                tmem_ld32(to + c, v);
-                                tmem_wait_ld();
+                                uint32_t o[32];
+                                tmem_ld32(to + c, o);
+                                tmem_wait_ld(o);
 #pragma unroll
-                                for (int j = 0; j < 32; ++j) v[j] = __float_as_uint(__uint_as_float(v[j]) * f);
-                                tmem_st32(to + c, v);
+                                for (int j = 0; j < 32; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * f);
+                                tmem_st32(to + c, o);
                             }
                         }
                         ref = to_ref;
                     }
                     const float nref = ref == -INFINITY ? 0.f : -ref;
-                    float part[4] = {0.f, 0.f, 0.f, 0.f};
+                    const float2 cm2 = make_float2(cm, cm), nref2 = make_float2(nref, nref);
+                    float2 part0 = make_float2(0.f, 0.f), part1 = part0;
 #pragma unroll
                     for (int c = 0; c < 4; ++c) {
-                        uint32_t v[32], p[16];
-                        tmem_ld32(ts + c * 32, v);
-                        tmem_wait_ld();
+                        uint32_t p[16];
 #pragma unroll
                         for (int j = 0; j < 32; j += 4) {
-                            float x[4] = {__uint_as_float(v[j]), __uint_as_float(v[j + 1]), __uint_as_float(v[j + 2]),
-                                          __uint_as_float(v[j + 3])};
-                            if constexpr (kFp8) {
-                                const float4 k4 = *reinterpret_cast<const float4*>(&inf->ks[c * 32 + j]);
-                                x[0] *= k4.x;
-                                x[1] *= k4.y;
-                                x[2] *= k4.z;
-                                x[3] *= k4.w;
-                            }
-#pragma unroll
-                            for (int i = 0; i < 4; ++i) {
-                                x[i] = ex2(fmaf(x[i], cm, nref));
-                                if (masked && !((vis[c] >> (j + i)) & 1u)) x[i] = 0.f;
-                                part[i] += x[i];
-                            }
+                            float2 lo = __ffma2_rn(make_float2(__uint_as_float(v[c][j]), __uint_as_float(v[c][j + 1])), cm2, nref2);
+                            float2 hi = __ffma2_rn(make_float2(__uint_as_float(v[c][j + 2]), __uint_as_float(v[c][j + 3])), cm2, nref2);
+                            lo = make_float2(ex2(lo.x), ex2(lo.y));
+                            hi = make_float2(ex2(hi.x), ex2(hi.y));
+                            part0 = __fadd2_rn(part0, lo);
+                            part1 = __fadd2_rn(part1, hi);
                             if constexpr (kFp8) {
                                 const float4 v4 = *reinterpret_cast<const float4*>(&inf->vs[c * 32 + j]);
-                                x[0] = masked && !((vis[c] >> j) & 1u) ? 0.f : x[0] * v4.x;
-                                x[1] = masked && !((vis[c] >> (j + 1)) & 1u) ? 0.f : x[1] * v4.y;
-                                x[2] = masked && !((vis[c] >> (j + 2)) & 1u) ? 0.f : x[2] * v4.z;
-                                x[3] = masked && !((vis[c] >> (j + 3)) & 1u) ? 0.f : x[3] * v4.w;
+                                lo = __fmul2_rn(lo, make_float2(v4.x, v4.y));
+                                hi = __fmul2_rn(hi, make_float2(v4.z, v4.w));
+                                if (masked) {                   // 0 x a scale that is not finite
+                                    if (!((vis[c] >> j) & 1u)) lo.x = 0.f;
+                                    if (!((vis[c] >> (j + 1)) & 1u)) lo.y = 0.f;
+                                    if (!((vis[c] >> (j + 2)) & 1u)) hi.x = 0.f;
+                                    if (!((vis[c] >> (j + 3)) & 1u)) hi.y = 0.f;
+                                }
                             }
-                            p[j / 2] = pack2(x[0], x[1], TO());
-                            p[j / 2 + 1] = pack2(x[2], x[3], TO());
+                            p[j / 2] = pack2(lo.x, lo.y, TO());
+                            p[j / 2 + 1] = pack2(hi.x, hi.y, TO());
                         }
                         tmem_st16(ts + c * 16, p);              // over scores that have been read
-                    }
-                    sum += (part[0] + part[1]) + (part[2] + part[3]);
-                }
-                if (drafted) {
-                    // V elements of drafted tokens that are not finite: zeroed for the matrix
-                    // instructions, added to the rows that see them at the end
-                    const uint32_t it = item_of_v(item, tl, nt), st = it % stages;
-                    ok = __all_sync(0xffffffffu, wait_or_abort(&sh->full[st], (it / stages) & 1u, abort));
-                    if (!ok) break;
-                    if (kb + row >= w.r.p0 && kb + row < w.r.len) {
-                        uint8_t* v = ring + st * L::kStage;
-                        constexpr uint32_t kExp = std::is_same<TO, __nv_bfloat16>::value ? 0x7F80u : 0x7C00u;
-                        bool found = false;
-                        for (int c = 0; c < t.c.dim / 8; ++c) {
-                            uint4* at = reinterpret_cast<uint4*>(v + chunk_at(row, c));
-                            uint4 x = *at;
-                            uint32_t* xw = &x.x;
-                            bool here = false;
-#pragma unroll
-                            for (int i = 0; i < 4; ++i) {
-                                if ((xw[i] & kExp) == kExp) {
-                                    xw[i] &= 0xFFFF0000u;
-                                    here = true;
-                                }
-                                if ((xw[i] & (kExp << 16)) == (kExp << 16)) {
-                                    xw[i] &= 0xFFFFu;
-                                    here = true;
-                                }
-                            }
-                            if (here) *at = x;
-                            found |= here;
+                        if (c & 1) {
+                            tmem_wait_st();
+                            tc_fence_before();
+                            __syncwarp();
+                            if (lane == 0) mbar_arrive(&sh->p_full[s][c >> 1]);
                         }
-                        if (found) *(volatile int*)&sh->odd[seg & 1] = 1;
                     }
-                    fence_proxy_async_smem();
+                    sum += (part0.x + part0.y) + (part1.x + part1.y);
+                } else {
+                    tc_fence_before();
+                    __syncwarp();
+                    if (lane < 2) mbar_arrive(&sh->p_full[s][lane]);
                 }
-                tmem_wait_st();
-                tc_fence_before();
-                __syncwarp();
-                if (lane == 0) mbar_arrive(&sh->p_full[s]);
             }
             // ---- the segment's result
             if (tid == 0) sh->odd[(seg + 1) & 1] = 0;
-            ok = ok && wait_or_abort(&sh->o_full, seg & 1u, abort);
-            ok = __all_sync(0xffffffffu, ok);
+            ok = __all_sync(0xffffffffu, ok && wait_or_abort(&sh->o_full, seg & 1u, abort));
             if (!ok) break;
             tc_fence_after();
             float2* swap = reinterpret_cast<float2*>(sq);       // [2][128]: Q has been used
             if (!both) swap[s * kRows + row] = make_float2(ref, sum);
-            __syncwarp();
-            if (lane == 0) mbar_arrive(&sh->joined);
-            ok = __all_sync(0xffffffffu, wait_or_abort(&sh->joined, 0u, abort));
+            join();
             if (!ok) break;
             float f0 = 1.f, f1 = 0.f;                           // factors of the two accumulators
-            if (!both && nt > 1) {
-                const float2 x = swap[row], y = swap[kRows + row];
-                const float top = fmaxf(x.x, y.x);
-                f0 = top == -INFINITY ? 1.f : ex2(x.x - top);
-                f1 = top == -INFINITY ? 1.f : ex2(y.x - top);
-                ref = top;
-                sum = x.y * f0 + y.y * f1;
-            } else if (!both) {
+            if (!both) {
                 const float2 x = swap[row];
                 ref = x.x;
                 sum = x.y;
+                if (nt > 1) {
+                    const float2 y = swap[kRows + row];
+                    ref = fmaxf(x.x, y.x);
+                    f0 = ref == -INFINITY ? 1.f : ex2(x.x - ref);
+                    f1 = ref == -INFINITY ? 1.f : ex2(y.x - ref);
+                    sum = x.y * f0 + y.y * f1;
+                }
             }
             const bool odd = *(volatile int*)&sh->odd[seg & 1] != 0;
-            // the exchange area is Q's: nobody overwrites it before everyone has read it
-            __syncwarp();
-            if (lane == 0) mbar_arrive(&sh->joined);
-            ok = __all_sync(0xffffffffu, wait_or_abort(&sh->joined, 1u, abort));
+            join();                                             // the exchange area is about to be reused
             if (!ok) break;
+            const bool whole = w.k0 == 0 && w.k1 == w.tiles;
             if (any_row) {
-                const bool whole = w.k0 == 0 && w.k1 == w.tiles;
-                const int slot = 2 * blockIdx.x + (w.k0 == 0 ? 1 : 0);
-                const int gq = (row0 + my) - token * t.group;
-                const long long qrow = w.r.lo + token;
-                const int hq = w.h * t.group + gq;
-                TQ* out = static_cast<TQ*>(t.out) + qrow * t.out_token_stride + hq * t.out_head_stride;
-                float* po = a.part_o + ((long long)slot * (kRows * qt) + my) * DP;
+                const long long slot = 2 * blockIdx.x + (w.k0 == 0 ? 1 : 0);
+                const int per = kRows * qt;
+                float4* po = a.part_o + slot * (DP / 4) * per + my;
+                uint8_t* so = sq + (my >> 7) * L::kStage;
                 const float inv = sum == 0.f ? 0.f : 1.0f / sum;
                 const int c0 = both ? 0 : s * (DP / 2), c1 = both ? DP : c0 + DP / 2;
 #pragma unroll 1
                 for (int c = c0; c < c1 && c < t.c.dim; c += 32) {
                     uint32_t v[32];
                     tmem_ld32(tmem + lanes + 256 + (both ? s * 128 : 0) + c, v);
-                    tmem_wait_ld();
                     if (!both && nt > 1) {
                         uint32_t y[32];
                         tmem_ld32(tmem + lanes + 256 + 128 + c, y);
-                        tmem_wait_ld();
+                        tmem_wait_ld(v);
+                        tmem_wait_ld(y);
 #pragma unroll
                         for (int j = 0; j < 32; ++j)
                             v[j] = __float_as_uint(__uint_as_float(v[j]) * f0 + __uint_as_float(y[j]) * f1);
+                    } else {
+                        tmem_wait_ld(v);
                     }
-                    if (my < nrows) {
-                        if (odd) {
-                            const int pages = (int)(t.c.slots / t.page_size);
-                            const int n0 = max(0, w.k0 * kTile - w.r.p0), n1 = min(w.r.len, w.k1 * kTile) - w.r.p0;
-                            for (int j = max(n0, -w.r.p0); j < n1; ++j) {
-                                if (!(t.mask ? j < 64 && ((bits >> j) & 1) : j <= token)) continue;
-                                const int pos = w.r.p0 + j, page = __ldg(t.table + (long long)w.b * t.table_stride + pos / t.page_size);
-                                if (page < 0 || page >= pages) continue;
-                                const long long at = (long long)(page * t.page_size + pos % t.page_size) * t.c.slot_stride +
-                                                     (long long)w.h * t.c.head_stride + c;
+                    if (odd && my < nrows) {
+                        const int pages = (int)(t.c.slots / t.page_size);
+                        const int n0 = max(max(0, w.k0 * kTile - w.r.p0), -w.r.p0), n1 = min(w.r.len, w.k1 * kTile) - w.r.p0;
+                        for (int j = n0; j < n1; ++j) {
+                            if (!(t.mask ? j < 64 && ((bits >> j) & 1) : j <= token)) continue;
+                            const int pos = w.r.p0 + j;
+                            const int page = __ldg(t.table + (long long)w.b * t.table_stride + pos / t.page_size);
+                            if (page < 0 || page >= pages) continue;
+                            const long long at = (long long)(page * t.page_size + pos % t.page_size) * t.c.slot_stride +
+                                                 (long long)w.h * t.c.head_stride + c;
 #pragma unroll
-                                for (int d = 0; d < 32; ++d) {
-                                    if (c + d >= t.c.dim) break;
-                                    float x;
-                                    if constexpr (kFp8) {
-                                        const uint8_t q8 = static_cast<const uint8_t*>(t.c.v)[at + d];
-                                        x = (q8 & 0x7F) == 0x7F ? __int_as_float(0x7fffffff) : 0.f;
-                                    } else {
-                                        x = (float)static_cast<const TQ*>(t.c.v)[at + d];
-                                        if (fabsf(x) < __int_as_float(0x7f800000)) x = 0.f;
-                                    }
-                                    v[d] = __float_as_uint(__uint_as_float(v[d]) + x);
+                            for (int d = 0; d < 32; ++d) {
+                                if (c + d >= t.c.dim) break;
+                                float x;
+                                if constexpr (kFp8) {
+                                    const uint8_t q8 = static_cast<const uint8_t*>(t.c.v)[at + d];
+                                    x = (q8 & 0x7F) == 0x7F ? __int_as_float(0x7fffffff) : 0.f;
+                                } else {
+                                    x = (float)static_cast<const TQ*>(t.c.v)[at + d];
+                                    if (fabsf(x) < __int_as_float(0x7f800000)) x = 0.f;
                                 }
+                                v[d] = __float_as_uint(__uint_as_float(v[d]) + x);
                             }
                         }
-                        if (whole) {
+                    }
+                    if (whole) {
 #pragma unroll
-                            for (int j = 0; j < 32; j += 8) {
-                                if (c + j >= t.c.dim) break;
-                                uint32_t p[4];
+                        for (int j = 0; j < 32; j += 8) {
+                            uint32_t p[4];
 #pragma unroll
-                                for (int i = 0; i < 4; ++i)
-                                    p[i] = pack2(__uint_as_float(v[j + 2 * i]) * inv, __uint_as_float(v[j + 2 * i + 1]) * inv, TQ());
-                                *reinterpret_cast<uint4*>(out + c + j) = make_uint4(p[0], p[1], p[2], p[3]);
-                            }
-                        } else {
-#pragma unroll
-                            for (int j = 0; j < 32; j += 4)
-                                *reinterpret_cast<uint4*>(po + c + j) = make_uint4(v[j], v[j + 1], v[j + 2], v[j + 3]);
+                            for (int i = 0; i < 4; ++i)
+                                p[i] = pack2(__uint_as_float(v[j + 2 * i]) * inv, __uint_as_float(v[j + 2 * i + 1]) * inv, TQ());
+                            *reinterpret_cast<uint4*>(so + chunk_at(row, (c + j) / 8)) = make_uint4(p[0], p[1], p[2], p[3]);
                         }
+                    } else if (my < nrows) {
+#pragma unroll
+                        for (int j = 0; j < 32; j += 4)
+                            po[(c + j) / 4 * per] = make_float4(__uint_as_float(v[j]), __uint_as_float(v[j + 1]),
+                                                                __uint_as_float(v[j + 2]), __uint_as_float(v[j + 3]));
                     }
                 }
                 if (my < nrows && (both || s == 0)) {
                     if (!whole)
-                        a.part_ml[(long long)slot * (kRows * qt) + my] = make_float2(ref, sum);
+                        a.part_ml[slot * per + my] = make_float2(ref, sum);
                     else if (t.lse)
-                        t.lse[qrow * t.q_heads + hq] = sum == 0.f ? -INFINITY : (ref + log2f(sum)) * kLn2;
+                        t.lse[(long long)(w.r.lo + token) * t.q_heads + w.h * t.group + gq] =
+                            sum == 0.f ? -INFINITY : (ref + log2f(sum)) * kLn2;
+                }
+            }
+            if (whole) {
+                // rows leave through shared memory, 16 bytes a thread and whole rows a warp; each
+                // thread later writes the next Q where it has read here
+                join();
+                if (!ok) break;
+                TQ* out = static_cast<TQ*>(t.out) + sub * 8;
+                if (sub_live) {
+#pragma unroll 4
+                    for (int r = r_first; r < nrows; r += kStep)
+                        *reinterpret_cast<uint4*>(out + q_offset(r, t.out_token_stride, t.out_head_stride)) =
+                            *reinterpret_cast<const uint4*>(sq + (r >> 7) * L::kStage + chunk_at(r & 127, sub));
                 }
             }
             tc_fence_before();
@@ -1084,7 +1143,8 @@ __global__ void __launch_bounds__(threads<kFp8>(), 1) attn_kernel(const __grid_c
 }
 
 // ---- joining the parts of an item ------------------------------------------------------------
-// CTAs first..last hold parts of an item; the blocks first + 1..last share its rows, a warp a row.
+// CTAs first..last hold parts of an item; the blocks (first + 1..last, y) share its rows and
+// columns, four columns a thread, rows adjacent as the parts have them.
 constexpr int kCombineThreads = 128;
 
 template <typename TQ, int DP>
@@ -1093,56 +1153,39 @@ __global__ void __launch_bounds__(kCombineThreads) combine_kernel(const __grid_c
     const Split sp = a.splits[blockIdx.x];
     if (!sp.valid) return;
     const TreeAttnArgs& t = a.t;
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const Request r = request_of(t, a.qt, sp.b);
     const int row0 = sp.block * kRows * a.qt, nrows = min(r.rows - row0, kRows * a.qt);
     const int parts = sp.last - sp.first + 1, per = kRows * a.qt;
-    constexpr int kCols = DP / 32;
-    constexpr int kWarps = kCombineThreads / 32;
-    for (int row = ((int)blockIdx.x - sp.first - 1) * kWarps + warp; row < nrows; row += (parts - 1) * kWarps) {
+    const int workers = (parts - 1) * gridDim.y * kCombineThreads;
+    for (int u = (((int)blockIdx.x - sp.first - 1) * gridDim.y + blockIdx.y) * kCombineThreads + threadIdx.x;
+         u < nrows * (t.c.dim / 4); u += workers) {
+        const int c4 = u / nrows, row = u - c4 * nrows;
+        const float2* ml = a.part_ml + row;
+        const float4* po = a.part_o + c4 * per + row;
+        auto slot_of = [&](int p) { return (long long)(2 * (sp.first + p) + (p == 0)); };
         float top = -INFINITY;
-        for (int p = lane; p < parts; p += 32) {
-            const int slot = 2 * (sp.first + p) + (p == 0);
-            top = fmaxf(top, __ldcg(&a.part_ml[(long long)slot * per + row]).x);
-        }
-#pragma unroll
-        for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-        float sum = 0.f, acc[kCols];
-#pragma unroll
-        for (int i = 0; i < kCols; ++i) acc[i] = 0.f;
+#pragma unroll 4
+        for (int p = 0; p < parts; ++p) top = fmaxf(top, __ldcg(ml + slot_of(p) * per).x);
+        float sum = 0.f, acc[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll 4
         for (int p = 0; p < parts; ++p) {
-            const long long at = (long long)(2 * (sp.first + p) + (p == 0)) * per + row;
-            const float2 ml = __ldcg(&a.part_ml[at]);
-            const float f = top == -INFINITY ? 1.f : ex2(ml.x - top);
-            sum += ml.y * f;
-            float x[kCols];
-            if constexpr (kCols == 4) {
-                const float4 v = __ldcg(reinterpret_cast<const float4*>(a.part_o + at * DP) + lane);
-                x[0] = v.x;
-                x[1] = v.y;
-                x[2] = v.z;
-                x[3] = v.w;
-            } else {
-                const float2 v = __ldcg(reinterpret_cast<const float2*>(a.part_o + at * DP) + lane);
-                x[0] = v.x;
-                x[1] = v.y;
-            }
-#pragma unroll
-            for (int i = 0; i < kCols; ++i) acc[i] = fmaf(x[i], f, acc[i]);
+            const float2 m = __ldcg(ml + slot_of(p) * per);
+            const float4 x = __ldcg(po + slot_of(p) * (DP / 4) * per);
+            const float f = top == -INFINITY ? 1.f : ex2(m.x - top);
+            sum = fmaf(m.y, f, sum);
+            acc[0] = fmaf(x.x, f, acc[0]);
+            acc[1] = fmaf(x.y, f, acc[1]);
+            acc[2] = fmaf(x.z, f, acc[2]);
+            acc[3] = fmaf(x.w, f, acc[3]);
         }
         const int token = (row0 + row) / t.group;
         const long long qrow = r.lo + token;
         const int hq = sp.h * t.group + (row0 + row) - token * t.group;
         const float inv = sum == 0.f ? 0.f : 1.0f / sum;
-        TQ* out = static_cast<TQ*>(t.out) + qrow * t.out_token_stride + hq * t.out_head_stride + lane * kCols;
-        if (lane * kCols < t.c.dim) {
-#pragma unroll
-            for (int i = 0; i < kCols; i += 2)
-                *reinterpret_cast<uint32_t*>(out + i) = pack2(acc[i] * inv, acc[i + 1] * inv, TQ());
-        }
-        if (lane == 0 && t.lse)
-            t.lse[qrow * t.q_heads + hq] = sum == 0.f ? -INFINITY : (top + log2f(sum)) * kLn2;
+        TQ* out = static_cast<TQ*>(t.out) + qrow * t.out_token_stride + hq * t.out_head_stride + 4 * c4;
+        *reinterpret_cast<uint2*>(out) =
+            make_uint2(pack2(acc[0] * inv, acc[1] * inv, TQ()), pack2(acc[2] * inv, acc[3] * inv, TQ()));
+        if (c4 == 0 && t.lse) t.lse[qrow * t.q_heads + hq] = sum == 0.f ? -INFINITY : (top + log2f(sum)) * kLn2;
     }
 }
 
@@ -1162,12 +1205,15 @@ int launch(const KernelArgs& a, int sms, cudaStream_t st) {
     if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess)
         return kLaunchFailed;
     const int grid = sms < kMaxCtas ? sms : kMaxCtas;
-    kern<<<grid, threads<kFp8>(), smem, st>>>(a);
+    kern<<<grid, kThreads, smem, st>>>(a);
     if (cudaGetLastError() != cudaSuccess) return kLaunchFailed;
     // items of one tile are never cut
     if ((long long)a.t.max_pages * a.t.page_size <= kTile) return kOk;
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(grid);
+    // two units of four columns a thread where an item is cut in two
+    const long long rows = (long long)a.t.group * a.t.width;
+    const long long units = (rows < kRows * a.qt ? rows : kRows * a.qt) * (a.t.c.dim / 4);
+    cfg.gridDim = dim3(grid, (unsigned)((units + 2 * kCombineThreads - 1) / (2 * kCombineThreads)));
     cfg.blockDim = dim3(kCombineThreads);
     cfg.stream = st;
     cudaLaunchAttribute attr[1];
@@ -1194,7 +1240,7 @@ int launch_tree_attn(const TreeAttnArgs& t, int dtype, cudaStream_t st) {
     char* ws = static_cast<char*>(t.ws);
     a.splits = reinterpret_cast<Split*>(ws);
     a.part_ml = reinterpret_cast<float2*>(ws + kSplitBytes);
-    a.part_o = reinterpret_cast<float*>(ws + kSplitBytes + kMlBytes(a.qt));
+    a.part_o = reinterpret_cast<float4*>(ws + kSplitBytes + kMlBytes(a.qt));
     int dev = 0, sms = 0;
     if (cudaGetDevice(&dev) != cudaSuccess ||
         cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess)

@@ -461,7 +461,8 @@ int dsv_kv_read(int64_t tokens, const void* slots, int32_t slots_int64, const ds
  * (drafted tokens from 64 on: never), or, with tree_mask NULL, where j <= i.
  * out[row, head] = sum softmax(scale * q . k) v over those, rounded once to dtype; lse [rows,
  * q_heads] fp32 (may be NULL) the natural logsumexp of the scaled scores.  A row that sees
- * nothing gets zeros and -inf.  Query head hq reads KV head hq / (q_heads / heads).
+ * nothing gets zeros and -inf.  Query head hq reads KV head hq / (q_heads / heads)
+ * (at most 4096 of them each).
  * dtype (q and out) DSV_BF16 or DSV_F16; the cache has the same type or is e4m3; dim a multiple
  * of 16, at most 128; cache->slots a multiple of page_size; scale positive and finite.  `width`
  * is with q_indptr a bound on the rows of a request, by which the work is laid out (a request
