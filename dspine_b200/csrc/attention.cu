@@ -12,20 +12,23 @@
 //
 //   attn_kernel     persistent, one CTA per SM.  The rows of one (request, KV head), t_b tokens x
 //                   `group` query heads, are the M = 128 rows of the matrix instructions, so a key
-//                   is read once for all of them.  The tiles of 128 keys of all (request, KV head,
+//                   is read once for all of them.  The tiles of 64 keys of all (request, KV head,
 //                   row block) items form one line that is cut into equal pieces, one per CTA:
 //                   every SM streams the same number of tiles however ragged the lengths are.
-//                     warps 0-7    two softmax warpgroups, one TMEM lane (row) per thread, its 128
-//                                  scores in registers
-//                     warp 8       TMEM allocation and the MMA issuer (its warpgroup is else idle)
-//                     warps 12-15  producers: K and V rows of a tile, slot by slot, into a ring of
+//                     warps 0-7    two softmax warpgroups, one TMEM lane (row) per thread, its
+//                                  scores of a tile in registers
+//                     warp 8       TMEM allocation and the MMA issuer
+//                     warp 9       index: slots, scales and validity of the tiles to come
+//                     warps 10..   producers: K and V rows of a tile, slot by slot, into a ring of
 //                                  128-byte-swizzled shared-memory stages
 //                   S = Q K^T (kind::f16, both operands in shared memory) and O += P V (P from
 //                   TMEM, written over S; V as a matrix with rows of keys, "MN-major").
 //                   Two streams keep the tensor core and the exponentials busy at once: with more
 //                   than 128 rows each warpgroup owns 128 of them and both use every tile, else
 //                   both own the same rows and take every other tile, with an accumulator each,
-//                   joined at the end.
+//                   joined at the end.  Each stream has two score buffers, so the scores of its
+//                   next tile are computed while it works on one: with tiles of 128 keys and one
+//                   buffer the chain scores -> weights -> accumulate -> scores set the pace.
 //   combine_kernel  joins the partial results of items that a cut went through.
 //
 // Softmax: weights are 2^(s c - ref), c = scale log2(e), ref a running reference that follows the
@@ -58,67 +61,37 @@ namespace dsv {
 namespace attn {
 
 constexpr int kRows = 128;                 // rows of a Q tile (MMA M)
-constexpr int kTile = 128;                 // keys of a tile
-constexpr int kBlock = kTile * 128;        // bytes of a [128 rows][128 bytes] swizzled block
+constexpr int kTile = 64;                  // keys of a tile
+constexpr int kQBlock = kRows * 128;       // bytes of a [128 rows][128 bytes] swizzled block of Q
+constexpr int kBlock = kTile * 128;        // the same of a K or V tile
 constexpr int kMaxCtas = 148;              // SMs of a B200; partial results are laid out for these
-constexpr int kInfo = 8;                   // tiles whose validity and scales are held at once
+constexpr int kInfo = 16;                  // tiles that are described in shared memory at once
+constexpr int kBatch = 4;                  // tiles that the index warp looks up at once
+constexpr int kAheadUnits = 4;             // score tiles in TMEM: two streams x two buffers
 constexpr int kSoftmaxThreads = 256;
-constexpr int kMinTiles = 2;               // tiles per CTA below which fewer CTAs take part
+constexpr int kMinTiles = 4;               // tiles per CTA below which fewer CTAs take part
 constexpr float kSlack = 8.0f;             // log2 by which a maximum may outgrow the reference
 constexpr float kL2E = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
 
-constexpr int kProducers = 4;              // producer warps
-constexpr int kThreads = 512;              // four warpgroups: softmax, softmax, MMA issuer, producers
+// warps 0-7 softmax, 8 MMA issuer, 9 index, 10.. producers
+constexpr int kMmaWarp = 8, kIndexWarp = 9, kFirstProducer = 10;
+template <bool kFp8> constexpr int producers() { return kFp8 ? 6 : 4; }
+template <bool kFp8> constexpr int threads() { return 32 * (kFirstProducer + producers<kFp8>()); }
 
-// one slot of the tile ring beside the stages
-struct TileInfo {
-    uint32_t valid[4];        // positions of the tile that exist and can be read
-    float vmax[kProducers];   // e4m3: largest finite V scale, per producer warp
-    float ks[kTile];          // e4m3: K scale x scale x log2(e)
-    float vs[kTile];          // e4m3: V scale
+// a tile of keys, as the index warp describes it to the others
+struct alignas(16) TileInfoPlain {
+    int slot[kTile];          // of each position; -1 where there is none or it cannot be read
+    uint32_t valid[2];        // the positions with a slot
+    int head, tiles, ahead;   // of the segment: KV head, tiles, K tiles loaded before its first V tile
+    float vmax;               // e4m3: largest finite V scale
 };
-struct TileInfoPlain {
-    uint32_t valid[4];
+struct TileInfoScaled : TileInfoPlain {
+    alignas(16) float ks[kTile];   // K scale x scale x log2(e)
+    alignas(16) float vs[kTile];   // V scale
 };
 template <bool kFp8> struct InfoOf { using type = TileInfoPlain; };
-template <> struct InfoOf<true> { using type = TileInfo; };
-
-constexpr int kMaxStages = 12;
-
-struct alignas(16) Shared {
-    uint64_t full[kMaxStages];   // stage holds a K or V tile
-    uint64_t empty[kMaxStages];  // the matrix instructions that read it are done
-    uint64_t info[kInfo];        // TileInfo written
-    uint64_t q_full;             // Q of the segment in shared memory, last segment's TMEM read
-    uint64_t s_full[2];          // scores of a stream's tile in TMEM
-    uint64_t p_full[2][2];       // weights of a stream's tile in TMEM: its first and second 64 keys
-    uint64_t o_full;             // the segment's accumulators are complete
-    uint64_t joined;             // both warpgroups have written what the other reads
-    uint64_t drain;
-    uint32_t tmem;
-    int abort;
-    int odd[2];                  // a drafted V element was not finite (by segment parity)
-    // where this CTA starts on the line of tiles
-    int start_b;
-    long long start_in_b;
-    long long scan[32];
-};
-
-template <int DP, bool kFp8> struct Layout {
-    static constexpr int kStage = (DP / 64) * kBlock;      // bytes of a K or V stage
-    static __host__ __device__ constexpr int stages(int qt) {
-        return DP == 128 ? (kFp8 ? 6 - qt : 7 - qt) : (kFp8 ? 8 : 12);
-    }
-    static constexpr size_t info_bytes = sizeof(typename InfoOf<kFp8>::type) * kInfo;
-    static constexpr size_t smem(int qt) {
-        return (size_t)(qt + stages(qt)) * kStage + sizeof(Shared) + info_bytes + (kFp8 ? 1024 : 0) + 1024;
-    }
-};
-static_assert(Layout<128, false>::smem(1) <= 232448 && Layout<128, false>::smem(2) <= 232448 &&
-                  Layout<128, true>::smem(1) <= 232448 && Layout<128, true>::smem(2) <= 232448 &&
-                  Layout<64, false>::smem(2) <= 232448 && Layout<64, true>::smem(2) <= 232448,
-              "shared memory of one CTA");
+template <> struct InfoOf<true> { using type = TileInfoScaled; };
 
 // ---- partial results ------------------------------------------------------------------------
 // CTA c has two slots: 2c for a segment that continues an item, 2c + 1 for one that begins an item
@@ -187,10 +160,13 @@ __device__ __forceinline__ long long tiles_of_head(const TreeAttnArgs& a, int qt
     return n;
 }
 
-__device__ __forceinline__ long long first_tile(long long c, long long total, int ctas) { return c * total / ctas; }
+__device__ __forceinline__ long long first_tile(long long c, long long total, int ctas) {
+    return total < (1 << 24) ? (long long)((uint32_t)c * (uint32_t)total / (uint32_t)ctas) : c * total / ctas;
+}
 // the CTA whose piece holds tile x
 __device__ __forceinline__ int cta_of(long long x, long long total, int ctas) {
-    return (int)(((x + 1) * ctas - 1) / total);
+    return total < (1 << 24) ? (int)(((uint32_t)(x + 1) * (uint32_t)ctas - 1u) / (uint32_t)total)
+                             : (int)(((x + 1) * ctas - 1) / total);
 }
 
 // The segments (runs of tiles of one item) of a CTA, in order.  Every warp walks them by itself.
@@ -202,11 +178,15 @@ struct Walk {
     long long left;         // tiles of this CTA after this segment
     int next_k0;            // where the item goes on
 
-    __device__ __forceinline__ void begin(const KernelArgs& a, int b0, long long in_b, long long count) {
+    // tile in_b of request b0's tiles (per_head of them for each KV head)
+    __device__ __forceinline__ void begin(const KernelArgs& a, int b0, const Request& r0, long long per_head, long long in_b,
+                                          long long count) {
         b = b0;
-        r = request_of(a.t, a.qt, b);
-        const long long per_head = tiles_of_head(a.t, a.qt, r);
-        h = (int)(in_b / per_head);
+        r = r0;
+        if (in_b < 0x7fffffff && per_head < 0x7fffffff)
+            h = (int)((uint32_t)in_b / (uint32_t)per_head);
+        else
+            h = (int)(in_b / per_head);
         long long at = in_b - h * per_head;
         block = 0;
         tiles = tiles_of(a.t, a.qt, r, 0);
@@ -247,6 +227,41 @@ struct Walk {
     __device__ __forceinline__ bool shared_rows(int qt) const { return rows(qt) <= kRows; }
 };
 
+constexpr int kMaxStages = 12;
+
+struct alignas(16) Shared {
+    uint64_t full[kMaxStages];       // stage holds a K or V tile
+    uint64_t empty[kMaxStages];      // the matrix instructions that read it are done
+    uint64_t info_full[kInfo];       // tile described
+    uint64_t info_empty[kInfo];      // its last matrix instructions are done
+    uint64_t q_full;                 // Q of the segment in shared memory, last segment's TMEM read
+    uint64_t s_full[2][2];           // scores of a stream's buffer in TMEM
+    uint64_t p_full[2][2];           // weights of a stream's buffer in TMEM
+    uint64_t pv_done[2];             // a stream's last weights have been accumulated
+    uint64_t o_full;                 // the segment's accumulators are complete
+    uint64_t joined;                 // both warpgroups have written what the other reads
+    uint64_t drain;
+    uint32_t tmem;
+    int abort;
+    int odd[2];                      // a drafted V element was not finite (by segment parity)
+    long long scan[32];
+    Walk start;                      // where this CTA starts on the line of tiles
+};
+
+template <int DP, bool kFp8> struct Layout {
+    static constexpr int kQTile = (DP / 64) * kQBlock;     // bytes of a Q tile
+    static constexpr int kStage = (DP / 64) * kBlock;      // bytes of a K or V stage
+    static __host__ __device__ constexpr int stages(int qt) { return DP == 128 ? 13 - 2 * qt : 12; }
+    static constexpr size_t info_bytes = sizeof(typename InfoOf<kFp8>::type) * kInfo;
+    static constexpr size_t smem(int qt) {
+        return (size_t)qt * kQTile + (size_t)stages(qt) * kStage + sizeof(Shared) + info_bytes + (kFp8 ? 1024 : 0) + 1024;
+    }
+};
+static_assert(Layout<128, false>::smem(1) <= 232448 && Layout<128, false>::smem(2) <= 232448 &&
+                  Layout<128, true>::smem(1) <= 232448 && Layout<128, true>::smem(2) <= 232448 &&
+                  Layout<64, false>::smem(2) <= 232448 && Layout<64, true>::smem(2) <= 232448,
+              "shared memory of one CTA");
+
 // ---- PTX helpers ------------------------------------------------------------------------------
 
 // Order between the threads' writes to shared memory and the matrix instructions' reads (another
@@ -266,23 +281,28 @@ __device__ __forceinline__ uint64_t desc(uint32_t low) { return ((uint64_t)kDesc
 __device__ __forceinline__ void tc_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void tc_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
 
+// Executed by the whole warp, issued by one elected lane: outside a divergent branch the operands
+// stay in uniform registers, where the instruction wants them (issued from `if (lane == 0)` each
+// took 90 cycles).
 __device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
     asm volatile(
-        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-        "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d), "l"(a), "l"(b), "r"(idesc),
+        "{\n\t.reg .pred p, one;\n\tsetp.ne.b32 p, %4, 0;\n\telect.sync _|one, 0xffffffff;\n\t"
+        "@one tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d), "l"(a), "l"(b), "r"(idesc),
         "r"(accumulate)
         : "memory");
 }
 __device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
     asm volatile(
-        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d), "r"(a), "l"(b), "r"(idesc),
+        "{\n\t.reg .pred p, one;\n\tsetp.ne.b32 p, %4, 0;\n\telect.sync _|one, 0xffffffff;\n\t"
+        "@one tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d), "r"(a), "l"(b), "r"(idesc),
         "r"(accumulate)
         : "memory");
 }
 __device__ __forceinline__ void mma_commit(uint64_t* bar) {
-    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(bar))
-                 : "memory");
+    asm volatile(
+        "{\n\t.reg .pred one;\n\telect.sync _|one, 0xffffffff;\n\t"
+        "@one tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}" ::"r"(smem_u32(bar))
+        : "memory");
 }
 __device__ __forceinline__ void mbar_arrive(uint64_t* bar) {
     asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(bar)) : "memory");
@@ -356,6 +376,14 @@ __device__ __forceinline__ void cp16(uint32_t dst, const void* src, bool ok) {
     asm volatile("cp.async.cg.shared.global.L2::128B [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(ok ? 16 : 0)
                  : "memory");
 }
+// 16 bytes that are read once: past L1, where they would push out what the warps spill there
+__device__ __forceinline__ uint4 ld16_once(const void* p) {
+    uint4 v;
+    asm("ld.global.nc.L1::no_allocate.L2::128B.v4.u32 {%0, %1, %2, %3}, [%4];"
+        : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
+        : "l"(p));
+    return v;
+}
 // arrives at `bar` once this thread's copies so far have landed
 __device__ __forceinline__ void cp_arrive(uint64_t* bar) {
     asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
@@ -363,8 +391,7 @@ __device__ __forceinline__ void cp_arrive(uint64_t* bar) {
 __device__ __forceinline__ void cp_wait_all() { asm volatile("cp.async.wait_all;" ::: "memory"); }
 
 // bounded wait that also gives up when another warp of the CTA has given up
-__device__ __forceinline__ bool wait_or_abort(uint64_t* bar, uint32_t parity, volatile int* abort) {
-    if (mbar_try_wait(bar, parity)) return true;
+__device__ __noinline__ bool wait_slow(uint64_t* bar, uint32_t parity, volatile int* abort) {
     const uint64_t t0 = globaltimer_ns();
     for (uint32_t i = 1;; ++i) {
         if (mbar_try_wait(bar, parity)) return true;
@@ -376,103 +403,64 @@ __device__ __forceinline__ bool wait_or_abort(uint64_t* bar, uint32_t parity, vo
         }
     }
 }
-
-template <int N> __device__ __forceinline__ void regs_down() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N)); }
-template <int N> __device__ __forceinline__ void regs_up() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N)); }
-
-// 16-byte chunk c of row `row` in a tile of 128-byte-swizzled blocks
-__device__ __forceinline__ uint32_t chunk_at(int row, int c) {
-    return (uint32_t)((c >> 3) * kBlock + row * 128 + (((c ^ row) & 7) << 4));
+__device__ __forceinline__ bool wait_or_abort(uint64_t* bar, uint32_t parity, volatile int* abort) {
+    return mbar_try_wait(bar, parity) || wait_slow(bar, parity, abort);
 }
 
-// ---- the tiles of a CTA, in the order they are loaded -------------------------------------------
-// per segment of n tiles: K0, K1, V0, K2, V1, ..., K(n-1), V(n-2), V(n-1): the order in which the
-// matrix instructions use them (the scores of a tile are computed one tile ahead of its V).
-__device__ __forceinline__ uint32_t item_of_k(uint32_t base, int t) { return base + (t == 0 ? 0 : 2 * t - 1); }
-__device__ __forceinline__ uint32_t item_of_v(uint32_t base, int t, int n) { return base + (t == n - 1 ? 2 * n - 1 : 2 * t + 2); }
+// 16-byte chunk c of row `row` in a tile of 128-byte-swizzled blocks of `block` bytes
+template <int block>
+__device__ __forceinline__ uint32_t chunk_at(int row, int c) {
+    return (uint32_t)((c >> 3) * block + row * 128 + (((c ^ row) & 7) << 4));
+}
 
-// A producer warp's view: which tile comes next, and the slot of the lane's token in it.
-template <int kTokens>  // tokens of a tile that one warp loads (lane l looks after token l % kTokens)
-struct Tiles {
-    Walk w;
-    int i, n;                 // item of the segment, tiles of the segment
-    int token;
-    int cur, prev, ahead;     // slots: the newest tile's, the one before, the one after (-1: none)
-    uint32_t tile;            // tiles begun so far
-    bool is_k;
-
-    __device__ __forceinline__ int slot_of(const KernelArgs& a, int t) const {
-        const int pos = (w.k0 + t) * kTile + token;
-        if (t >= n || pos >= w.r.len) return -1;
-        const int page = pos / a.t.page_size;
-        const int entry = __ldg(a.t.table + (long long)w.b * a.t.table_stride + page);
-        const int pages = (int)(a.t.c.slots / a.t.page_size);
-        if (entry < 0 || entry >= pages) {
-            if (a.t.err) atomicOr(a.t.err, 2u);
-            return -1;
-        }
-        return entry * a.t.page_size + (pos - page * a.t.page_size);
-    }
-    __device__ __forceinline__ void begin(const KernelArgs& a, const Walk& from, int tok) {
-        w = from;
-        token = tok;
-        i = -1;
-        n = w.count();
-        tile = 0;
-        cur = prev = -1;
-        ahead = slot_of(a, 0);
-    }
-    // the next item; false at the end
-    __device__ __forceinline__ bool next(const KernelArgs& a) {
-        if (++i == 2 * n) {
-            if (!w.advance(a)) return false;
-            i = 0;
-            n = w.count();
-            ahead = slot_of(a, 0);
-        }
-        is_k = i == 0 || ((i & 1) && i != 2 * n - 1);
-        if (is_k) {
-            prev = cur;
-            cur = ahead;
-            ahead = slot_of(a, ((i + 1) >> 1) + 1);
-            ++tile;
-        }
-        return true;
-    }
-    // slot of the lane's token in this item
-    __device__ __forceinline__ int slot() const { return is_k || i == 2 * n - 1 ? cur : prev; }
-};
+// ---- the order of the tiles ---------------------------------------------------------------------
+// A unit is one stream's share of a tile: unit u belongs to stream u & 1 and uses its score buffer
+// (u >> 1) & 1; its tile is u, or u >> 1 where both streams use every tile.  The scores of unit
+// u + 4 are issued behind the accumulation of unit u, so that two score tiles of each stream are in
+// work; K tiles are therefore loaded `ahead` tiles before V: K0 .. K(ahead-1), V0, K(ahead), V1, ...
+__device__ __forceinline__ int item_of_k(int t, int ahead) { return t < ahead ? t : 2 * t - ahead + 1; }
+__device__ __forceinline__ int item_of_v(int t, int n, int ahead) {
+    return n <= ahead ? n + t : ahead + t + min(t, n - ahead);
+}
 
 // ---- the kernel ---------------------------------------------------------------------------------
 
 template <typename TQ, bool kFp8, int DP>
-__global__ void __launch_bounds__(kThreads, 1) attn_kernel(const __grid_constant__ KernelArgs a) {
+__global__ void __launch_bounds__(threads<kFp8>(), 1) attn_kernel(const __grid_constant__ KernelArgs a) {
     using L = Layout<DP, kFp8>;
     using Info = typename InfoOf<kFp8>::type;
     using TO = typename std::conditional<kFp8, __half, TQ>::type;   // operands of the matrix instructions
+    constexpr int kThreads = threads<kFp8>();
+    constexpr int kProducers = producers<kFp8>();
+    constexpr int kElem = kFp8 ? 1 : 2;                    // bytes of a cached element
     extern __shared__ uint8_t smem_raw[];
     const int qt = a.qt, stages = L::stages(qt);
     uint8_t* base = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
-    uint8_t* sq = base;                                    // [qt][kStage]
-    uint8_t* ring = base + qt * L::kStage;                 // [stages][kStage]
+    uint8_t* sq = base;                                    // [qt][kQTile]
+    uint8_t* ring = base + qt * L::kQTile;                 // [stages][kStage]
     Shared* sh = reinterpret_cast<Shared*>(ring + stages * L::kStage);
     Info* info = reinterpret_cast<Info*>(sh + 1);
     float* row_mul = reinterpret_cast<float*>(info + kInfo);        // e4m3: [128 qt] power of two of a row of q
     volatile int* abort = &sh->abort;
-    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;
     const TreeAttnArgs& t = a.t;
 
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
 
-    if (tid == 0) a.splits[blockIdx.x].valid = 0;
+    if (tid == 0) a.splits[blockIdx.x].valid = 0;     // before the scan's barrier, after which it may be set
 
     // ---- this CTA's piece of the line of tiles: a block scan over the requests' tiles, a second
-    // one (another round over the requests) only where they are more than the threads
-    long long total = 0, c = 0, upto = 0;                 // of all; of this thread's request; up to it
+    // round over the requests only where they are more than the threads
+    long long total = 0, per_head = 0, c = 0, upto = 0;   // of all; of this thread's request; up to it
+    Request rq;
     auto scan = [&](int b0) {
         const int b = b0 + tid;
-        c = 0;
-        if (b < t.batch) c = tiles_of_head(t, qt, request_of(t, qt, b)) * t.c.heads;
+        c = per_head = 0;
+        if (b < t.batch) {
+            rq = request_of(t, qt, b);
+            per_head = tiles_of_head(t, qt, rq);
+            c = per_head * t.c.heads;
+        }
         upto = c;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
@@ -511,23 +499,34 @@ __global__ void __launch_bounds__(kThreads, 1) attn_kernel(const __grid_constant
                 before += all;
             }
             if (c > 0 && mine >= upto - c && mine < upto) {
-                sh->start_b = b0 + tid;
-                sh->start_in_b = mine - (upto - c);
+                Walk w0;
+                w0.begin(a, b0 + tid, rq, per_head, mine - (upto - c), count);
+                sh->start = w0;
+                if (w0.k0 > 0) {
+                    const long long i0 = mine - w0.k0;
+                    Split sp = {1, w0.b, w0.h, w0.block, cta_of(i0, total, ctas), cta_of(i0 + w0.tiles - 1, total, ctas), {0, 0}};
+                    a.splits[blockIdx.x] = sp;
+                }
             }
         }
     }
 
     if (tid == 0) {
         for (int s = 0; s < stages; ++s) {
-            mbar_init(&sh->full[s], kFp8 ? kProducers : kProducers * 32);
+            mbar_init(&sh->full[s], kFp8 ? 1 : 32);
             mbar_init(&sh->empty[s], 1);
         }
-        for (int i = 0; i < kInfo; ++i) mbar_init(&sh->info[i], kProducers);
+        for (int i = 0; i < kInfo; ++i) {
+            mbar_init(&sh->info_full[i], 1);
+            mbar_init(&sh->info_empty[i], 1);
+        }
         mbar_init(&sh->q_full, 8);
         for (int i = 0; i < 2; ++i) {
-            mbar_init(&sh->s_full[i], 1);
-            mbar_init(&sh->p_full[i][0], 4);
-            mbar_init(&sh->p_full[i][1], 4);
+            for (int j = 0; j < 2; ++j) {
+                mbar_init(&sh->s_full[i][j], 1);
+                mbar_init(&sh->p_full[i][j], 4);
+            }
+            mbar_init(&sh->pv_done[i], 1);
         }
         mbar_init(&sh->o_full, 1);
         mbar_init(&sh->joined, 8);
@@ -536,7 +535,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_kernel(const __grid_constant
         sh->odd[0] = sh->odd[1] = 0;
         fence_mbar_init();
     }
-    if (warp == 8) {
+    if (warp == kMmaWarp) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_u32(&sh->tmem))
                      : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
@@ -544,150 +543,176 @@ __global__ void __launch_bounds__(kThreads, 1) attn_kernel(const __grid_constant
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
-    const uint32_t tmem = sh->tmem;
-    Walk w;
-    w.begin(a, sh->start_b, sh->start_in_b, count);
-    if (tid == 0 && w.k0 > 0) {
-        const long long i0 = mine - w.k0;
-        Split s = {1, w.b, w.h, w.block, cta_of(i0, total, ctas), cta_of(i0 + w.tiles - 1, total, ctas), {0, 0}};
-        a.splits[blockIdx.x] = s;
-    }
+    constexpr uint32_t tmem = 0;                           // all 512 columns were allocated
+    Walk w = sh->start;
 
-    if (warp >= 12) {
-        // ---------------- producers ----------------
-        if constexpr (!kFp8) regs_down<56>();
-        const int pw = warp - 12;
-        constexpr int kTokens = kTile / kProducers;             // tokens of a tile per warp
-        Tiles<kTokens> g;
-        g.begin(a, w, pw * kTokens + (lane & (kTokens - 1)));
-        uint32_t n = 0;
+    if (warp >= kFirstProducer) {
+        // ---------------- producers: a warp takes whole items (a tile of K or of V), in turn -------
+        // One copy of this loop serves every item: unrolled over register buffers instead, its code
+        // pushed the other warps' out of the instruction cache (64x16 e4m3 458 us).
+        uint32_t item = warp - kFirstProducer;                  // of the CTA
+        int i = (int)item, base = 0, n = 0, ahead = 0;          // item of the segment, first tile, tiles, lead of K
         bool ok = true;
-        if constexpr (!kFp8) {
-            constexpr int kLanes = DP / 8;                      // lanes of a row (16-byte chunks)
-            const int sub = lane % kLanes, dr = lane / kLanes;
-            const bool live = sub * 8 < t.c.dim;
-            while (ok && g.next(a)) {
-                if (g.is_k) {
-                    const uint32_t valid = __ballot_sync(0xffffffffu, g.cur >= 0);
-                    if (lane == 0) {
-                        Info* inf = info + (g.tile - 1) % kInfo;
-                        inf->valid[pw] = valid;
-                        mbar_arrive(&sh->info[(g.tile - 1) % kInfo]);
-                    }
-                }
-                const uint32_t s = n % stages, ph = (n / stages) & 1u;
+        const uint32_t stride = (uint32_t)t.c.slot_stride * (uint32_t)kElem;   // bytes from slot to slot
+        constexpr int kLanes = DP * kElem / 16;                 // lanes of a row (16 bytes each)
+        constexpr int kRowsAtOnce = 32 / kLanes, kSteps = kTile / kRowsAtOnce;
+        const int sub = lane % kLanes, r0 = lane / kLanes;
+        const bool live = sub * (16 / kElem) < t.c.dim;
+        auto described = [&](int ti) {
+            ok = __all_sync(0xffffffffu, wait_or_abort(&sh->info_full[ti % kInfo], (uint32_t)(ti / kInfo) & 1u, abort));
+        };
+        long long head_at = 0;
+        for (;; item += kProducers, i += kProducers) {
+            while (ok && i >= 2 * n) {                          // on to the segment that holds the item
+                i -= 2 * n;
+                base += n;
+                n = 0;
+                if (base >= (int)count) break;
+                described(base);
+                if (!ok) break;
+                const Info* f = info + base % kInfo;
+                n = f->tiles;
+                ahead = min(f->ahead, n);
+                head_at = kElem * (f->head * t.c.head_stride) + sub * 16;
+            }
+            if (!ok || n == 0) break;
+            const int j = i - ahead, pairs = 2 * (n - ahead);
+            const bool is_k = j < 0 || ((j & 1) && j < pairs);
+            const int tl = base + (is_k ? (j < 0 ? i : ahead + (j >> 1)) : (j < pairs ? j >> 1 : j - (pairs >> 1)));
+            described(tl);
+            if (!ok) break;
+            const int* slots = info[tl % kInfo].slot + r0;
+            const uint8_t* src = static_cast<const uint8_t*>(is_k ? t.c.k : t.c.v) + head_at;
+            const uint32_t s = item % stages, ph = (item / stages) & 1u;
+            if constexpr (!kFp8) {
                 ok = __all_sync(0xffffffffu, wait_or_abort(&sh->empty[s], ph ^ 1u, abort));
                 if (!ok) break;
-                const uint8_t* src = static_cast<const uint8_t*>(g.is_k ? t.c.k : t.c.v) +
-                                     2 * (g.w.h * t.c.head_stride + sub * 8);
                 const uint32_t dst = smem_u32(ring + s * L::kStage);
-                const int mine_slot = g.slot();
-#pragma unroll
-                for (int i = 0; i < kTokens; i += 32 / kLanes) {
-                    const int tok = i + dr;
-                    const int slot = __shfl_sync(0xffffffffu, mine_slot, tok);
-                    const bool get = live && slot >= 0;
-                    cp16(dst + chunk_at(pw * kTokens + tok, sub), src + (get ? 2 * (slot * t.c.slot_stride) : 0), get);
+#pragma unroll 8
+                for (int k = 0; k < kSteps; ++k) {
+                    const int slot = live ? slots[k * kRowsAtOnce] : -1;
+                    cp16(dst + chunk_at<kBlock>(k * kRowsAtOnce + r0, sub), src + (uint64_t)(uint32_t)max(slot, 0) * stride,
+                         slot >= 0);
                 }
                 cp_arrive(&sh->full[s]);
-                ++n;
-            }
-            cp_wait_all();
-        } else {
-            constexpr int kLanes = DP / 16;                     // lanes of a row (16 codes each)
-            constexpr int kSteps = kTokens * kLanes / 64;       // 16-byte loads of half an item, per lane
-            constexpr int kAhead = 5;                           // half items whose loads are in flight
-            const int sub = lane % kLanes, dr = lane / kLanes;
-            const bool live = sub * 16 < t.c.dim;
-            uint4 buf[kAhead][kSteps];
-            uint32_t issued = 0, done = 0;                      // half items
-            int item_slot = -1;
-            const uint8_t* src = nullptr;
-            bool more = true;
-            auto issue = [&](uint4 (&x)[kSteps]) {
-                if (!(issued & 1u)) {
-                    more = g.next(a);
-                    if (!more) return;
-                    item_slot = g.slot();
-                    src = static_cast<const uint8_t*>(g.is_k ? t.c.k : t.c.v) + (g.w.h * t.c.head_stride + sub * 16);
-                    if (g.is_k) {
-                        const int at_info = (g.tile - 1) % kInfo;
-                        Info* inf = info + at_info;
-                        const uint32_t valid = __ballot_sync(0xffffffffu, item_slot >= 0);
-                        float ks = 0.f, vs = 0.f;
-                        if (item_slot >= 0) {
-                            const long long at = item_slot * t.c.scale_stride + g.w.h;
-                            ks = __ldg(t.c.k_scale + at);
-                            vs = __ldg(t.c.v_scale + at);
-                        }
-                        float top = fabsf(vs) < __int_as_float(0x7f800000) ? fabsf(vs) : 0.f;
+            } else {
+                // codes in registers, then as fp16 into the stage
+                uint4 x[kSteps];
 #pragma unroll
-                        for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-                        inf->ks[pw * kTokens + lane] = ks * (t.scale * kL2E);
-                        inf->vs[pw * kTokens + lane] = vs;
-                        if (lane == 0) {
-                            inf->valid[pw] = valid;
-                            inf->vmax[pw] = top;
-                        }
-                        __syncwarp();
-                        if (lane == 0) mbar_arrive(&sh->info[at_info]);
-                    }
+                for (int k = 0; k < kSteps; ++k) {
+                    const int slot = live ? slots[k * kRowsAtOnce] : -1;
+                    x[k] = make_uint4(0, 0, 0, 0);
+                    if (slot >= 0) x[k] = ld16_once(src + (uint64_t)(uint32_t)slot * stride);
                 }
-                const int first = (issued & 1u) * (kTokens / 2) + dr;
-#pragma unroll
-                for (int i = 0; i < kSteps; ++i) {
-                    const int slot = __shfl_sync(0xffffffffu, item_slot, first + i * (32 / kLanes));
-                    x[i] = make_uint4(0, 0, 0, 0);
-                    if (live && slot >= 0) x[i] = __ldg(reinterpret_cast<const uint4*>(src + slot * t.c.slot_stride));
-                }
-                ++issued;
-            };
-            auto finish = [&](const uint4 (&x)[kSteps]) {
-                const uint32_t s = n % stages, ph = (n / stages) & 1u;
-                if (!(done & 1u)) {
-                    ok = __all_sync(0xffffffffu, wait_or_abort(&sh->empty[s], ph ^ 1u, abort));
-                    if (!ok) return;
-                }
+                ok = __all_sync(0xffffffffu, wait_or_abort(&sh->empty[s], ph ^ 1u, abort));
+                if (!ok) break;
                 uint8_t* dst = ring + s * L::kStage;
-                const int first = pw * kTokens + (done & 1u) * (kTokens / 2) + dr;
+                // the two 16-byte stores of a lane go to even and odd chunks; the upper half of a
+                // row's lanes swaps them, so that eight lanes of a store hit eight banks of four
+                const bool upper = sub >= 4;
+                const int first = 2 * sub + (upper ? 1 : 0), second = first ^ 1;
 #pragma unroll
-                for (int i = 0; i < kSteps; ++i) {
-                    const int row = first + i * (32 / kLanes);
-                    const uint32_t c8[4] = {x[i].x, x[i].y, x[i].z, x[i].w};
+                for (int k = 0; k < kSteps; ++k) {
+                    const int row = k * kRowsAtOnce + r0;
+                    const uint32_t c4[4] = {x[k].x, x[k].y, x[k].z, x[k].w};
                     uint32_t o[8];
 #pragma unroll
-                    for (int j = 0; j < 8; ++j) {
-                        const __half2_raw h =
-                            __nv_cvt_fp8x2_to_halfraw2((uint16_t)(c8[j >> 1] >> (16 * (j & 1))), __NV_E4M3);
-                        o[j] = (uint32_t)h.x | ((uint32_t)h.y << 16);
+                    for (int q = 0; q < 8; ++q) {
+                        const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2((uint16_t)(c4[q >> 1] >> (16 * (q & 1))), __NV_E4M3);
+                        o[q] = (uint32_t)h.x | ((uint32_t)h.y << 16);
                     }
-                    *reinterpret_cast<uint4*>(dst + chunk_at(row, 2 * sub)) = make_uint4(o[0], o[1], o[2], o[3]);
-                    *reinterpret_cast<uint4*>(dst + chunk_at(row, 2 * sub + 1)) = make_uint4(o[4], o[5], o[6], o[7]);
+                    const uint4 lo = make_uint4(o[0], o[1], o[2], o[3]), hi = make_uint4(o[4], o[5], o[6], o[7]);
+                    *reinterpret_cast<uint4*>(dst + chunk_at<kBlock>(row, first)) = upper ? hi : lo;
+                    *reinterpret_cast<uint4*>(dst + chunk_at<kBlock>(row, second)) = upper ? lo : hi;
                 }
-                if (done & 1u) {
-                    __syncwarp();
-                    if (lane == 0) mbar_arrive(&sh->full[s]);
-                    ++n;
-                }
-                ++done;
-            };
-#pragma unroll
-            for (int i = 0; i < kAhead; ++i)
-                if (more) issue(buf[i]);
-            while (ok && done < issued) {
-#pragma unroll
-                for (int i = 0; i < kAhead; ++i) {
-                    if (ok && done < issued) {
-                        finish(buf[i]);
-                        if (ok && more) issue(buf[i]);
-                    }
-                }
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&sh->full[s]);
             }
         }
-    } else if (warp >= 8) {
+        if constexpr (!kFp8) cp_wait_all();
+    } else if (warp == kIndexWarp) {
+        // ---------------- index: slots, scales and masks of the tiles to come ----------------
+        int ti = 0;
+        bool ok = true;
+        const int pages = (int)(t.c.slots / t.page_size);
+        do {
+            const int nt = w.count(), ahead = w.shared_rows(qt) ? kAheadUnits : kAheadUnits / 2;
+            for (int t0 = 0; ok && t0 < nt; t0 += kBatch) {
+                int slot[kBatch][2];
+                float ks[kBatch][2], vs[kBatch][2];
+#pragma unroll
+                for (int k = 0; k < kBatch; ++k) {
+#pragma unroll
+                    for (int e = 0; e < 2; ++e) {
+                        const int pos = (w.k0 + t0 + k) * kTile + e * 32 + lane;
+                        slot[k][e] = -1;
+                        if (t0 + k < nt && pos < w.r.len) {
+                            const int page = pos / t.page_size;
+                            const int entry = __ldg(t.table + (long long)w.b * t.table_stride + page);
+                            if (entry >= 0 && entry < pages)
+                                slot[k][e] = entry * t.page_size + (pos - page * t.page_size);
+                            else if (t.err)
+                                atomicOr(t.err, 2u);
+                        }
+                    }
+                }
+                if constexpr (kFp8) {
+#pragma unroll
+                    for (int k = 0; k < kBatch; ++k) {
+#pragma unroll
+                        for (int e = 0; e < 2; ++e) {
+                            ks[k][e] = vs[k][e] = 0.f;
+                            if (slot[k][e] >= 0) {
+                                const long long at = slot[k][e] * t.c.scale_stride + w.h;
+                                ks[k][e] = __ldg(t.c.k_scale + at) * (t.scale * kL2E);
+                                vs[k][e] = __ldg(t.c.v_scale + at);
+                            }
+                        }
+                    }
+                }
+#pragma unroll
+                for (int k = 0; k < kBatch; ++k) {
+                    if (t0 + k >= nt) break;
+                    const int at = ti % kInfo;
+                    ok = __all_sync(0xffffffffu,
+                                    wait_or_abort(&sh->info_empty[at], ((uint32_t)(ti / kInfo) & 1u) ^ 1u, abort));
+                    if (!ok) break;
+                    Info* f = info + at;
+                    f->slot[lane] = slot[k][0];
+                    f->slot[lane + 32] = slot[k][1];
+                    const uint32_t v0 = __ballot_sync(0xffffffffu, slot[k][0] >= 0);
+                    const uint32_t v1 = __ballot_sync(0xffffffffu, slot[k][1] >= 0);
+                    float top = 0.f;
+                    if constexpr (kFp8) {
+                        f->ks[lane] = ks[k][0];
+                        f->ks[lane + 32] = ks[k][1];
+                        f->vs[lane] = vs[k][0];
+                        f->vs[lane + 32] = vs[k][1];
+                        uint32_t bits = 0;                      // of finite sizes: ordered as they are
+#pragma unroll
+                        for (int e = 0; e < 2; ++e) {
+                            const uint32_t x = __float_as_uint(fabsf(vs[k][e]));
+                            if (x < 0x7f800000u) bits = max(bits, x);
+                        }
+                        top = __uint_as_float(__reduce_max_sync(0xffffffffu, bits));
+                    }
+                    if (lane == 0) {
+                        f->valid[0] = v0;
+                        f->valid[1] = v1;
+                        f->head = w.h;
+                        f->tiles = nt;
+                        f->ahead = ahead;
+                        f->vmax = top;
+                    }
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(&sh->info_full[at]);
+                    ++ti;
+                }
+            }
+        } while (ok && w.advance(a));
+    } else if (warp == kMmaWarp) {
         // ---------------- MMA issuer ----------------
-        regs_down<kFp8 ? 40 : 56>();
-        if (warp == 8 && lane == 0) {
+        {
             constexpr uint32_t kFormat = std::is_same<TO, __nv_bfloat16>::value ? 1u : 0u;
             constexpr uint32_t kCommon = (1u << 4) | (kFormat << 7) | (kFormat << 10) | ((uint32_t)(kRows >> 4) << 24);
             constexpr uint32_t kIdescS = kCommon | ((uint32_t)(kTile >> 3) << 17);
@@ -695,59 +720,75 @@ __global__ void __launch_bounds__(kThreads, 1) attn_kernel(const __grid_constant
             const int ksteps = t.c.dim / 16;
             const uint32_t q0 = desc_low(smem_u32(sq), 16), k0 = desc_low(smem_u32(ring), 16),
                            v0 = desc_low(smem_u32(ring), kBlock);
-            uint32_t item = 0, seg = 0, su[2] = {0, 0};  // items before the segment, segments, units per stream
+            uint32_t tile0 = 0, seg = 0, ph = 0;             // ph: parity of each (stream, buffer)
+            uint32_t st = 0, sp = 0;                         // next stage of the ring and its parity
             bool ok = true;
-            do {
-                const bool both = !w.shared_rows(qt);    // both streams use every tile
-                const int nt = w.count(), units = both ? 2 * nt : nt;
-                ok = wait_or_abort(&sh->q_full, seg & 1u, abort);
+            auto wait_all = [&](uint64_t* bar, uint32_t parity) {
+                ok = __all_sync(0xffffffffu, wait_or_abort(bar, parity, abort));
+            };
+            // the next stage, filled: tiles are used in the order in which they are loaded
+            auto take_stage = [&]() {
+                const uint32_t mine = st;
+                wait_all(&sh->full[mine], sp);
+                fence_proxy_async_smem();
+                if (++st == (uint32_t)stages) {
+                    st = 0;
+                    sp ^= 1u;
+                }
+                return mine;
+            };
+            auto scores = [&](uint32_t sb, uint32_t stage, uint32_t q_off) {   // sb: 2 x stream + buffer
+                const uint32_t qa = q0 + q_off, kb = k0 + stage * (L::kStage >> 4), d = tmem + sb * kTile;
+#pragma unroll
+                for (int k = 0; k < DP / 16; ++k) {
+                    const uint32_t col = (k & 3) * 2;
+                    if (k < ksteps)
+                        mma_ss(d, desc(qa + (k >> 2) * (kQBlock >> 4) + col), desc(kb + (k >> 2) * (kBlock >> 4) + col), kIdescS,
+                               k != 0);
+                }
+                mma_commit(&sh->s_full[0][0] + sb);
+            };
+            auto weights = [&](uint32_t sb, uint32_t stage, uint32_t more) {   // O += P V
+                wait_all(&sh->p_full[0][0] + sb, (ph >> sb) & 1u);
+                if (!ok) return;
+                ph ^= 1u << sb;
                 fence_proxy_async_smem();
                 tc_fence_after();
-                auto scores = [&](int u) {
-                    const int s = u & 1, tl = both ? u >> 1 : u;
-                    const uint32_t it = item_of_k(item, tl), st = it % stages;
-                    if (!both || s == 0) {
-                        ok = wait_or_abort(&sh->full[st], (it / stages) & 1u, abort);
-                        if (!ok) return;
-                        fence_proxy_async_smem();
-                        tc_fence_after();
-                    }
-                    const uint32_t qa = q0 + (both && s ? L::kStage >> 4 : 0), kb = k0 + st * (L::kStage >> 4);
-                    const uint32_t d = tmem + s * kTile;
+                const uint32_t vb = v0 + stage * (L::kStage >> 4), d = tmem + 256 + (sb >> 1) * 128, p = tmem + sb * kTile;
 #pragma unroll
-                    for (int k = 0; k < DP / 16; ++k) {
-                        const uint32_t off = (k >> 2) * (kBlock >> 4) + (k & 3) * 2;
-                        if (k < ksteps) mma_ss(d, desc(qa + off), desc(kb + off), kIdescS, k != 0);
-                    }
-                    if (!both || s == 1) mma_commit(&sh->empty[st]);
-                    mma_commit(&sh->s_full[s]);
-                };
-                for (int u = 0; ok && u < 2 && u < units; ++u) scores(u);
-                for (int u = 0; ok && u < units; ++u) {
-                    const int s = u & 1, tl = both ? u >> 1 : u;
-                    const uint32_t it = item_of_v(item, tl, nt), st = it % stages;
-                    if (!both || s == 0) {
-                        ok = wait_or_abort(&sh->full[st], (it / stages) & 1u, abort);
+                for (int k = 0; k < kTile / 16; ++k) mma_ts(d, p + k * 8, desc(vb + k * (2048 >> 4)), idesc_o, k ? 1u : more);
+                mma_commit(&sh->pv_done[sb >> 1]);
+            };
+            do {
+                const bool both = !w.shared_rows(qt);        // both streams use every tile
+                const int nt = w.count();
+                wait_all(&sh->q_full, seg & 1u);
+                fence_proxy_async_smem();
+                tc_fence_after();
+                // unit u: stream u & 1, buffer (u >> 1) & 1; its tile u, or u >> 1 where both streams use it
+                const int units = both ? 2 * nt : nt;
+                uint32_t ks = 0, vs = 0;
+                for (int u = -kAheadUnits; ok && u < units; ++u) {
+                    const uint32_t s = u & 1, sb = (s << 1) | ((u >> 1) & 1);
+                    const bool fresh = !both || s == 0, last = !both || s == 1;   // first, last use of a tile
+                    if (u >= 0) {
+                        if (fresh) vs = take_stage();
+                        if (ok) weights(sb, vs, u > 1);
                         if (!ok) break;
-                        fence_proxy_async_smem();
+                        if (last) {
+                            mma_commit(&sh->empty[vs]);
+                            mma_commit(&sh->info_empty[(tile0 + (both ? u >> 1 : u)) % kInfo]);
+                        }
                     }
-                    const uint32_t vb = v0 + st * (L::kStage >> 4), d = tmem + 256 + s * 128, p = tmem + s * kTile;
-#pragma unroll
-                    for (int half = 0; half < 2; ++half) {
-                        ok = ok && wait_or_abort(&sh->p_full[s][half], su[s] & 1u, abort);
+                    if (u + kAheadUnits < units) {
+                        if (fresh) ks = take_stage();
                         if (!ok) break;
-                        tc_fence_after();
-#pragma unroll
-                        for (int k = 4 * half; k < 4 * half + 4; ++k)
-                            mma_ts(d, p + k * 8, desc(vb + k * (2048 >> 4)), idesc_o, u >= 2 || k != 0);
+                        scores(sb, ks, both && s ? L::kQTile >> 4 : 0);
+                        if (last) mma_commit(&sh->empty[ks]);
                     }
-                    if (!ok) break;
-                    ++su[s];
-                    if (!both || s == 1) mma_commit(&sh->empty[st]);
-                    if (u + 2 < units) scores(u + 2);
                 }
                 if (ok) mma_commit(&sh->o_full);
-                item += 2 * nt;
+                tile0 += nt;
                 ++seg;
             } while (ok && w.advance(a));
             // every instruction issued here is done before TMEM is released
@@ -757,16 +798,16 @@ __global__ void __launch_bounds__(kThreads, 1) attn_kernel(const __grid_constant
         __syncwarp();
     } else {
         // ---------------- softmax and epilogue: one row per thread ----------------
-        regs_up<kFp8 ? 168 : 200>();
         const int s = warp >> 2, quarter = warp & 3, row = quarter * 32 + lane;
         const uint32_t lanes = (uint32_t)(quarter * 32) << 16;
-        const uint32_t ts = tmem + lanes + s * kTile, to = tmem + lanes + 256 + s * 128;
+        const uint32_t to = tmem + lanes + 256 + s * 128;
         constexpr int kLanes = DP / 8;                          // 16-byte chunks of a row
         constexpr int kStep = kSoftmaxThreads / kLanes;         // rows that the 256 threads move at once
         const int sub = tid % kLanes, r_first = tid / kLanes;
         const bool sub_live = sub * 8 < t.c.dim;
         const uint32_t group_inv = (0xFFFFFFFFu / (uint32_t)t.group) + 1u;  // ceil(2^32 / group), 0 for 1
-        uint32_t seg = 0, su = 0, tile0 = 0, item = 0, jp = 0;  // jp: phases of `joined`
+        uint32_t seg = 0, tile0 = 0, item = 0, jp = 0;          // jp: phases of `joined`
+        uint32_t ph = 0, su = 0;                                // parity of each buffer; units of the stream
         bool ok = true;
         auto join = [&]() {                                     // both warpgroups have come here
             __syncwarp();
@@ -829,7 +870,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_kernel(const __grid_constant
                                               pack2(f[4] * up, f[5] * up, __half()), pack2(f[6] * up, f[7] * up, __half()));
                         }
                         if (r < filled)
-                            *reinterpret_cast<uint4*>(sq + (r >> 7) * L::kStage + chunk_at(r & 127, sub)) = x[i];
+                            *reinterpret_cast<uint4*>(sq + (r >> 7) * L::kQTile + chunk_at<kQBlock>(r & 127, sub)) = x[i];
                     }
                 }
                 tc_fence_before();
@@ -847,29 +888,32 @@ __global__ void __launch_bounds__(kThreads, 1) attn_kernel(const __grid_constant
                 if (t.mask) bits = (uint64_t)__ldg(reinterpret_cast<const long long*>(t.mask) + w.r.lo + token);
             }
             float ref = -INFINITY, sum = 0.f, vmax = 0.f;
-            const int step = both ? 1 : 2;
-            for (int tl = both ? 0 : s; ok && tl < nt; tl += step, ++su) {
-                const uint32_t ti = tile0 + tl;
+            const int step = both ? 1 : 2, ahead = min(nt, both ? kAheadUnits / 2 : kAheadUnits);
+            int b = 0;
+            for (int tl = both ? 0 : s; ok && tl < nt; tl += step, ++su, b ^= 1) {
+                const uint32_t ti = tile0 + tl, ts = tmem + lanes + s * 128 + b * kTile;
                 const Info* inf = info + ti % kInfo;
-                ok = wait_or_abort(&sh->info[ti % kInfo], (ti / kInfo) & 1u, abort) &&
-                     wait_or_abort(&sh->s_full[s], su & 1u, abort);
+                ok = wait_or_abort(&sh->info_full[ti % kInfo], (ti / kInfo) & 1u, abort) &&
+                     wait_or_abort(&sh->s_full[s][b], (ph >> b) & 1u, abort);
                 ok = __all_sync(0xffffffffu, ok);
                 if (!ok) break;
+                ph ^= 1u << b;
                 tc_fence_after();
                 const int kb = (w.k0 + tl) * kTile;             // first position of the tile
                 const bool drafted = kb + kTile > w.r.p0;
                 if (drafted) {
                     // V elements of drafted tokens that are not finite: zeroed for the matrix
                     // instructions, added to the rows that see them at the end
-                    const uint32_t it = item_of_v(item, tl, nt), st = it % stages;
+                    const uint32_t it = item + item_of_v(tl, nt, ahead), st = it % stages;
                     ok = __all_sync(0xffffffffu, wait_or_abort(&sh->full[st], (it / stages) & 1u, abort));
                     if (!ok) break;
-                    if (kb + row >= w.r.p0 && kb + row < w.r.len) {
+                    const int key = row & (kTile - 1);          // two threads a key
+                    if (kb + key >= w.r.p0 && kb + key < w.r.len) {
                         uint8_t* v = ring + st * L::kStage;
                         constexpr uint32_t kExp = std::is_same<TO, __nv_bfloat16>::value ? 0x7F80u : 0x7C00u;
                         bool found = false;
-                        for (int c = 0; c < t.c.dim / 8; ++c) {
-                            uint4* at = reinterpret_cast<uint4*>(v + chunk_at(row, c));
+                        for (int c = row / kTile; c < t.c.dim / 8; c += 2) {
+                            uint4* at = reinterpret_cast<uint4*>(v + chunk_at<kBlock>(key, c));
                             const uint4 x = *at;
                             uint32_t xw[4] = {x.x, x.y, x.z, x.w};
                             bool here = false;
@@ -889,20 +933,18 @@ __global__ void __launch_bounds__(kThreads, 1) attn_kernel(const __grid_constant
                         }
                         if (found) *(volatile int*)&sh->odd[seg & 1] = 1;
                     }
-                    fence_proxy_async_smem();
                 }
                 if (any_row) {
-                    // this row's 128 scores stay in registers: one read of TMEM
-                    uint32_t v[4][32];
-#pragma unroll
-                    for (int c = 0; c < 4; ++c) tmem_ld32(ts + c * 32, v[c]);
-                    const uint4 valid = *reinterpret_cast<const uint4*>(inf->valid);
-                    const bool masked = drafted || (valid.x & valid.y & valid.z & valid.w) != ~0u;
-                    uint32_t vis[4] = {~0u, ~0u, ~0u, ~0u};
+                    // this row's 64 scores stay in registers: one read of TMEM
+                    uint32_t v[2][32];
+                    tmem_ld32(ts, v[0]);
+                    tmem_ld32(ts + 32, v[1]);
+                    const uint2 valid = *reinterpret_cast<const uint2*>(inf->valid);
+                    const bool masked = drafted || (valid.x & valid.y) != ~0u;
+                    uint32_t vis[2] = {~0u, ~0u};
                     if (masked) {
-                        const uint32_t vw[4] = {valid.x, valid.y, valid.z, valid.w};
 #pragma unroll
-                        for (int i = 0; i < 4; ++i) {
+                        for (int i = 0; i < 2; ++i) {
                             const int pos = kb + 32 * i;
                             const int n = (t.mask ? w.r.p0 : w.r.p0 + token + 1) - pos;
                             uint32_t m = n >= 32 ? ~0u : (n <= 0 ? 0u : (1u << n) - 1u);
@@ -913,12 +955,12 @@ __global__ void __launch_bounds__(kThreads, 1) attn_kernel(const __grid_constant
                                 else if (d > -32)
                                     m |= (uint32_t)(bits << -d);
                             }
-                            vis[i] = m & vw[i];
+                            vis[i] = m & (i ? valid.y : valid.x);
                         }
                     }
-                    float mx[4];
+                    float mx[2];
 #pragma unroll
-                    for (int c = 0; c < 4; ++c) {
+                    for (int c = 0; c < 2; ++c) {
                         tmem_wait_ld(v[c]);
                         if constexpr (kFp8) {
 #pragma unroll
@@ -947,10 +989,9 @@ __global__ void __launch_bounds__(kThreads, 1) attn_kernel(const __grid_constant
                         }
                         mx[c] = fmaxf(a0, a1);
                     }
-                    float target = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * cm;
+                    float target = fmaxf(mx[0], mx[1]) * cm;
                     if constexpr (kFp8) {
-                        const float4 vm = *reinterpret_cast<const float4*>(inf->vmax);
-                        vmax = fmaxf(vmax, fmaxf(fmaxf(vm.x, vm.y), fmaxf(vm.z, vm.w)));
+                        vmax = fmaxf(vmax, inf->vmax);
                         // 2^ev is the first power of two above the V scales so far
                         const int ev = max(-90, min(120, (int)(__float_as_uint(vmax) >> 23) - 126));
                         target += (float)(ev - 6);
@@ -960,6 +1001,9 @@ __global__ void __launch_bounds__(kThreads, 1) attn_kernel(const __grid_constant
                     if (__any_sync(0xffffffffu, target > ref + kSlack)) {
                         const float to_ref = fmaxf(ref, target);
                         if (tl >= step) {                       // the accumulator holds something
+                            ok = __all_sync(0xffffffffu, wait_or_abort(&sh->pv_done[s], (su - 1) & 1u, abort));
+                            if (!ok) break;
+                            tc_fence_after();
                             const float f = ref == -INFINITY ? 1.0f : ex2(ref - to_ref);
                             sum *= f;
 #pragma unroll 1
@@ -978,7 +1022,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_kernel(const __grid_constant
                     const float2 cm2 = make_float2(cm, cm), nref2 = make_float2(nref, nref);
                     float2 part0 = make_float2(0.f, 0.f), part1 = part0;
 #pragma unroll
-                    for (int c = 0; c < 4; ++c) {
+                    for (int c = 0; c < 2; ++c) {
                         uint32_t p[16];
 #pragma unroll
                         for (int j = 0; j < 32; j += 4) {
@@ -1003,19 +1047,13 @@ __global__ void __launch_bounds__(kThreads, 1) attn_kernel(const __grid_constant
                             p[j / 2 + 1] = pack2(hi.x, hi.y, TO());
                         }
                         tmem_st16(ts + c * 16, p);              // over scores that have been read
-                        if (c & 1) {
-                            tmem_wait_st();
-                            tc_fence_before();
-                            __syncwarp();
-                            if (lane == 0) mbar_arrive(&sh->p_full[s][c >> 1]);
-                        }
                     }
                     sum += (part0.x + part0.y) + (part1.x + part1.y);
-                } else {
-                    tc_fence_before();
-                    __syncwarp();
-                    if (lane < 2) mbar_arrive(&sh->p_full[s][lane]);
+                    tmem_wait_st();
                 }
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&sh->p_full[s][b]);
             }
             // ---- the segment's result
             if (tid == 0) sh->odd[(seg + 1) & 1] = 0;
@@ -1047,7 +1085,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_kernel(const __grid_constant
                 const long long slot = 2 * blockIdx.x + (w.k0 == 0 ? 1 : 0);
                 const int per = kRows * qt;
                 float4* po = a.part_o + slot * (DP / 4) * per + my;
-                uint8_t* so = sq + (my >> 7) * L::kStage;
+                uint8_t* so = sq + (my >> 7) * L::kQTile;
                 const float inv = sum == 0.f ? 0.f : 1.0f / sum;
                 const int c0 = both ? 0 : s * (DP / 2), c1 = both ? DP : c0 + DP / 2;
 #pragma unroll 1
@@ -1097,7 +1135,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_kernel(const __grid_constant
 #pragma unroll
                             for (int i = 0; i < 4; ++i)
                                 p[i] = pack2(__uint_as_float(v[j + 2 * i]) * inv, __uint_as_float(v[j + 2 * i + 1]) * inv, TQ());
-                            *reinterpret_cast<uint4*>(so + chunk_at(row, (c + j) / 8)) = make_uint4(p[0], p[1], p[2], p[3]);
+                            *reinterpret_cast<uint4*>(so + chunk_at<kQBlock>(row, (c + j) / 8)) = make_uint4(p[0], p[1], p[2], p[3]);
                         }
                     } else if (my < nrows) {
 #pragma unroll
@@ -1124,7 +1162,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_kernel(const __grid_constant
 #pragma unroll 4
                     for (int r = r_first; r < nrows; r += kStep)
                         *reinterpret_cast<uint4*>(out + q_offset(r, t.out_token_stride, t.out_head_stride)) =
-                            *reinterpret_cast<const uint4*>(sq + (r >> 7) * L::kStage + chunk_at(r & 127, sub));
+                            *reinterpret_cast<const uint4*>(sq + (r >> 7) * L::kQTile + chunk_at<kQBlock>(r & 127, sub));
                 }
             }
             tc_fence_before();
@@ -1136,9 +1174,9 @@ __global__ void __launch_bounds__(kThreads, 1) attn_kernel(const __grid_constant
 
     __syncthreads();
     if (tid == 0 && *abort && t.err) atomicOr(t.err, 4u);
-    if (warp == 8) {
+    if (warp == kMmaWarp) {
         tc_fence_after();
-        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem) : "memory");
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(sh->tmem) : "memory");
     }
 }
 
@@ -1205,7 +1243,7 @@ int launch(const KernelArgs& a, int sms, cudaStream_t st) {
     if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess)
         return kLaunchFailed;
     const int grid = sms < kMaxCtas ? sms : kMaxCtas;
-    kern<<<grid, kThreads, smem, st>>>(a);
+    kern<<<grid, threads<kFp8>(), smem, st>>>(a);
     if (cudaGetLastError() != cudaSuccess) return kLaunchFailed;
     // items of one tile are never cut
     if ((long long)a.t.max_pages * a.t.page_size <= kTile) return kOk;
