@@ -17,9 +17,9 @@
 //                   every SM streams the same number of tiles however ragged the lengths are.
 //                     warps 0-7    two softmax warpgroups, one TMEM lane (row) per thread, its
 //                                  scores of a tile in registers
-//                     warp 8       TMEM allocation and the MMA issuer
-//                     warp 9       index: slots, scales and validity of the tiles to come
-//                     warps 10..   producers: K and V rows of a tile, slot by slot, into a ring of
+//                     warps 8, 9   MMA issuers: scores (and TMEM allocation), accumulation
+//                     warp 10      index: slots, scales and validity of the tiles to come
+//                     warps 11..   producers: K and V rows of a tile, slot by slot, into a ring of
 //                                  128-byte-swizzled shared-memory stages
 //                   S = Q K^T (kind::f16, both operands in shared memory) and O += P V (P from
 //                   TMEM, written over S; V as a matrix with rows of keys, "MN-major").
@@ -50,6 +50,7 @@
 #include <cuda_fp16.h>
 #include <cuda_fp8.h>
 #include <cuda_runtime.h>
+#include <stddef.h>
 #include <stdint.h>
 
 #include <type_traits>
@@ -66,7 +67,6 @@ constexpr int kQBlock = kRows * 128;       // bytes of a [128 rows][128 bytes] s
 constexpr int kBlock = kTile * 128;        // the same of a K or V tile
 constexpr int kMaxCtas = 148;              // SMs of a B200; partial results are laid out for these
 constexpr int kInfo = 16;                  // tiles that are described in shared memory at once
-constexpr int kBatch = 4;                  // tiles that the index warp looks up at once
 constexpr int kAheadUnits = 4;             // score tiles in TMEM: two streams x two buffers
 constexpr int kSoftmaxThreads = 256;
 constexpr int kMinTiles = 4;               // tiles per CTA below which fewer CTAs take part
@@ -74,9 +74,9 @@ constexpr float kSlack = 8.0f;             // log2 by which a maximum may outgro
 constexpr float kL2E = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
 
-// warps 0-7 softmax, 8 MMA issuer, 9 index, 10.. producers
-constexpr int kMmaWarp = 8, kIndexWarp = 9, kFirstProducer = 10;
-template <bool kFp8> constexpr int producers() { return kFp8 ? 6 : 4; }
+// warps 0-7 softmax, 8 and 9 MMA issuers (scores, accumulation), 10 index, 11.. producers
+constexpr int kScoreWarp = 8, kAccumWarp = 9, kIndexWarp = 10, kFirstProducer = 11;
+template <bool kFp8> constexpr int producers() { return kFp8 ? 5 : 4; }
 template <bool kFp8> constexpr int threads() { return 32 * (kFirstProducer + producers<kFp8>()); }
 
 // a tile of keys, as the index warp describes it to the others
@@ -84,11 +84,11 @@ struct alignas(16) TileInfoPlain {
     int slot[kTile];          // of each position; -1 where there is none or it cannot be read
     uint32_t valid[2];        // the positions with a slot
     int head, tiles, ahead;   // of the segment: KV head, tiles, K tiles loaded before its first V tile
-    float vmax;               // e4m3: largest finite V scale
+    int pad;
 };
 struct TileInfoScaled : TileInfoPlain {
-    alignas(16) float ks[kTile];   // K scale x scale x log2(e)
-    alignas(16) float vs[kTile];   // V scale
+    alignas(16) float ks[kTile];   // scales of K and V, 0 where there is no slot
+    alignas(16) float vs[kTile];
 };
 template <bool kFp8> struct InfoOf { using type = TileInfoPlain; };
 template <> struct InfoOf<true> { using type = TileInfoScaled; };
@@ -103,8 +103,21 @@ struct Split {          // written by CTA c for the item that reaches into it fr
     int pad[2];
 };
 
+// division by a number fixed for the launch: q = (m + ((n - m) >> s1)) >> s2 with m = mul * n >> 32,
+// exact for every 32-bit n (Granlund and Montgomery's round-up method)
+struct Divisor {
+    uint32_t mul;
+    int s1, s2;
+    __device__ __forceinline__ uint32_t divide(uint32_t n) const {
+        const uint32_t m = __umulhi(mul, n);
+        return (m + ((n - m) >> s1)) >> s2;
+    }
+};
+
 struct KernelArgs {
     TreeAttnArgs t;
+    Divisor page;           // by page_size
+    int pages;              // of the cache
     int qt;                 // Q tiles of a row block
     Split* splits;          // [kMaxCtas]
     float2* part_ml;        // [2 * kMaxCtas][128 qt] (reference, sum)
@@ -237,10 +250,10 @@ struct alignas(16) Shared {
     uint64_t q_full;                 // Q of the segment in shared memory, last segment's TMEM read
     uint64_t s_full[2][2];           // scores of a stream's buffer in TMEM
     uint64_t p_full[2][2];           // weights of a stream's buffer in TMEM
-    uint64_t pv_done[2];             // a stream's last weights have been accumulated
+    uint64_t s_free[2][2];           // the weights in a stream's buffer have been accumulated
     uint64_t o_full;                 // the segment's accumulators are complete
     uint64_t joined;                 // both warpgroups have written what the other reads
-    uint64_t drain;
+    uint64_t drain[2];
     uint32_t tmem;
     int abort;
     int odd[2];                      // a drafted V element was not finite (by segment parity)
@@ -298,10 +311,10 @@ __device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint3
         "r"(accumulate)
         : "memory");
 }
-__device__ __forceinline__ void mma_commit(uint64_t* bar) {
+__device__ __forceinline__ void mma_commit(uint32_t bar) {
     asm volatile(
         "{\n\t.reg .pred one;\n\telect.sync _|one, 0xffffffff;\n\t"
-        "@one tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}" ::"r"(smem_u32(bar))
+        "@one tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}" ::"r"(bar)
         : "memory");
 }
 __device__ __forceinline__ void mbar_arrive(uint64_t* bar) {
@@ -376,6 +389,9 @@ __device__ __forceinline__ void cp16(uint32_t dst, const void* src, bool ok) {
     asm volatile("cp.async.cg.shared.global.L2::128B [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(ok ? 16 : 0)
                  : "memory");
 }
+__device__ __forceinline__ void cp4(uint32_t dst, const void* src, bool ok) {
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src), "r"(ok ? 4 : 0) : "memory");
+}
 // 16 bytes that are read once: past L1, where they would push out what the warps spill there
 __device__ __forceinline__ uint4 ld16_once(const void* p) {
     uint4 v;
@@ -405,6 +421,33 @@ __device__ __noinline__ bool wait_slow(uint64_t* bar, uint32_t parity, volatile 
 }
 __device__ __forceinline__ bool wait_or_abort(uint64_t* bar, uint32_t parity, volatile int* abort) {
     return mbar_try_wait(bar, parity) || wait_slow(bar, parity, abort);
+}
+
+// the same by shared-memory address, for the issuing warps: all lanes wait, one vote
+__device__ __forceinline__ bool try_wait_at(uint32_t bar, uint32_t parity) {
+    uint32_t ok;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(ok)
+        : "r"(bar), "r"(parity)
+        : "memory");
+    return ok != 0;
+}
+__device__ __noinline__ bool wait_slow_at(uint32_t bar, uint32_t parity, volatile int* abort) {
+    const uint64_t t0 = globaltimer_ns();
+    for (uint32_t i = 1;; ++i) {
+        if (try_wait_at(bar, parity)) return true;
+        if (i % 32 != 0) continue;
+        if (*abort) return false;
+        if (globaltimer_ns() - t0 > 2000000000ull) {
+            *abort = 1;
+            return false;
+        }
+    }
+}
+__device__ __forceinline__ bool wait_at(uint32_t bar, uint32_t parity, volatile int* abort) {
+    if (__all_sync(0xffffffffu, try_wait_at(bar, parity))) return true;
+    return __all_sync(0xffffffffu, wait_slow_at(bar, parity, abort));
 }
 
 // 16-byte chunk c of row `row` in a tile of 128-byte-swizzled blocks of `block` bytes
@@ -484,6 +527,8 @@ __global__ void __launch_bounds__(threads<kFp8>(), 1) attn_kernel(const __grid_c
         if (t.err && blockIdx.x == 0 && b0 + tid < t.batch && __ldg(t.lens + b0 + tid) > t.max_pages * t.page_size)
             atomicOr(t.err, 2u);
     }
+    // the same in every lane; said so, that what follows counts as uniform control flow
+    total = __shfl_sync(0xffffffffu, total, 0);
     const long long want = total / kMinTiles;
     const int ctas = (int)(want < 1 ? 1 : (want < (long long)gridDim.x ? want : (long long)gridDim.x));
     if (total == 0 || (int)blockIdx.x >= ctas) return;
@@ -517,7 +562,7 @@ __global__ void __launch_bounds__(threads<kFp8>(), 1) attn_kernel(const __grid_c
             mbar_init(&sh->empty[s], 1);
         }
         for (int i = 0; i < kInfo; ++i) {
-            mbar_init(&sh->info_full[i], 1);
+            mbar_init(&sh->info_full[i], kFp8 ? 33 : 1);
             mbar_init(&sh->info_empty[i], 1);
         }
         mbar_init(&sh->q_full, 8);
@@ -525,17 +570,17 @@ __global__ void __launch_bounds__(threads<kFp8>(), 1) attn_kernel(const __grid_c
             for (int j = 0; j < 2; ++j) {
                 mbar_init(&sh->s_full[i][j], 1);
                 mbar_init(&sh->p_full[i][j], 4);
+                mbar_init(&sh->s_free[i][j], 1);
             }
-            mbar_init(&sh->pv_done[i], 1);
+            mbar_init(&sh->drain[i], 1);
         }
         mbar_init(&sh->o_full, 1);
         mbar_init(&sh->joined, 8);
-        mbar_init(&sh->drain, 1);
         sh->abort = 0;
         sh->odd[0] = sh->odd[1] = 0;
         fence_mbar_init();
     }
-    if (warp == kMmaWarp) {
+    if (warp == kScoreWarp) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_u32(&sh->tmem))
                      : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
@@ -556,7 +601,11 @@ __global__ void __launch_bounds__(threads<kFp8>(), 1) attn_kernel(const __grid_c
         const uint32_t stride = (uint32_t)t.c.slot_stride * (uint32_t)kElem;   // bytes from slot to slot
         constexpr int kLanes = DP * kElem / 16;                 // lanes of a row (16 bytes each)
         constexpr int kRowsAtOnce = 32 / kLanes, kSteps = kTile / kRowsAtOnce;
-        const int sub = lane % kLanes, r0 = lane / kLanes;
+        // lane's place in a row and among the rows of a step.  Where a row of codes becomes two blocks
+        // of fp16, four lanes of one row stand beside four of the next: their stores of eight then
+        // hit eight different groups of banks
+        const int sub = kFp8 && DP == 128 ? (lane & 3) | ((lane >> 1) & 4) : lane % kLanes;
+        const int r0 = kFp8 && DP == 128 ? ((lane >> 2) & 1) | ((lane >> 3) & 2) : lane / kLanes;
         const bool live = sub * (16 / kElem) < t.c.dim;
         auto described = [&](int ti) {
             ok = __all_sync(0xffffffffu, wait_or_abort(&sh->info_full[ti % kInfo], (uint32_t)(ti / kInfo) & 1u, abort));
@@ -607,10 +656,6 @@ __global__ void __launch_bounds__(threads<kFp8>(), 1) attn_kernel(const __grid_c
                 ok = __all_sync(0xffffffffu, wait_or_abort(&sh->empty[s], ph ^ 1u, abort));
                 if (!ok) break;
                 uint8_t* dst = ring + s * L::kStage;
-                // the two 16-byte stores of a lane go to even and odd chunks; the upper half of a
-                // row's lanes swaps them, so that eight lanes of a store hit eight banks of four
-                const bool upper = sub >= 4;
-                const int first = 2 * sub + (upper ? 1 : 0), second = first ^ 1;
 #pragma unroll
                 for (int k = 0; k < kSteps; ++k) {
                     const int row = k * kRowsAtOnce + r0;
@@ -621,9 +666,8 @@ __global__ void __launch_bounds__(threads<kFp8>(), 1) attn_kernel(const __grid_c
                         const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2((uint16_t)(c4[q >> 1] >> (16 * (q & 1))), __NV_E4M3);
                         o[q] = (uint32_t)h.x | ((uint32_t)h.y << 16);
                     }
-                    const uint4 lo = make_uint4(o[0], o[1], o[2], o[3]), hi = make_uint4(o[4], o[5], o[6], o[7]);
-                    *reinterpret_cast<uint4*>(dst + chunk_at<kBlock>(row, first)) = upper ? hi : lo;
-                    *reinterpret_cast<uint4*>(dst + chunk_at<kBlock>(row, second)) = upper ? lo : hi;
+                    *reinterpret_cast<uint4*>(dst + chunk_at<kBlock>(row, 2 * sub)) = make_uint4(o[0], o[1], o[2], o[3]);
+                    *reinterpret_cast<uint4*>(dst + chunk_at<kBlock>(row, 2 * sub + 1)) = make_uint4(o[4], o[5], o[6], o[7]);
                 }
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&sh->full[s]);
@@ -631,78 +675,65 @@ __global__ void __launch_bounds__(threads<kFp8>(), 1) attn_kernel(const __grid_c
         }
         if constexpr (!kFp8) cp_wait_all();
     } else if (warp == kIndexWarp) {
-        // ---------------- index: slots, scales and masks of the tiles to come ----------------
+        // ---------------- index: slots, scales and validity of the tiles to come ----------------
         int ti = 0;
         bool ok = true;
-        const int pages = (int)(t.c.slots / t.page_size);
         do {
             const int nt = w.count(), ahead = w.shared_rows(qt) ? kAheadUnits : kAheadUnits / 2;
-            for (int t0 = 0; ok && t0 < nt; t0 += kBatch) {
-                int slot[kBatch][2];
-                float ks[kBatch][2], vs[kBatch][2];
+            const int* table = t.table + (long long)w.b * t.table_stride;
+            // a tile's page table entries are fetched one round of two tiles ahead
+            auto entry_of = [&](int tl, int e) {
+                const int pos = (w.k0 + tl) * kTile + e * 32 + lane;
+                return tl < nt && pos < w.r.len ? __ldg(table + a.page.divide(pos)) : 0;
+            };
+            int entry[2][2] = {{entry_of(0, 0), entry_of(0, 1)}, {entry_of(1, 0), entry_of(1, 1)}};
+#pragma unroll 1
+            for (int t0 = 0; ok && t0 < nt; t0 += 2) {
+                int now[2][2];
 #pragma unroll
-                for (int k = 0; k < kBatch; ++k) {
+                for (int k = 0; k < 2; ++k) {
 #pragma unroll
-                    for (int e = 0; e < 2; ++e) {
-                        const int pos = (w.k0 + t0 + k) * kTile + e * 32 + lane;
-                        slot[k][e] = -1;
-                        if (t0 + k < nt && pos < w.r.len) {
-                            const int page = pos / t.page_size;
-                            const int entry = __ldg(t.table + (long long)w.b * t.table_stride + page);
-                            if (entry >= 0 && entry < pages)
-                                slot[k][e] = entry * t.page_size + (pos - page * t.page_size);
-                            else if (t.err)
-                                atomicOr(t.err, 2u);
-                        }
-                    }
-                }
-                if constexpr (kFp8) {
-#pragma unroll
-                    for (int k = 0; k < kBatch; ++k) {
-#pragma unroll
-                        for (int e = 0; e < 2; ++e) {
-                            ks[k][e] = vs[k][e] = 0.f;
-                            if (slot[k][e] >= 0) {
-                                const long long at = slot[k][e] * t.c.scale_stride + w.h;
-                                ks[k][e] = __ldg(t.c.k_scale + at) * (t.scale * kL2E);
-                                vs[k][e] = __ldg(t.c.v_scale + at);
-                            }
-                        }
-                    }
+                    for (int e = 0; e < 2; ++e) now[k][e] = entry[k][e];
                 }
 #pragma unroll
-                for (int k = 0; k < kBatch; ++k) {
+                for (int k = 0; k < 2; ++k) {
+#pragma unroll
+                    for (int e = 0; e < 2; ++e) entry[k][e] = entry_of(t0 + 2 + k, e);
+                }
+#pragma unroll
+                for (int k = 0; k < 2; ++k) {
                     if (t0 + k >= nt) break;
                     const int at = ti % kInfo;
                     ok = __all_sync(0xffffffffu,
                                     wait_or_abort(&sh->info_empty[at], ((uint32_t)(ti / kInfo) & 1u) ^ 1u, abort));
                     if (!ok) break;
                     Info* f = info + at;
-                    f->slot[lane] = slot[k][0];
-                    f->slot[lane + 32] = slot[k][1];
-                    const uint32_t v0 = __ballot_sync(0xffffffffu, slot[k][0] >= 0);
-                    const uint32_t v1 = __ballot_sync(0xffffffffu, slot[k][1] >= 0);
-                    float top = 0.f;
-                    if constexpr (kFp8) {
-                        f->ks[lane] = ks[k][0];
-                        f->ks[lane + 32] = ks[k][1];
-                        f->vs[lane] = vs[k][0];
-                        f->vs[lane + 32] = vs[k][1];
-                        uint32_t bits = 0;                      // of finite sizes: ordered as they are
+                    uint32_t valid[2];
 #pragma unroll
-                        for (int e = 0; e < 2; ++e) {
-                            const uint32_t x = __float_as_uint(fabsf(vs[k][e]));
-                            if (x < 0x7f800000u) bits = max(bits, x);
+                    for (int e = 0; e < 2; ++e) {
+                        const int pos = (w.k0 + t0 + k) * kTile + e * 32 + lane, page = now[k][e];
+                        int slot = -1;
+                        if (pos < w.r.len) {
+                            if (page >= 0 && page < a.pages)
+                                slot = page * t.page_size + (pos - (int)a.page.divide(pos) * t.page_size);
+                            else if (t.err)
+                                atomicOr(t.err, 2u);
                         }
-                        top = __uint_as_float(__reduce_max_sync(0xffffffffu, bits));
+                        f->slot[e * 32 + lane] = slot;
+                        valid[e] = __ballot_sync(0xffffffffu, slot >= 0);
+                        if constexpr (kFp8) {
+                            const long long from = max(slot, 0) * t.c.scale_stride + w.h;
+                            cp4(smem_u32(f->ks + e * 32 + lane), t.c.k_scale + from, slot >= 0);
+                            cp4(smem_u32(f->vs + e * 32 + lane), t.c.v_scale + from, slot >= 0);
+                        }
                     }
+                    if constexpr (kFp8) cp_arrive(&sh->info_full[at]);
                     if (lane == 0) {
-                        f->valid[0] = v0;
-                        f->valid[1] = v1;
+                        f->valid[0] = valid[0];
+                        f->valid[1] = valid[1];
                         f->head = w.h;
                         f->tiles = nt;
                         f->ahead = ahead;
-                        f->vmax = top;
                     }
                     __syncwarp();
                     if (lane == 0) mbar_arrive(&sh->info_full[at]);
@@ -710,91 +741,96 @@ __global__ void __launch_bounds__(threads<kFp8>(), 1) attn_kernel(const __grid_c
                 }
             }
         } while (ok && w.advance(a));
-    } else if (warp == kMmaWarp) {
-        // ---------------- MMA issuer ----------------
-        {
-            constexpr uint32_t kFormat = std::is_same<TO, __nv_bfloat16>::value ? 1u : 0u;
-            constexpr uint32_t kCommon = (1u << 4) | (kFormat << 7) | (kFormat << 10) | ((uint32_t)(kRows >> 4) << 24);
-            constexpr uint32_t kIdescS = kCommon | ((uint32_t)(kTile >> 3) << 17);
-            const uint32_t idesc_o = kCommon | (1u << 16) | ((uint32_t)(t.c.dim >> 3) << 17);  // B: MN-major
-            const int ksteps = t.c.dim / 16;
-            const uint32_t q0 = desc_low(smem_u32(sq), 16), k0 = desc_low(smem_u32(ring), 16),
-                           v0 = desc_low(smem_u32(ring), kBlock);
-            uint32_t tile0 = 0, seg = 0, ph = 0;             // ph: parity of each (stream, buffer)
-            uint32_t st = 0, sp = 0;                         // next stage of the ring and its parity
-            bool ok = true;
-            auto wait_all = [&](uint64_t* bar, uint32_t parity) {
-                ok = __all_sync(0xffffffffu, wait_or_abort(bar, parity, abort));
-            };
-            // the next stage, filled: tiles are used in the order in which they are loaded
-            auto take_stage = [&]() {
-                const uint32_t mine = st;
-                wait_all(&sh->full[mine], sp);
-                fence_proxy_async_smem();
-                if (++st == (uint32_t)stages) {
-                    st = 0;
-                    sp ^= 1u;
-                }
-                return mine;
-            };
-            auto scores = [&](uint32_t sb, uint32_t stage, uint32_t q_off) {   // sb: 2 x stream + buffer
-                const uint32_t qa = q0 + q_off, kb = k0 + stage * (L::kStage >> 4), d = tmem + sb * kTile;
-#pragma unroll
-                for (int k = 0; k < DP / 16; ++k) {
-                    const uint32_t col = (k & 3) * 2;
-                    if (k < ksteps)
-                        mma_ss(d, desc(qa + (k >> 2) * (kQBlock >> 4) + col), desc(kb + (k >> 2) * (kBlock >> 4) + col), kIdescS,
-                               k != 0);
-                }
-                mma_commit(&sh->s_full[0][0] + sb);
-            };
-            auto weights = [&](uint32_t sb, uint32_t stage, uint32_t more) {   // O += P V
-                wait_all(&sh->p_full[0][0] + sb, (ph >> sb) & 1u);
-                if (!ok) return;
-                ph ^= 1u << sb;
-                fence_proxy_async_smem();
-                tc_fence_after();
-                const uint32_t vb = v0 + stage * (L::kStage >> 4), d = tmem + 256 + (sb >> 1) * 128, p = tmem + sb * kTile;
-#pragma unroll
-                for (int k = 0; k < kTile / 16; ++k) mma_ts(d, p + k * 8, desc(vb + k * (2048 >> 4)), idesc_o, k ? 1u : more);
-                mma_commit(&sh->pv_done[sb >> 1]);
-            };
-            do {
-                const bool both = !w.shared_rows(qt);        // both streams use every tile
-                const int nt = w.count();
-                wait_all(&sh->q_full, seg & 1u);
-                fence_proxy_async_smem();
-                tc_fence_after();
-                // unit u: stream u & 1, buffer (u >> 1) & 1; its tile u, or u >> 1 where both streams use it
-                const int units = both ? 2 * nt : nt;
-                uint32_t ks = 0, vs = 0;
-                for (int u = -kAheadUnits; ok && u < units; ++u) {
+        if constexpr (kFp8) cp_wait_all();
+    } else if (warp == kScoreWarp || warp == kAccumWarp) {
+        // ---------------- MMA issuers: one warp for S = Q K^T, one for O += P V ----------------
+        // Two, because a unit costs the issuing warp more in waits, commits and issue than the
+        // tensor core needs for it (one warp: 1960 cycles a unit of 640 tensor cycles).
+        constexpr uint32_t kFormat = std::is_same<TO, __nv_bfloat16>::value ? 1u : 0u;
+        constexpr uint32_t kCommon = (1u << 4) | (kFormat << 7) | (kFormat << 10) | ((uint32_t)(kRows >> 4) << 24);
+        constexpr uint32_t kIdescS = kCommon | ((uint32_t)(kTile >> 3) << 17);
+        const uint32_t bars = smem_u32(sh), full = bars + offsetof(Shared, full), empty = bars + offsetof(Shared, empty),
+                       s_full = bars + offsetof(Shared, s_full), p_full = bars + offsetof(Shared, p_full),
+                       s_free = bars + offsetof(Shared, s_free);
+        const bool scores = warp == kScoreWarp;
+        uint32_t seg = 0, tile0 = 0, ph = 0;                 // ph: parity of each (stream, buffer)
+        uint32_t st = 0, sp = 0;                             // stage of the ring, and its parity
+        bool ok = true;
+        auto skip = [&](uint32_t n) {                        // n items on
+            st += n;
+            if (st >= (uint32_t)stages) {
+                st -= stages;
+                sp ^= 1u;
+            }
+        };
+        do {
+            // broadcasts: what the loop turns on is uniform, and so its operands stay in uniform registers
+            const bool both = __shfl_sync(0xffffffffu, (int)!w.shared_rows(qt), 0) != 0;   // both streams use every tile
+            const int nt = __shfl_sync(0xffffffffu, w.count(), 0);
+            const int ahead = min(nt, both ? kAheadUnits / 2 : kAheadUnits);
+            // unit u: stream u & 1, buffer (u >> 1) & 1; its tile u, or u >> 1 where both streams use it
+            const uint32_t step = both ? 1u : 0u;
+            const int units = nt << step;
+            if (scores) {
+                const int ksteps = t.c.dim / 16;
+                const uint32_t q0 = desc_low(smem_u32(sq), 16), k0 = desc_low(smem_u32(ring), 16);
+                ok = wait_at(bars + offsetof(Shared, q_full), seg & 1u, abort);
+                int left = ahead;                            // K tiles before the first V tile
+                for (int u = 0; ok && u < units; ++u) {
                     const uint32_t s = u & 1, sb = (s << 1) | ((u >> 1) & 1);
-                    const bool fresh = !both || s == 0, last = !both || s == 1;   // first, last use of a tile
-                    if (u >= 0) {
-                        if (fresh) vs = take_stage();
-                        if (ok) weights(sb, vs, u > 1);
-                        if (!ok) break;
-                        if (last) {
-                            mma_commit(&sh->empty[vs]);
-                            mma_commit(&sh->info_empty[(tile0 + (both ? u >> 1 : u)) % kInfo]);
-                        }
+                    if (!(s & step)) ok = wait_at(full + 8 * st, sp, abort);
+                    ok = ok && wait_at(s_free + 8 * sb, ((ph >> sb) & 1u) ^ 1u, abort);
+                    if (!ok) break;
+                    ph ^= 1u << sb;
+                    fence_proxy_async_smem();
+                    tc_fence_after();
+                    const uint32_t qa = q0 + (s & step) * (L::kQTile >> 4), kb = k0 + st * (L::kStage >> 4), d = tmem + sb * kTile;
+#pragma unroll
+                    for (int k = 0; k < DP / 16; ++k) {
+                        const uint32_t col = (k & 3) * 2;
+                        if (k < ksteps)
+                            mma_ss(d, desc(qa + (k >> 2) * (kQBlock >> 4) + col), desc(kb + (k >> 2) * (kBlock >> 4) + col),
+                                   kIdescS, k != 0);
                     }
-                    if (u + kAheadUnits < units) {
-                        if (fresh) ks = take_stage();
-                        if (!ok) break;
-                        scores(sb, ks, both && s ? L::kQTile >> 4 : 0);
-                        if (last) mma_commit(&sh->empty[ks]);
+                    mma_commit(s_full + 8 * sb);
+                    if ((s & step) == step) {                // the last use of the tile
+                        mma_commit(empty + 8 * st);
+                        skip(u == units - 1 ? ahead + 1 : (--left > 0 ? 1 : 2));
                     }
                 }
-                if (ok) mma_commit(&sh->o_full);
-                tile0 += nt;
-                ++seg;
-            } while (ok && w.advance(a));
-            // every instruction issued here is done before TMEM is released
-            mma_commit(&sh->drain);
-            if (!mbar_wait_bounded(&sh->drain, 0)) *abort = 1;
-        }
+            } else {
+                const uint32_t v0 = desc_low(smem_u32(ring), kBlock);
+                const uint32_t idesc_o = kCommon | (1u << 16) | ((uint32_t)(t.c.dim >> 3) << 17);  // B: MN-major
+                int pairs = nt - ahead;                      // V tiles with a K tile behind them
+                skip(ahead);
+                for (int u = 0; ok && u < units; ++u) {
+                    const uint32_t s = u & 1, sb = (s << 1) | ((u >> 1) & 1);
+                    if (!(s & step)) ok = wait_at(full + 8 * st, sp, abort);
+                    ok = ok && wait_at(p_full + 8 * sb, (ph >> sb) & 1u, abort);
+                    if (!ok) break;
+                    ph ^= 1u << sb;
+                    fence_proxy_async_smem();
+                    tc_fence_after();
+                    const uint32_t vb = v0 + st * (L::kStage >> 4), d = tmem + 256 + s * 128, p = tmem + sb * kTile;
+#pragma unroll
+                    for (int k = 0; k < kTile / 16; ++k)
+                        mma_ts(d, p + k * 8, desc(vb + k * (2048 >> 4)), idesc_o, k ? 1u : (uint32_t)(u > 1));
+                    mma_commit(s_free + 8 * sb);
+                    if ((s & step) == step) {
+                        mma_commit(empty + 8 * st);
+                        mma_commit(bars + offsetof(Shared, info_empty) + 8 * ((tile0 + (u >> step)) % kInfo));
+                        skip(pairs-- > 0 ? 2 : 1);
+                    }
+                }
+                if (ok) mma_commit(bars + offsetof(Shared, o_full));
+            }
+            tile0 += nt;
+            ++seg;
+        } while (ok && __shfl_sync(0xffffffffu, (int)w.advance(a), 0) != 0);
+        // every instruction issued here is done before TMEM is released
+        uint64_t* drain = &sh->drain[scores ? 0 : 1];
+        mma_commit(smem_u32(drain));
+        if (!mbar_wait_bounded(drain, 0)) *abort = 1;
         __syncwarp();
     } else {
         // ---------------- softmax and epilogue: one row per thread ----------------
@@ -807,7 +843,7 @@ __global__ void __launch_bounds__(threads<kFp8>(), 1) attn_kernel(const __grid_c
         const bool sub_live = sub * 8 < t.c.dim;
         const uint32_t group_inv = (0xFFFFFFFFu / (uint32_t)t.group) + 1u;  // ceil(2^32 / group), 0 for 1
         uint32_t seg = 0, tile0 = 0, item = 0, jp = 0;          // jp: phases of `joined`
-        uint32_t ph = 0, su = 0;                                // parity of each buffer; units of the stream
+        uint32_t ph = 0;                                        // parity of each buffer
         bool ok = true;
         auto join = [&]() {                                     // both warpgroups have come here
             __syncwarp();
@@ -880,7 +916,7 @@ __global__ void __launch_bounds__(threads<kFp8>(), 1) attn_kernel(const __grid_c
                     ok = __all_sync(0xffffffffu, ok && wait_or_abort(&sh->q_full, seg & 1u, abort));
             }
             const bool any_row = (both ? s * kRows : 0) + quarter * 32 < nrows;  // this warp has rows
-            const float cm = kFp8 ? (any_row ? row_mul[my] : 1.f) : t.scale * kL2E;
+            const float cm = t.scale * kL2E * (kFp8 && any_row ? row_mul[my] : 1.f);
             int token = 0, gq = 0;                              // this row's drafted token and head
             uint64_t bits = 0;
             if (my < nrows) {
@@ -890,7 +926,7 @@ __global__ void __launch_bounds__(threads<kFp8>(), 1) attn_kernel(const __grid_c
             float ref = -INFINITY, sum = 0.f, vmax = 0.f;
             const int step = both ? 1 : 2, ahead = min(nt, both ? kAheadUnits / 2 : kAheadUnits);
             int b = 0;
-            for (int tl = both ? 0 : s; ok && tl < nt; tl += step, ++su, b ^= 1) {
+            for (int tl = both ? 0 : s; ok && tl < nt; tl += step, b ^= 1) {
                 const uint32_t ti = tile0 + tl, ts = tmem + lanes + s * 128 + b * kTile;
                 const Info* inf = info + ti % kInfo;
                 ok = wait_or_abort(&sh->info_full[ti % kInfo], (ti / kInfo) & 1u, abort) &&
@@ -942,6 +978,24 @@ __global__ void __launch_bounds__(threads<kFp8>(), 1) attn_kernel(const __grid_c
                     const uint2 valid = *reinterpret_cast<const uint2*>(inf->valid);
                     const bool masked = drafted || (valid.x & valid.y) != ~0u;
                     uint32_t vis[2] = {~0u, ~0u};
+                    if constexpr (kFp8) {
+                        // the largest V scale; a token whose V scale is not finite gets a K scale of NaN (the
+                        // rows that see it become NaN) and a V scale of 0 (the others do not); every warp
+                        // writes the same
+                        uint32_t top = 0;
+#pragma unroll
+                        for (int e = 0; e < 2; ++e) {
+                            const uint32_t x = __float_as_uint(fabsf(inf->vs[e * 32 + lane]));
+                            if (x >= 0x7f800000u) {
+                                const_cast<Info*>(inf)->ks[e * 32 + lane] = __int_as_float(0x7fffffff);
+                                const_cast<Info*>(inf)->vs[e * 32 + lane] = 0.f;
+                            } else {
+                                top = max(top, x);              // finite sizes: ordered as their bits
+                            }
+                        }
+                        vmax = fmaxf(vmax, __uint_as_float(__reduce_max_sync(0xffffffffu, top)));
+                        __syncwarp();
+                    }
                     if (masked) {
 #pragma unroll
                         for (int i = 0; i < 2; ++i) {
@@ -991,7 +1045,6 @@ __global__ void __launch_bounds__(threads<kFp8>(), 1) attn_kernel(const __grid_c
                     }
                     float target = fmaxf(mx[0], mx[1]) * cm;
                     if constexpr (kFp8) {
-                        vmax = fmaxf(vmax, inf->vmax);
                         // 2^ev is the first power of two above the V scales so far
                         const int ev = max(-90, min(120, (int)(__float_as_uint(vmax) >> 23) - 126));
                         target += (float)(ev - 6);
@@ -1001,7 +1054,7 @@ __global__ void __launch_bounds__(threads<kFp8>(), 1) attn_kernel(const __grid_c
                     if (__any_sync(0xffffffffu, target > ref + kSlack)) {
                         const float to_ref = fmaxf(ref, target);
                         if (tl >= step) {                       // the accumulator holds something
-                            ok = __all_sync(0xffffffffu, wait_or_abort(&sh->pv_done[s], (su - 1) & 1u, abort));
+                            ok = __all_sync(0xffffffffu, wait_or_abort(&sh->s_free[s][b ^ 1], ((ph >> (b ^ 1)) & 1u) ^ 1u, abort));
                             if (!ok) break;
                             tc_fence_after();
                             const float f = ref == -INFINITY ? 1.0f : ex2(ref - to_ref);
@@ -1036,12 +1089,6 @@ __global__ void __launch_bounds__(threads<kFp8>(), 1) attn_kernel(const __grid_c
                                 const float4 v4 = *reinterpret_cast<const float4*>(&inf->vs[c * 32 + j]);
                                 lo = __fmul2_rn(lo, make_float2(v4.x, v4.y));
                                 hi = __fmul2_rn(hi, make_float2(v4.z, v4.w));
-                                if (masked) {                   // 0 x a scale that is not finite
-                                    if (!((vis[c] >> j) & 1u)) lo.x = 0.f;
-                                    if (!((vis[c] >> (j + 1)) & 1u)) lo.y = 0.f;
-                                    if (!((vis[c] >> (j + 2)) & 1u)) hi.x = 0.f;
-                                    if (!((vis[c] >> (j + 3)) & 1u)) hi.y = 0.f;
-                                }
                             }
                             p[j / 2] = pack2(lo.x, lo.y, TO());
                             p[j / 2 + 1] = pack2(hi.x, hi.y, TO());
@@ -1174,7 +1221,7 @@ __global__ void __launch_bounds__(threads<kFp8>(), 1) attn_kernel(const __grid_c
 
     __syncthreads();
     if (tid == 0 && *abort && t.err) atomicOr(t.err, 4u);
-    if (warp == kMmaWarp) {
+    if (warp == kScoreWarp) {
         tc_fence_after();
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(sh->tmem) : "memory");
     }
@@ -1229,6 +1276,13 @@ __global__ void __launch_bounds__(kCombineThreads) combine_kernel(const __grid_c
 
 // ---- host side ---------------------------------------------------------------------------------
 
+Divisor divisor(uint32_t d) {
+    int l = 0;
+    while ((1ull << l) < d) ++l;
+    const uint64_t mul = ((((1ull << l) - d) << 32) / d) + 1;
+    return {(uint32_t)mul, l < 1 ? l : 1, l > 1 ? l - 1 : 0};
+}
+
 int q_tiles(int group, int width) { return (long long)group * width > kRows ? 2 : 1; }
 int padded_dim(int dim) { return dim <= 64 ? 64 : 128; }
 
@@ -1275,6 +1329,8 @@ int launch_tree_attn(const TreeAttnArgs& t, int dtype, cudaStream_t st) {
     KernelArgs a = {};
     a.t = t;
     a.qt = q_tiles(t.group, t.width);
+    a.page = divisor((uint32_t)t.page_size);
+    a.pages = (int)(t.c.slots / t.page_size);
     char* ws = static_cast<char*>(t.ws);
     a.splits = reinterpret_cast<Split*>(ws);
     a.part_ml = reinterpret_cast<float2*>(ws + kSplitBytes);
