@@ -15,7 +15,7 @@ from dataclasses import dataclass
 import torch
 
 from . import _lib
-from .kvcache import on_device
+from .kvcache import launch
 from .verify import CompactOutputs, Workspace, new_outputs, workspace_for  # noqa: F401
 
 T = 16
@@ -92,12 +92,20 @@ class TreeAccept:
 
     @staticmethod
     def allocate(batch: int, width: int, device, *, slots=True) -> "TreeAccept":
-        def empty(*shape, dtype=torch.int32):
-            return torch.empty(shape, dtype=dtype, device=device)
+        """Outputs for `batch` requests, parts of two allocations."""
+        n = batch * width
+        bonus, output = torch.empty(batch + n, dtype=torch.int64, device=device).split((batch, n))
+        small = torch.empty(3 * batch + (2 if slots else 1) * n, dtype=torch.int32, device=device)
+        accept, commit, new_seq, path, *kept = small.split((batch, batch, batch, n, n) if slots else (batch, batch, batch, n))
+        shape = (batch, width)
+        return TreeAccept(accept, commit, bonus, output.view(shape), path.view(shape), kept[0].view(shape) if slots else None, new_seq)
 
-        return TreeAccept(empty(batch), empty(batch), empty(batch, dtype=torch.int64),
-                          empty(batch, width, dtype=torch.int64), empty(batch, width),
-                          empty(batch, width) if slots else None, empty(batch))
+    def _check(self, batch, width, dev, slots):
+        for x, shape, dtype in ((self.accept, (batch,), torch.int32), (self.commit, (batch,), torch.int32), (self.bonus, (batch,), torch.int64),
+                                (self.output, (batch, width), torch.int64), (self.path, (batch, width), torch.int32),
+                                (self.new_seq, (batch,), torch.int32)) + (((self.kept_slots, (batch, width), torch.int32),) if slots else ()):
+            _check(x is not None and x.shape == shape and x.dtype == dtype and x.device == dev and x.is_contiguous(),
+                   "outputs must be as TreeAccept.allocate gives them")
 
 
 def accept_tree(tokens, top1, tree_mask, *, q_indptr=None, prefix_lens=None, slots=None, width=None, outputs=None):
@@ -115,38 +123,40 @@ def accept_tree(tokens, top1, tree_mask, *, q_indptr=None, prefix_lens=None, slo
     when None) + commit.  At most the first `width` (<= 64, default 64 or nodes) rows of a request
     are looked at; a request without rows gets commit 0 and bonus -1."""
     dev = tokens.device
+    shape = tokens.shape
     if q_indptr is None:
-        _check(tokens.dim() == 2, "without q_indptr tokens must be [requests, nodes]")
-        B, nodes = tokens.shape
+        _check(len(shape) == 2, "without q_indptr tokens must be [requests, nodes]")
+        B, nodes = shape
         width = max(1, nodes) if width is None else int(width)
         _check(nodes <= width, "width must hold every node")
+        indptr, rows = None, B * nodes
     else:
-        _check(tokens.dim() == 1, "with q_indptr tokens must be [rows]")
+        _check(len(shape) == 1, "with q_indptr tokens must be [rows]")
         _check(q_indptr.dim() == 1 and q_indptr.shape[0] >= 1 and q_indptr.dtype == torch.int32 and q_indptr.device == dev
                and q_indptr.is_contiguous(), "q_indptr must be contiguous int32 [requests + 1]")
         B, nodes = q_indptr.shape[0] - 1, 0
         width = 64 if width is None else int(width)
+        indptr, rows = q_indptr.data_ptr(), shape[0]
     _check(1 <= width <= 64, "a draft tree has at most 64 nodes")
-    for name, x in (("tokens", tokens), ("top1", top1), ("tree_mask", tree_mask)):
-        _check(x.shape == tokens.shape and x.dtype == torch.int64 and x.is_contiguous() and x.device == dev,
-               f"{name} must be contiguous int64, one value a node")
-    _check(prefix_lens is None or (prefix_lens.shape == (B,) and prefix_lens.dtype == torch.int32 and prefix_lens.device == dev
-                                   and prefix_lens.is_contiguous()), "prefix_lens must be contiguous int32 [requests]")
-    _check(slots is None or (slots.shape == tokens.shape and slots.dtype == torch.int32 and slots.device == dev
-                             and slots.is_contiguous()), "slots must be contiguous int32, one value a node")
+    for x in (tokens, top1, tree_mask):
+        if x.dtype != torch.int64 or x.shape != shape or x.device != dev or not x.is_contiguous():
+            name = "tokens" if x is tokens else ("top1" if x is top1 else "tree_mask")
+            _check(False, f"{name} must be contiguous int64, one value a node")
+    if prefix_lens is not None:
+        _check(prefix_lens.dtype == torch.int32 and prefix_lens.shape == (B,) and prefix_lens.device == dev and prefix_lens.is_contiguous(),
+               "prefix_lens must be contiguous int32 [requests]")
+    if slots is not None:
+        _check(slots.dtype == torch.int32 and slots.shape == shape and slots.device == dev and slots.is_contiguous(),
+               "slots must be contiguous int32, one value a node")
     if outputs is None:
         outputs = TreeAccept.allocate(B, width, dev, slots=slots is not None)
-    o = outputs
-    for x, shape, dtype in ((o.accept, (B,), torch.int32), (o.commit, (B,), torch.int32), (o.bonus, (B,), torch.int64),
-                            (o.output, (B, width), torch.int64), (o.path, (B, width), torch.int32),
-                            (o.new_seq, (B,), torch.int32)) + (((o.kept_slots, (B, width), torch.int32),) if slots is not None else ()):
-        _check(x is not None and x.shape == shape and x.dtype == dtype and x.device == dev and x.is_contiguous(),
-               "outputs must be as TreeAccept.allocate gives them")
+    else:
+        outputs._check(B, width, dev, slots is not None)
     _check(dev.type == "cuda", "tensors must be on a CUDA device")
+    o = outputs
     if B:
-        with on_device(dev) as stream:
-            _lib.call("dsv_accept_tree", B, tokens.numel(), tokens.data_ptr(), top1.data_ptr(), tree_mask.data_ptr(),
-                      _lib.ptr(q_indptr), nodes, _lib.ptr(prefix_lens), _lib.ptr(slots), width, o.accept.data_ptr(),
-                      o.commit.data_ptr(), o.bonus.data_ptr(), o.output.data_ptr(), o.path.data_ptr(),
-                      o.kept_slots.data_ptr() if slots is not None else None, o.new_seq.data_ptr(), stream)
+        launch("dsv_accept_tree", dev, B, rows, tokens.data_ptr(), top1.data_ptr(), tree_mask.data_ptr(), indptr, nodes,
+               None if prefix_lens is None else prefix_lens.data_ptr(), None if slots is None else slots.data_ptr(), width,
+               o.accept.data_ptr(), o.commit.data_ptr(), o.bonus.data_ptr(), o.output.data_ptr(), o.path.data_ptr(),
+               None if slots is None else o.kept_slots.data_ptr(), o.new_seq.data_ptr())
     return outputs

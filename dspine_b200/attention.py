@@ -15,7 +15,7 @@ import math
 import torch
 
 from . import _lib
-from .kvcache import _check, check_err, describe, on_device
+from .kvcache import _check, check_err, describe, launch
 
 MAX_DIM = 128
 MAX_NODES = 64
@@ -77,61 +77,77 @@ def tree_attention(q, k_cache, v_cache, page_table, kv_lens, *, page_size=1, q_i
     reaches the rows that see it alone, infinities and NaN included."""
     c = describe(k_cache, v_cache, k_scale, v_scale)
     dev = k_cache.device
-    _check(q.dim() == 3 and q.dtype in _DTYPES, "q must be bf16 or fp16 [rows, q_heads, dim]")
-    rows, q_heads, dim = q.shape
-    dtype = _DTYPES[q.dtype]
-    _check(dim == c.dim and dim <= MAX_DIM, f"q and the cache must have one dim, at most {MAX_DIM}")
-    _check(q_heads >= 1 and q_heads % c.heads == 0 and q_heads <= 4096 * c.heads,
+    shape = q.shape
+    dtype = _DTYPES.get(q.dtype)
+    _check(len(shape) == 3 and dtype is not None, "q must be bf16 or fp16 [rows, q_heads, dim]")
+    rows, q_heads, dim = shape
+    heads = c.heads
+    _check(dim == c.dim and dim <= MAX_DIM, "q and the cache must have one dim, at most 128")
+    _check(q_heads >= 1 and q_heads % heads == 0 and q_heads <= 4096 * heads,
            "q_heads must be a multiple of the cache's heads, at most 4096 of them each")
     _check(c.dtype == 3 or c.dtype == dtype, "the cache must have q's type or be e4m3")
-    _check(page_table.dim() == 2 and page_table.dtype == torch.int32, "page_table must be int32 [requests, pages]")
+    _check(page_table.dtype == torch.int32 and page_table.dim() == 2, "page_table must be int32 [requests, pages]")
     batch, pages = page_table.shape
-    _check(pages <= 1 or page_table.stride(1) == 1, "page_table's rows must be contiguous")
-    _check(batch <= 1 or page_table.stride(0) >= pages, "page_table's rows overlap")
-    _check(kv_lens.shape == (batch,) and kv_lens.dtype == torch.int32 and (batch <= 1 or kv_lens.stride(0) == 1),
-           "kv_lens must be contiguous int32 [requests]")
+    table_stride, one = page_table.stride()
+    _check(one == 1 or pages <= 1, "page_table's rows must be contiguous")
+    if batch <= 1:
+        table_stride = pages
+    _check(table_stride >= pages, "page_table's rows overlap")
+    _check(kv_lens.dtype == torch.int32 and kv_lens.shape == (batch,) and kv_lens.is_contiguous(), "kv_lens must be contiguous int32 [requests]")
     page_size = int(page_size)
     _check(page_size >= 1 and c.slots % page_size == 0, "the cache must hold whole pages of page_size slots")
+    _check(q.device == dev and page_table.device == dev and kv_lens.device == dev, "tensors must be on one CUDA device")
     if q_indptr is None:
         _check(batch > 0 and rows % batch == 0 or rows == 0, "without q_indptr every request has the same number of rows")
         width = max(1, rows // max(batch, 1))
-        _check(tree_mask is None or width <= MAX_NODES, f"a draft tree has at most {MAX_NODES} nodes")
+        _check(tree_mask is None or width <= MAX_NODES, "a draft tree has at most 64 nodes")
+        indptr = None
     else:
-        _check(q_indptr.shape == (batch + 1,) and q_indptr.dtype == torch.int32 and (batch < 1 or q_indptr.stride(0) == 1),
+        _check(q_indptr.dtype == torch.int32 and q_indptr.shape == (batch + 1,) and q_indptr.is_contiguous(),
                "q_indptr must be contiguous int32 [requests + 1]")
+        _check(q_indptr.device == dev, "tensors must be on one CUDA device")
         width = (max(rows, 1) if tree_mask is None else MAX_NODES) if max_width is None else int(max_width)
         _check(width >= 1, "max_width must be at least 1")
-        _check(q_indptr.device == dev, "tensors must be on one CUDA device")
+        indptr = q_indptr.data_ptr()
+    mask = None
     if tree_mask is not None:
-        _check(tree_mask.shape == (rows,) and tree_mask.dtype == torch.int64 and (rows <= 1 or tree_mask.stride(0) == 1),
+        _check(tree_mask.dtype == torch.int64 and tree_mask.shape == (rows,) and tree_mask.is_contiguous(),
                "tree_mask must be contiguous int64 [rows]")
         _check(tree_mask.device == dev, "tensors must be on one CUDA device")
-    _check(q.device == dev and page_table.device == dev and kv_lens.device == dev, "tensors must be on one CUDA device")
+        mask = tree_mask.data_ptr()
     scale = 1.0 / math.sqrt(dim) if scale is None else float(scale)
     _check(0.0 < scale < 3.4e38, "scale must be positive and finite")
+    q_stride, q_head_stride, one = q.stride()
+    _check(one == 1 or rows == 0, "rows of q and out must be contiguous")
     if out is None:
-        out = torch.empty((rows, q_heads, dim), dtype=q.dtype, device=dev)
-    _check(out.shape == q.shape and out.dtype == q.dtype and out.device == dev, "out must be like q")
-    for x in (q, out):
-        _check(rows == 0 or x.stride(2) == 1, "rows of q and out must be contiguous")
-    _check((rows <= 1 or out.stride(0) >= dim) and (q_heads == 1 or out.stride(1) >= dim), "the rows of out overlap")
-    if lse is None and return_lse:
+        out = torch.empty(shape, dtype=q.dtype, device=dev)
+        out_stride, out_head_stride = q_heads * dim, dim
+    else:
+        _check(out.shape == shape and out.dtype == q.dtype and out.device == dev, "out must be like q")
+        out_stride, out_head_stride, one = out.stride()
+        _check(one == 1 or rows == 0, "rows of q and out must be contiguous")
+        _check((rows <= 1 or out_stride >= dim) and (q_heads == 1 or out_head_stride >= dim), "the rows of out overlap")
+    if lse is not None:
+        _check(lse.shape == (rows, q_heads) and lse.dtype == torch.float32 and lse.is_contiguous() and lse.device == dev,
+               "lse must be contiguous fp32 [rows, q_heads]")
+    elif return_lse:
         lse = torch.empty((rows, q_heads), dtype=torch.float32, device=dev)
-    _check(lse is None or (lse.shape == (rows, q_heads) and lse.dtype == torch.float32 and lse.is_contiguous() and lse.device == dev),
-           "lse must be contiguous fp32 [rows, q_heads]")
-    check_err(err, dev)
+    if err is not None:
+        check_err(err, dev)
     _check(dev.type == "cuda", "tensors must be on a CUDA device")
     if rows and batch:
-        need = workspace_bytes(q_heads, c.heads, dim, width)
-        with on_device(dev) as stream:
-            if workspace is None:
-                workspace = torch.empty(need, dtype=torch.uint8, device=dev)
+        need = workspace_bytes(q_heads, heads, dim, width)
+        if workspace is None:
+            workspace = torch.empty(need, dtype=torch.uint8, device=dev)
+        else:
             _check(workspace.dtype == torch.uint8 and workspace.is_contiguous() and workspace.numel() >= need and workspace.device == dev,
-                   f"workspace must be {need} bytes (uint8) on the cache's device")
-            _lib.call("dsv_tree_attention", batch, rows, q_heads, dtype, q.data_ptr(), q.stride(0) if rows > 1 else 0,
-                      q.stride(1) if q_heads > 1 else 0, c, page_table.data_ptr() if pages else None,
-                      page_table.stride(0) if batch > 1 else pages, pages, page_size, kv_lens.data_ptr(), _lib.ptr(q_indptr), width,
-                      _lib.ptr(tree_mask), scale, out.data_ptr(), out.stride(0) if rows > 1 else 0,
-                      out.stride(1) if q_heads > 1 else 0, _lib.ptr(lse), _lib.ptr(err), workspace.data_ptr() if need else None,
-                      workspace.numel(), stream)
+                   "workspace must be workspace_bytes(...) bytes (uint8) on the cache's device")
+        if rows == 1:
+            q_stride = out_stride = 0
+        if q_heads == 1:
+            q_head_stride = out_head_stride = 0
+        launch("dsv_tree_attention", dev, batch, rows, q_heads, dtype, q.data_ptr(), q_stride, q_head_stride, c,
+               page_table.data_ptr() if pages else None, table_stride, pages, page_size, kv_lens.data_ptr(), indptr, width, mask, scale,
+               out.data_ptr(), out_stride, out_head_stride, None if lse is None else lse.data_ptr(), None if err is None else err.data_ptr(),
+               workspace.data_ptr(), workspace.numel())
     return (out, lse) if return_lse else out

@@ -16,6 +16,7 @@ from . import _lib
 
 E4M3 = torch.float8_e4m3fn
 _CACHE = {torch.bfloat16: 0, torch.float16: 2, E4M3: 3}
+_INDEX = {torch.int32: 0, torch.int64: 1}
 _ROWS = {torch.bfloat16: 0, torch.float32: 1, torch.float16: 2}
 
 
@@ -24,25 +25,24 @@ def _check(cond, msg):
         raise ValueError(msg)
 
 
-class on_device:
-    """The tensors' device made current for a launch (nothing to do where it is already)."""
+# the cheap forms of torch.cuda.current_device() and current_stream(index).cuda_stream
+_current_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", lambda index: torch.cuda.current_stream(index).cuda_stream)
 
-    __slots__ = ("index", "before")
 
-    def __init__(self, device):
-        self.index = device.index
-        self.before = None
-
-    def __enter__(self):
-        now = torch.cuda.current_device()
-        if now != self.index:
-            self.before = now
-            torch.cuda.set_device(self.index)
-        return torch.cuda.current_stream(self.index).cuda_stream
-
-    def __exit__(self, *exc):
-        if self.before is not None:
-            torch.cuda.set_device(self.before)
+def launch(fn, dev, *args):
+    """Call the C entry `fn` with the current stream of `dev` as its last argument, `dev` made current for
+    the launch where it is not."""
+    index = dev.index
+    now = _current_device()
+    if now == index:
+        _lib.call(fn, *args, _raw_stream(index))
+        return
+    torch.cuda.set_device(index)
+    try:
+        _lib.call(fn, *args, _raw_stream(index))
+    finally:
+        torch.cuda.set_device(now)
 
 
 def allocate_kv(slots, heads, dim, *, dtype=torch.bfloat16, device="cuda"):
@@ -60,44 +60,53 @@ def allocate_kv(slots, heads, dim, *, dtype=torch.bfloat16, device="cuda"):
 
 def describe(k_cache, v_cache, k_scale, v_scale):
     """The C view of a cache (_lib.KvCache), its tensors checked."""
-    _check(k_cache.dim() == 3 and k_cache.shape == v_cache.shape, "k_cache and v_cache must be [slots, heads, dim]")
+    shape, s = k_cache.shape, k_cache.stride()
     dtype = _CACHE.get(k_cache.dtype)
-    _check(dtype is not None and v_cache.dtype == k_cache.dtype, f"a KV cache holds bf16, fp16 or e4m3 rows, got {k_cache.dtype}, {v_cache.dtype}")
-    slots, heads, dim = k_cache.shape
-    s = k_cache.stride()
-    _check(s == v_cache.stride() and (s[2] == 1 or dim == 1), "k_cache and v_cache must have the same strides and contiguous rows")
     dev = k_cache.device
-    _check(v_cache.device == dev, "the cache must be on one device")
-    _check(dim % 16 == 0 and dim >= 16, "dim must be a multiple of 16")
-    _check(slots >= 1 and heads >= 1, "the cache has no slots")
+    if dtype is None or len(shape) != 3 or v_cache.shape != shape or v_cache.dtype != k_cache.dtype or v_cache.stride() != s or v_cache.device != dev:
+        _check(k_cache.dim() == 3 and v_cache.shape == shape, "k_cache and v_cache must be [slots, heads, dim]")
+        _check(dtype is not None and v_cache.dtype == k_cache.dtype,
+               f"a KV cache holds bf16, fp16 or e4m3 rows, got {k_cache.dtype}, {v_cache.dtype}")
+        _check(v_cache.device == dev, "the cache must be on one device")
+        _check(False, "k_cache and v_cache must have the same strides and contiguous rows")
+    slots, heads, dim = shape
+    slot_stride, head_stride, one = s
     step = 16 if dtype == 3 else 8
-    _check((slots == 1 or (s[0] >= dim and s[0] % step == 0)) and (heads == 1 or (s[1] >= dim and s[1] % step == 0)),
-           "the cache's rows must be 16-byte aligned and not overlap")
+    if dim % 16 or not dim or one != 1 or slots < 1 or heads < 1:
+        _check(dim % 16 == 0 and dim >= 16, "dim must be a multiple of 16")
+        _check(one == 1, "k_cache and v_cache must have the same strides and contiguous rows")
+        _check(False, "the cache has no slots")
     # a dimension of one element may carry any stride: it is never stepped over
-    slot_stride = s[0] if slots > 1 else max(heads * dim, dim)
-    head_stride = s[1] if heads > 1 else dim
-    if dtype == 3:
-        _check(k_scale is not None and v_scale is not None, "an e4m3 cache needs k_scale and v_scale")
-        for x in (k_scale, v_scale):
-            _check(x.shape == (slots, heads) and x.dtype == torch.float32 and x.device == dev, "k_scale and v_scale must be fp32 [slots, heads]")
-            _check(heads == 1 or x.stride(1) == 1, "a slot's scales must be adjacent")
-        _check(k_scale.stride(0) == v_scale.stride(0) or slots == 1, "k_scale and v_scale must have the same strides")
-        scale_stride = k_scale.stride(0) if slots > 1 else heads
-        _check(scale_stride >= heads, "the scales of two slots overlap")
-        ks, vs = k_scale.data_ptr(), v_scale.data_ptr()
-    else:
+    if slots == 1:
+        slot_stride = heads * dim
+    if heads == 1:
+        head_stride = dim
+    if slot_stride < dim or slot_stride % step or head_stride < dim or head_stride % step:
+        _check(False, "the cache's rows must be 16-byte aligned and not overlap")
+    if dtype != 3:
         _check(k_scale is None and v_scale is None, "only an e4m3 cache has scales")
-        ks = vs = None
-        scale_stride = heads
-    return _lib.KvCache(k_cache.data_ptr(), v_cache.data_ptr(), ks, vs, slots, slot_stride, head_stride, scale_stride,
-                        heads, dim, dtype)
+        return _lib.KvCache(k_cache.data_ptr(), v_cache.data_ptr(), None, None, slots, slot_stride, head_stride, heads, heads, dim,
+                            dtype)
+    _check(k_scale is not None and v_scale is not None, "an e4m3 cache needs k_scale and v_scale")
+    for x in (k_scale, v_scale):
+        if x.shape != (slots, heads) or x.dtype != torch.float32 or x.device != dev:
+            _check(False, "k_scale and v_scale must be fp32 [slots, heads]")
+    ss = k_scale.stride()
+    if ss != v_scale.stride() or (heads > 1 and ss[1] != 1):
+        _check(heads == 1 or (ss[1] == 1 and v_scale.stride(1) == 1), "a slot's scales must be adjacent")
+        _check(slots == 1, "k_scale and v_scale must have the same strides")
+    scale_stride = ss[0] if slots > 1 else heads
+    _check(scale_stride >= heads, "the scales of two slots overlap")
+    return _lib.KvCache(k_cache.data_ptr(), v_cache.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), slots, slot_stride, head_stride,
+                        scale_stride, heads, dim, dtype)
 
 
-def _slots(slots, n, dev):
-    _check(slots.dim() == 1 and (n is None or slots.shape[0] == n), "slots must be [tokens]")
-    _check(slots.dtype in (torch.int32, torch.int64) and slots.device == dev, "slots must be int32 or int64 on the cache's device")
-    _check(slots.shape[0] <= 1 or slots.stride(0) == 1, "slots must be contiguous")
-    return int(slots.dtype == torch.int64)
+def _slots(slots, dev):
+    if slots.dim() != 1 or slots.dtype not in _INDEX or slots.device != dev or not slots.is_contiguous():
+        _check(slots.dim() == 1, "slots must be [tokens]")
+        _check(slots.dtype in _INDEX and slots.device == dev, "slots must be int32 or int64 on the cache's device")
+        _check(False, "slots must be contiguous")
+    return _INDEX[slots.dtype]
 
 
 def check_err(err, dev):
@@ -114,24 +123,30 @@ def write_kv(k, v, k_cache, v_cache, slots, *, k_scale=None, v_scale=None, err=N
     slots of one call should differ: of tokens that share one, any may be kept, or a mixture."""
     c = describe(k_cache, v_cache, k_scale, v_scale)
     dev = k_cache.device
-    _check(k.dim() == 3 and v.dim() == 3 and k.shape == v.shape and k.shape[1:] == k_cache.shape[1:],
-           "k and v must be [tokens, heads, dim] as the cache")
+    shape = k.shape
+    _check(len(shape) == 3 and v.shape == shape and shape[1] == c.heads and shape[2] == c.dim, "k and v must be [tokens, heads, dim] as the cache")
     dtype = _ROWS.get(k.dtype)
-    _check(dtype is not None and v.dtype == k.dtype, f"rows must be bf16, fp16 or fp32, got {k.dtype}, {v.dtype}")
+    if dtype is None or v.dtype != k.dtype:
+        _check(False, f"rows must be bf16, fp16 or fp32, got {k.dtype}, {v.dtype}")
     _check(c.dtype == 3 or c.dtype == dtype, "a cache that is not e4m3 takes rows of its own type")
     _check(k.device == dev and v.device == dev, "tensors must be on one CUDA device")
-    _check(k.stride(2) == 1 and v.stride(2) == 1, "rows must be contiguous")
+    (kt, kh, k1), (vt, vh, v1) = k.stride(), v.stride()
+    _check(k1 == 1 and v1 == 1, "rows must be contiguous")
     _check(c.dim <= 256, "dim must be at most 256")
-    is64 = _slots(slots, k.shape[0], dev)
-    check_err(err, dev)
+    is64 = _slots(slots, dev)
+    n = shape[0]
+    _check(slots.shape[0] == n, "slots must be [tokens]")
+    if err is not None:
+        check_err(err, dev)
     _check(dev.type == "cuda", "the cache must be on a CUDA device")
-    n = k.shape[0]
     if n == 0:
         return
-    with on_device(dev) as stream:
-        _lib.call("dsv_kv_write", n, dtype, k.data_ptr(), k.stride(0) if n > 1 else 0, k.stride(1) if c.heads > 1 else 0,
-                  v.data_ptr(), v.stride(0) if n > 1 else 0, v.stride(1) if c.heads > 1 else 0, slots.data_ptr(), is64,
-                  c, _lib.ptr(err), stream)
+    if n == 1:
+        kt = vt = 0
+    if c.heads == 1:
+        kh = vh = 0
+    launch("dsv_kv_write", dev, n, dtype, k.data_ptr(), kt, kh, v.data_ptr(), vt, vh, slots.data_ptr(), is64, c,
+           None if err is None else err.data_ptr())
 
 
 def read_kv(k_cache, v_cache, slots, *, k_scale=None, v_scale=None, dtype=torch.bfloat16, out=None, err=None):
@@ -141,20 +156,24 @@ def read_kv(k_cache, v_cache, slots, *, k_scale=None, v_scale=None, dtype=torch.
     c = describe(k_cache, v_cache, k_scale, v_scale)
     dev = k_cache.device
     _check(c.dim <= 256, "dim must be at most 256")
-    is64 = _slots(slots, None, dev)
-    check_err(err, dev)
+    is64 = _slots(slots, dev)
+    if err is not None:
+        check_err(err, dev)
     n = slots.shape[0]
     shape = (n, c.heads, c.dim)
     if out is None:
-        _check(dtype in _ROWS, f"rows are read as bf16, fp16 or fp32, got {dtype}")
-        out = (torch.empty(shape, dtype=dtype, device=dev), torch.empty(shape, dtype=dtype, device=dev))
-    k, v = out
-    for x in out:
-        _check(x.shape == shape and x.dtype in _ROWS and x.dtype == k.dtype and x.is_contiguous() and x.device == dev,
-               "out must be two contiguous [tokens, heads, dim] tensors of bf16, fp16 or fp32")
+        code = _ROWS.get(dtype)
+        if code is None:
+            _check(False, f"rows are read as bf16, fp16 or fp32, got {dtype}")
+        k = torch.empty(shape, dtype=dtype, device=dev)
+        v = torch.empty_like(k)
+    else:
+        k, v = out
+        code = _ROWS.get(k.dtype)
+        for x in out:
+            _check(code is not None and x.shape == shape and x.dtype == k.dtype and x.is_contiguous() and x.device == dev,
+                   "out must be two contiguous [tokens, heads, dim] tensors of bf16, fp16 or fp32")
     _check(dev.type == "cuda", "the cache must be on a CUDA device")
     if n:
-        with on_device(dev) as stream:
-            _lib.call("dsv_kv_read", n, slots.data_ptr(), is64, c, _ROWS[k.dtype], k.data_ptr(), v.data_ptr(),
-                      _lib.ptr(err), stream)
+        launch("dsv_kv_read", dev, n, slots.data_ptr(), is64, c, code, k.data_ptr(), v.data_ptr(), None if err is None else err.data_ptr())
     return k, v
