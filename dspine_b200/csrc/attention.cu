@@ -19,8 +19,8 @@
 //                                  scores of a tile in registers
 //                     warps 8, 9   MMA issuers: scores (and TMEM allocation), accumulation
 //                     warp 10      index: slots, scales and validity of the tiles to come
-//                     warps 11..   producers: K and V rows of a tile, slot by slot, into a ring of
-//                                  128-byte-swizzled shared-memory stages
+//                     warps 11..   loaders: K and V rows of a tile, slot by slot, into a ring of
+//                                  128-byte-swizzled shared-memory stages (e4m3: converted on the way)
 //                   S = Q K^T (kind::f16, both operands in shared memory) and O += P V (P from
 //                   TMEM, written over S; V as a matrix with rows of keys, "MN-major").
 //                   Two streams keep the tensor core and the exponentials busy at once: with more
@@ -37,8 +37,8 @@
 // 2^8 keeps fp16 weights below 2^14.  Sums and the accumulator are fp32; the weights are rounded
 // once to the operand type.
 //
-// e4m3 caches: codes are exact in fp16, so the producers convert them on the way into shared
-// memory and the matrix instructions run on fp16.  q goes to fp16 with a power of two per row.  K
+// e4m3 caches: codes are exact in fp16, so they are converted between two rings in shared memory
+// and the matrix instructions run on fp16.  q goes to fp16 with a power of two per row.  K
 // scales multiply the scores; V scales multiply the weights, and the reference moves by the running
 // maximum of the V scales (a power of two) so that weight x scale stays within fp16.
 //
@@ -74,14 +74,14 @@ constexpr float kSlack = 8.0f;             // log2 by which a maximum may outgro
 constexpr float kL2E = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
 
-// warps 0-7 softmax, 8 and 9 MMA issuers (scores, accumulation), 10 index, 11.. producers
-constexpr int kScoreWarp = 8, kAccumWarp = 9, kIndexWarp = 10, kFirstProducer = 11;
-template <bool kFp8> constexpr int producers() { return kFp8 ? 5 : 4; }
-template <bool kFp8> constexpr int threads() { return 32 * (kFirstProducer + producers<kFp8>()); }
+// warps 0-7 softmax, 8 and 9 MMA issuers (scores, accumulation), 10 index, 11.. loaders
+constexpr int kScoreWarp = 8, kAccumWarp = 9, kIndexWarp = 10, kFirstLoader = 11;
+template <bool kFp8> constexpr int loaders() { return kFp8 ? 4 : 2; }
+template <bool kFp8> constexpr int threads() { return 32 * (kFirstLoader + loaders<kFp8>()); }
 
 // a tile of keys, as the index warp describes it to the others
 struct alignas(16) TileInfoPlain {
-    int slot[kTile];          // of each position; -1 where there is none or it cannot be read
+    int slot[kTile];          // of each position; 0 where there is none or it cannot be read
     uint32_t valid[2];        // the positions with a slot
     int head, tiles, ahead;   // of the segment: KV head, tiles, K tiles loaded before its first V tile
     int pad;
@@ -241,6 +241,7 @@ struct Walk {
 };
 
 constexpr int kMaxStages = 12;
+constexpr int kRaw = 6;                    // e4m3: tiles of codes in shared memory, all but one in flight
 
 struct alignas(16) Shared {
     uint64_t full[kMaxStages];       // stage holds a K or V tile
@@ -264,10 +265,13 @@ struct alignas(16) Shared {
 template <int DP, bool kFp8> struct Layout {
     static constexpr int kQTile = (DP / 64) * kQBlock;     // bytes of a Q tile
     static constexpr int kStage = (DP / 64) * kBlock;      // bytes of a K or V stage
-    static __host__ __device__ constexpr int stages(int qt) { return DP == 128 ? 13 - 2 * qt : 12; }
+    static constexpr int kRawTile = kFp8 ? kTile * DP : 0; // bytes of a tile of codes
+    static __host__ __device__ constexpr int stages(int qt) {
+        return kFp8 ? (DP == 128 ? 9 - 2 * qt : 8) : (DP == 128 ? 13 - 2 * qt : 12);
+    }
     static constexpr size_t info_bytes = sizeof(typename InfoOf<kFp8>::type) * kInfo;
     static constexpr size_t smem(int qt) {
-        return (size_t)qt * kQTile + (size_t)stages(qt) * kStage + sizeof(Shared) + info_bytes + (kFp8 ? 1024 : 0) + 1024;
+        return (size_t)qt * kQTile + (size_t)stages(qt) * kStage + kRaw * kRawTile + sizeof(Shared) + info_bytes + (kFp8 ? 1024 : 0) + 1024;
     }
 };
 static_assert(Layout<128, false>::smem(1) <= 232448 && Layout<128, false>::smem(2) <= 232448 &&
@@ -384,26 +388,19 @@ __device__ __forceinline__ void unpack2(uint32_t w, float& a, float& b, __half) 
     b = f.y;
 }
 
-// 16 bytes global -> shared, zeros where !ok (nothing is read then)
-__device__ __forceinline__ void cp16(uint32_t dst, const void* src, bool ok) {
-    asm volatile("cp.async.cg.shared.global.L2::128B [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(ok ? 16 : 0)
-                 : "memory");
+// 16 bytes global -> shared
+__device__ __forceinline__ void cp16(uint32_t dst, const void* src) {
+    asm volatile("cp.async.cg.shared.global.L2::128B [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
 }
 __device__ __forceinline__ void cp4(uint32_t dst, const void* src, bool ok) {
     asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src), "r"(ok ? 4 : 0) : "memory");
-}
-// 16 bytes that are read once: past L1, where they would push out what the warps spill there
-__device__ __forceinline__ uint4 ld16_once(const void* p) {
-    uint4 v;
-    asm("ld.global.nc.L1::no_allocate.L2::128B.v4.u32 {%0, %1, %2, %3}, [%4];"
-        : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
-        : "l"(p));
-    return v;
 }
 // arrives at `bar` once this thread's copies so far have landed
 __device__ __forceinline__ void cp_arrive(uint64_t* bar) {
     asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
 }
+__device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N> __device__ __forceinline__ void cp_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
 __device__ __forceinline__ void cp_wait_all() { asm volatile("cp.async.wait_all;" ::: "memory"); }
 
 // bounded wait that also gives up when another warp of the CTA has given up
@@ -473,15 +470,14 @@ __global__ void __launch_bounds__(threads<kFp8>(), 1) attn_kernel(const __grid_c
     using L = Layout<DP, kFp8>;
     using Info = typename InfoOf<kFp8>::type;
     using TO = typename std::conditional<kFp8, __half, TQ>::type;   // operands of the matrix instructions
-    constexpr int kThreads = threads<kFp8>();
-    constexpr int kProducers = producers<kFp8>();
-    constexpr int kElem = kFp8 ? 1 : 2;                    // bytes of a cached element
+    constexpr int kThreads = threads<kFp8>(), kLoaders = loaders<kFp8>();
     extern __shared__ uint8_t smem_raw[];
     const int qt = a.qt, stages = L::stages(qt);
     uint8_t* base = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
     uint8_t* sq = base;                                    // [qt][kQTile]
     uint8_t* ring = base + qt * L::kQTile;                 // [stages][kStage]
-    Shared* sh = reinterpret_cast<Shared*>(ring + stages * L::kStage);
+    uint8_t* raw = ring + stages * L::kStage;              // e4m3: [kRaw][kRawTile]
+    Shared* sh = reinterpret_cast<Shared*>(raw + (kFp8 ? kRaw * L::kRawTile : 0));
     Info* info = reinterpret_cast<Info*>(sh + 1);
     float* row_mul = reinterpret_cast<float*>(info + kInfo);        // e4m3: [128 qt] power of two of a row of q
     volatile int* abort = &sh->abort;
@@ -558,7 +554,7 @@ __global__ void __launch_bounds__(threads<kFp8>(), 1) attn_kernel(const __grid_c
 
     if (tid == 0) {
         for (int s = 0; s < stages; ++s) {
-            mbar_init(&sh->full[s], kFp8 ? 1 : 32);
+            mbar_init(&sh->full[s], kFp8 ? kLoaders : 32);
             mbar_init(&sh->empty[s], 1);
         }
         for (int i = 0; i < kInfo; ++i) {
@@ -591,89 +587,134 @@ __global__ void __launch_bounds__(threads<kFp8>(), 1) attn_kernel(const __grid_c
     constexpr uint32_t tmem = 0;                           // all 512 columns were allocated
     Walk w = sh->start;
 
-    if (warp >= kFirstProducer) {
-        // ---------------- producers: a warp takes whole items (a tile of K or of V), in turn -------
-        // One copy of this loop serves every item: unrolled over register buffers instead, its code
-        // pushed the other warps' out of the instruction cache (64x16 e4m3 458 us).
-        uint32_t item = warp - kFirstProducer;                  // of the CTA
-        int i = (int)item, base = 0, n = 0, ahead = 0;          // item of the segment, first tile, tiles, lead of K
-        bool ok = true;
+    if (warp >= kFirstLoader) {
+        // ---------------- loaders: rows of K and V by 16-byte copies of the lanes -----------------
+        // fp16, bf16: a warp takes whole items (a tile of K or of V) in turn, straight into the
+        // swizzled stage.  e4m3: each warp takes its 16 rows of every item, as codes into its own
+        // part of a raw ring (kRaw - 1 items in flight), and from there as fp16 into the stage.
+        // Copies of a lane, not TMA: one warp of them reaches 5.6 TB/s, two 6.7, whatever the page
+        // size; gathers of four rows and bulk copies of one stay at 2.2 and 1.3 (scattered rows of
+        // 256 bytes, nothing else running).
+        const int lw = warp - kFirstLoader;
+        constexpr int kElem = kFp8 ? 1 : 2;                     // bytes of a cached element
+        constexpr int kStride = kFp8 ? 1 : kLoaders;            // items from one of this warp's to the next
         const uint32_t stride = (uint32_t)t.c.slot_stride * (uint32_t)kElem;   // bytes from slot to slot
-        constexpr int kLanes = DP * kElem / 16;                 // lanes of a row (16 bytes each)
-        constexpr int kRowsAtOnce = 32 / kLanes, kSteps = kTile / kRowsAtOnce;
-        // lane's place in a row and among the rows of a step.  Where a row of codes becomes two blocks
-        // of fp16, four lanes of one row stand beside four of the next: their stores of eight then
-        // hit eight different groups of banks
+        constexpr int kLanes = DP * kElem / 16, kAtOnce = 32 / kLanes;         // lanes of a row, rows at once
+        constexpr int kSteps = (kFp8 ? kTile / kLoaders : kTile) / kAtOnce;
+        // e4m3: a row of codes becomes up to two blocks of fp16; four lanes of one row then stand beside
+        // four of the next, so that their stores of eight hit eight different groups of banks
         const int sub = kFp8 && DP == 128 ? (lane & 3) | ((lane >> 1) & 4) : lane % kLanes;
-        const int r0 = kFp8 && DP == 128 ? ((lane >> 2) & 1) | ((lane >> 3) & 2) : lane / kLanes;
+        const int dr = kFp8 && DP == 128 ? ((lane >> 2) & 1) | ((lane >> 3) & 2) : lane / kLanes;
+        // rows of step k: e4m3 kAtOnce adjacent ones; else dr's own run of kSteps
+        const int row0 = kFp8 ? lw * (kTile / kLoaders) + dr : dr * kSteps;
         const bool live = sub * (16 / kElem) < t.c.dim;
+        int i = kFp8 ? 0 : lw, base = 0, n = 0, ahead = 0;      // item of the segment, first tile, tiles, lead of K
+        bool ok = true, more = true;
+        long long head_at = 0;
         auto described = [&](int ti) {
             ok = __all_sync(0xffffffffu, wait_or_abort(&sh->info_full[ti % kInfo], (uint32_t)(ti / kInfo) & 1u, abort));
         };
-        long long head_at = 0;
-        for (;; item += kProducers, i += kProducers) {
-            while (ok && i >= 2 * n) {                          // on to the segment that holds the item
+        // the next item's source and slots; false past the last
+        const uint8_t* src = nullptr;
+        const int* slots = nullptr;
+        auto next = [&]() {
+            while (i >= 2 * n) {                                // on to the segment that holds the item
                 i -= 2 * n;
                 base += n;
                 n = 0;
-                if (base >= (int)count) break;
+                if (base >= (int)count) return false;
                 described(base);
-                if (!ok) break;
+                if (!ok) return false;
                 const Info* f = info + base % kInfo;
                 n = f->tiles;
                 ahead = min(f->ahead, n);
                 head_at = kElem * (f->head * t.c.head_stride) + sub * 16;
             }
-            if (!ok || n == 0) break;
             const int j = i - ahead, pairs = 2 * (n - ahead);
             const bool is_k = j < 0 || ((j & 1) && j < pairs);
             const int tl = base + (is_k ? (j < 0 ? i : ahead + (j >> 1)) : (j < pairs ? j >> 1 : j - (pairs >> 1)));
             described(tl);
-            if (!ok) break;
-            const int* slots = info[tl % kInfo].slot + r0;
-            const uint8_t* src = static_cast<const uint8_t*>(is_k ? t.c.k : t.c.v) + head_at;
-            const uint32_t s = item % stages, ph = (item / stages) & 1u;
-            if constexpr (!kFp8) {
-                ok = __all_sync(0xffffffffu, wait_or_abort(&sh->empty[s], ph ^ 1u, abort));
+            slots = info[tl % kInfo].slot + row0;
+            src = static_cast<const uint8_t*>(is_k ? t.c.k : t.c.v) + head_at;
+            i += kStride;
+            return ok;
+        };
+        if constexpr (!kFp8) {
+            uint32_t s = lw, ph = 1;                            // stage, and the parity that says it is free
+            while (next()) {
+                ok = __all_sync(0xffffffffu, wait_or_abort(&sh->empty[s], ph, abort));
                 if (!ok) break;
-                const uint32_t dst = smem_u32(ring + s * L::kStage);
-#pragma unroll 8
-                for (int k = 0; k < kSteps; ++k) {
-                    const int slot = live ? slots[k * kRowsAtOnce] : -1;
-                    cp16(dst + chunk_at<kBlock>(k * kRowsAtOnce + r0, sub), src + (uint64_t)(uint32_t)max(slot, 0) * stride,
-                         slot >= 0);
+                // chunk of row r: rows are 128 bytes apart, the chunk's place is xored with r & 7
+                const uint32_t dst = smem_u32(ring + s * L::kStage) + (sub >> 3) * kBlock + row0 * 128 + ((sub & 7) << 4);
+                if (live) {
+#pragma unroll
+                    for (int k = 0; k < kSteps; k += 4) {
+                        const int4 four = *reinterpret_cast<const int4*>(slots + k);
+                        cp16((dst ^ ((k & 7) << 4)) + k * 128, src + (uint64_t)(uint32_t)four.x * stride);
+                        cp16((dst ^ (((k + 1) & 7) << 4)) + (k + 1) * 128, src + (uint64_t)(uint32_t)four.y * stride);
+                        cp16((dst ^ (((k + 2) & 7) << 4)) + (k + 2) * 128, src + (uint64_t)(uint32_t)four.z * stride);
+                        cp16((dst ^ (((k + 3) & 7) << 4)) + (k + 3) * 128, src + (uint64_t)(uint32_t)four.w * stride);
+                    }
                 }
                 cp_arrive(&sh->full[s]);
-            } else {
-                // codes in registers, then as fp16 into the stage
-                uint4 x[kSteps];
-#pragma unroll
-                for (int k = 0; k < kSteps; ++k) {
-                    const int slot = live ? slots[k * kRowsAtOnce] : -1;
-                    x[k] = make_uint4(0, 0, 0, 0);
-                    if (slot >= 0) x[k] = ld16_once(src + (uint64_t)(uint32_t)slot * stride);
+                s += kLoaders;
+                if (s >= (uint32_t)stages) {
+                    s -= stages;
+                    ph ^= 1u;
                 }
-                ok = __all_sync(0xffffffffu, wait_or_abort(&sh->empty[s], ph ^ 1u, abort));
+            }
+        } else {
+            constexpr int kPart = L::kRawTile / kLoaders;       // this warp's rows of a raw tile
+            uint8_t* mine_raw = raw + lw * kPart + dr * DP + sub * 16;
+            auto load = [&](uint32_t r) {
+                more = more && next();
+                if (more && live) {
+                    const uint32_t dst = smem_u32(mine_raw + r * L::kRawTile);
+#pragma unroll
+                    for (int k = 0; k < kSteps; ++k)
+                        cp16(dst + k * kAtOnce * DP, src + (uint64_t)(uint32_t)slots[k * kAtOnce] * stride);
+                }
+                cp_commit();
+            };
+            const long long items = 2 * count;
+            uint32_t s = 0, ph = 1, r = 0, ahead_r = 0;
+#pragma unroll 1
+            for (long long item = 1 - kRaw; item < items; ++item) {
+                load(ahead_r);                                  // item + kRaw - 1
+                if (++ahead_r == (uint32_t)kRaw) ahead_r = 0;
                 if (!ok) break;
+                if (item < 0) continue;
+                cp_wait<kRaw - 1>();                            // this item's codes have landed
+                ok = __all_sync(0xffffffffu, wait_or_abort(&sh->empty[s], ph, abort));
+                if (!ok) break;
+                const uint8_t* from = mine_raw + r * L::kRawTile;
                 uint8_t* dst = ring + s * L::kStage;
+                if (live) {
 #pragma unroll
-                for (int k = 0; k < kSteps; ++k) {
-                    const int row = k * kRowsAtOnce + r0;
-                    const uint32_t c4[4] = {x[k].x, x[k].y, x[k].z, x[k].w};
-                    uint32_t o[8];
+                    for (int k = 0; k < kSteps; ++k) {
+                        const int row = row0 + k * kAtOnce;
+                        const uint4 x = *reinterpret_cast<const uint4*>(from + k * kAtOnce * DP);
+                        const uint32_t c4[4] = {x.x, x.y, x.z, x.w};
+                        uint32_t o[8];
 #pragma unroll
-                    for (int q = 0; q < 8; ++q) {
-                        const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2((uint16_t)(c4[q >> 1] >> (16 * (q & 1))), __NV_E4M3);
-                        o[q] = (uint32_t)h.x | ((uint32_t)h.y << 16);
+                        for (int q = 0; q < 8; ++q) {
+                            const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2((uint16_t)(c4[q >> 1] >> (16 * (q & 1))), __NV_E4M3);
+                            o[q] = (uint32_t)h.x | ((uint32_t)h.y << 16);
+                        }
+                        *reinterpret_cast<uint4*>(dst + chunk_at<kBlock>(row, 2 * sub)) = make_uint4(o[0], o[1], o[2], o[3]);
+                        *reinterpret_cast<uint4*>(dst + chunk_at<kBlock>(row, 2 * sub + 1)) = make_uint4(o[4], o[5], o[6], o[7]);
                     }
-                    *reinterpret_cast<uint4*>(dst + chunk_at<kBlock>(row, 2 * sub)) = make_uint4(o[0], o[1], o[2], o[3]);
-                    *reinterpret_cast<uint4*>(dst + chunk_at<kBlock>(row, 2 * sub + 1)) = make_uint4(o[4], o[5], o[6], o[7]);
                 }
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&sh->full[s]);
+                if (++s == (uint32_t)stages) {
+                    s = 0;
+                    ph ^= 1u;
+                }
+                if (++r == (uint32_t)kRaw) r = 0;
             }
         }
-        if constexpr (!kFp8) cp_wait_all();
+        cp_wait_all();
     } else if (warp == kIndexWarp) {
         // ---------------- index: slots, scales and validity of the tiles to come ----------------
         int ti = 0;
@@ -719,7 +760,7 @@ __global__ void __launch_bounds__(threads<kFp8>(), 1) attn_kernel(const __grid_c
                             else if (t.err)
                                 atomicOr(t.err, 2u);
                         }
-                        f->slot[e * 32 + lane] = slot;
+                        f->slot[e * 32 + lane] = max(slot, 0);
                         valid[e] = __ballot_sync(0xffffffffu, slot >= 0);
                         if constexpr (kFp8) {
                             const long long from = max(slot, 0) * t.c.scale_stride + w.h;
@@ -937,29 +978,34 @@ __global__ void __launch_bounds__(threads<kFp8>(), 1) attn_kernel(const __grid_c
                 tc_fence_after();
                 const int kb = (w.k0 + tl) * kTile;             // first position of the tile
                 const bool drafted = kb + kTile > w.r.p0;
-                if (drafted) {
-                    // V elements of drafted tokens that are not finite: zeroed for the matrix
-                    // instructions, added to the rows that see them at the end
+                const uint2 valid = *reinterpret_cast<const uint2*>(inf->valid);
+                const bool masked = drafted || (valid.x & valid.y) != ~0u;
+                if (masked) {
+                    // V rows of positions that do not exist are zeroed (another slot's row was loaded);
+                    // elements of drafted tokens that are not finite too, and added to the rows that
+                    // see them at the end
                     const uint32_t it = item + item_of_v(tl, nt, ahead), st = it % stages;
                     ok = __all_sync(0xffffffffu, wait_or_abort(&sh->full[st], (it / stages) & 1u, abort));
                     if (!ok) break;
                     const int key = row & (kTile - 1);          // two threads a key
-                    if (kb + key >= w.r.p0 && kb + key < w.r.len) {
+                    const bool gone = !(((key & 32 ? valid.y : valid.x) >> (key & 31)) & 1u);
+                    if (gone || kb + key >= w.r.p0) {
                         uint8_t* v = ring + st * L::kStage;
                         constexpr uint32_t kExp = std::is_same<TO, __nv_bfloat16>::value ? 0x7F80u : 0x7C00u;
                         bool found = false;
+#pragma unroll 1
                         for (int c = row / kTile; c < t.c.dim / 8; c += 2) {
                             uint4* at = reinterpret_cast<uint4*>(v + chunk_at<kBlock>(key, c));
                             const uint4 x = *at;
                             uint32_t xw[4] = {x.x, x.y, x.z, x.w};
-                            bool here = false;
+                            bool here = gone;
 #pragma unroll
                             for (int i = 0; i < 4; ++i) {
-                                if ((xw[i] & kExp) == kExp) {
+                                if (gone || (xw[i] & kExp) == kExp) {
                                     xw[i] &= 0xFFFF0000u;
                                     here = true;
                                 }
-                                if ((xw[i] & (kExp << 16)) == (kExp << 16)) {
+                                if (gone || (xw[i] & (kExp << 16)) == (kExp << 16)) {
                                     xw[i] &= 0xFFFFu;
                                     here = true;
                                 }
@@ -967,7 +1013,7 @@ __global__ void __launch_bounds__(threads<kFp8>(), 1) attn_kernel(const __grid_c
                             if (here) *at = make_uint4(xw[0], xw[1], xw[2], xw[3]);
                             found |= here;
                         }
-                        if (found) *(volatile int*)&sh->odd[seg & 1] = 1;
+                        if (found && !gone) *(volatile int*)&sh->odd[seg & 1] = 1;
                     }
                 }
                 if (any_row) {
@@ -975,8 +1021,6 @@ __global__ void __launch_bounds__(threads<kFp8>(), 1) attn_kernel(const __grid_c
                     uint32_t v[2][32];
                     tmem_ld32(ts, v[0]);
                     tmem_ld32(ts + 32, v[1]);
-                    const uint2 valid = *reinterpret_cast<const uint2*>(inf->valid);
-                    const bool masked = drafted || (valid.x & valid.y) != ~0u;
                     uint32_t vis[2] = {~0u, ~0u};
                     if constexpr (kFp8) {
                         // the largest V scale; a token whose V scale is not finite gets a K scale of NaN (the

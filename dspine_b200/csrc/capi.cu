@@ -51,7 +51,7 @@ int check_cache(const dsv_kv_cache* c, int max_dim, dsv::KvCache* out) {
     if (c == nullptr) return DSV_BAD_POINTER;
     if (c->dtype != DSV_BF16 && c->dtype != DSV_F16 && c->dtype != DSV_E4M3) return DSV_BAD_DTYPE;
     if (c->slots < 1 || c->slots > 0x7fffffff || c->heads < 1 || c->dim < 16 || c->dim > max_dim ||
-        c->dim % 16 != 0 || c->head_stride < c->dim || c->slot_stride < c->dim ||
+        c->dim % 16 != 0 || c->head_stride < c->dim || c->slot_stride < c->dim || c->head_stride > ((int64_t)1 << 40) ||
         (c->dtype == DSV_E4M3 && c->scale_stride < c->heads) || c->slot_stride > 0x3fffffff)
         return DSV_BAD_SHAPE;
     const bool codes = c->dtype == DSV_E4M3;

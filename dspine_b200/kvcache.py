@@ -77,10 +77,10 @@ def describe(k_cache, v_cache, k_scale, v_scale):
         _check(one == 1, "k_cache and v_cache must have the same strides and contiguous rows")
         _check(False, "the cache has no slots")
     # a dimension of one element may carry any stride: it is never stepped over
-    if slots == 1:
-        slot_stride = heads * dim
     if heads == 1:
         head_stride = dim
+    if slots == 1:
+        slot_stride = heads * head_stride
     if slot_stride < dim or slot_stride % step or head_stride < dim or head_stride % step:
         _check(False, "the cache's rows must be 16-byte aligned and not overlap")
     if dtype != 3:
