@@ -74,10 +74,8 @@ constexpr float kSlack = 8.0f;             // log2 by which a maximum may outgro
 constexpr float kL2E = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
 
-// warps 0-7 softmax, 8 and 9 MMA issuers (scores, accumulation), 10 index, 11.. loaders
-constexpr int kScoreWarp = 8, kAccumWarp = 9, kIndexWarp = 10, kFirstLoader = 11;
-template <bool kFp8> constexpr int loaders() { return kFp8 ? 4 : 2; }
-template <bool kFp8> constexpr int threads() { return 32 * (kFirstLoader + loaders<kFp8>()); }
+// warps 0-7 softmax, 8 and 9 MMA issuers (scores, accumulation), 10 index, 11 idle, 12-15 loaders
+constexpr int kScoreWarp = 8, kAccumWarp = 9, kIndexWarp = 10, kFirstLoader = 12, kLoaders = 4, kThreads = 512;
 
 // a tile of keys, as the index warp describes it to the others
 struct alignas(16) TileInfoPlain {
@@ -216,22 +214,38 @@ struct Walk {
         k1 = (long long)(tiles - k0) < left ? tiles : k0 + (int)left;
         left -= k1 - k0;
     }
-    // the next segment; false at the end of the CTA's piece
-    __device__ __forceinline__ bool advance(const KernelArgs& a) {
+    // the next segment; false at the end of the CTA's piece.  By a whole warp, whose lanes all see
+    // (and write) the same
+    __device__ __noinline__ bool advance(const KernelArgs& a) {
+        __syncwarp();
         if (left <= 0) return false;
-        if (++block >= r.blocks) {
-            block = 0;
-            if (++h >= a.t.c.heads) {
-                h = 0;
+        int b_ = b, h_ = h, block_ = block + 1;
+        Request r_ = r;
+        if (block_ >= r_.blocks) {
+            block_ = 0;
+            if (++h_ >= a.t.c.heads) {
+                h_ = 0;
                 do {
-                    ++b;
-                    r = request_of(a.t, a.qt, b);
-                } while (r.rows == 0);
+                    ++b_;
+                    r_ = request_of(a.t, a.qt, b_);
+                } while (r_.rows == 0);
             }
         }
-        tiles = tiles_of(a.t, a.qt, r, block);
-        k0 = 0;
-        take();
+        const int tiles_ = tiles_of(a.t, a.qt, r_, block_);
+        const int take_ = tiles_ < left ? tiles_ : (int)left;
+        const long long left_ = left - take_;
+        __syncwarp();
+        if ((threadIdx.x & 31) == 0) {
+            b = b_;
+            h = h_;
+            block = block_;
+            r = r_;
+            tiles = tiles_;
+            k0 = 0;
+            k1 = take_;
+            left = left_;
+        }
+        __syncwarp();
         return true;
     }
     __device__ __forceinline__ int count() const { return k1 - k0; }
@@ -260,6 +274,7 @@ struct alignas(16) Shared {
     int odd[2];                      // a drafted V element was not finite (by segment parity)
     long long scan[32];
     Walk start;                      // where this CTA starts on the line of tiles
+    Walk walk[kThreads / 32];        // where each warp is: here, not in registers, which the scores fill
 };
 
 template <int DP, bool kFp8> struct Layout {
@@ -466,11 +481,10 @@ __device__ __forceinline__ int item_of_v(int t, int n, int ahead) {
 // ---- the kernel ---------------------------------------------------------------------------------
 
 template <typename TQ, bool kFp8, int DP>
-__global__ void __launch_bounds__(threads<kFp8>(), 1) attn_kernel(const __grid_constant__ KernelArgs a) {
+__global__ void __launch_bounds__(kThreads, 1) attn_kernel(const __grid_constant__ KernelArgs a) {
     using L = Layout<DP, kFp8>;
     using Info = typename InfoOf<kFp8>::type;
     using TO = typename std::conditional<kFp8, __half, TQ>::type;   // operands of the matrix instructions
-    constexpr int kThreads = threads<kFp8>(), kLoaders = loaders<kFp8>();
     extern __shared__ uint8_t smem_raw[];
     const int qt = a.qt, stages = L::stages(qt);
     uint8_t* base = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
@@ -585,8 +599,9 @@ __global__ void __launch_bounds__(threads<kFp8>(), 1) attn_kernel(const __grid_c
     __syncthreads();
     tc_fence_after();
     constexpr uint32_t tmem = 0;                           // all 512 columns were allocated
-    Walk w = sh->start;
-
+    Walk& w = sh->walk[warp];
+    if (lane == 0) w = sh->start;
+    __syncwarp();
     if (warp >= kFirstLoader) {
         // ---------------- loaders: rows of K and V by 16-byte copies of the lanes -----------------
         // fp16, bf16: a warp takes whole items (a tile of K or of V) in turn, straight into the
@@ -597,7 +612,6 @@ __global__ void __launch_bounds__(threads<kFp8>(), 1) attn_kernel(const __grid_c
         // 256 bytes, nothing else running).
         const int lw = warp - kFirstLoader;
         constexpr int kElem = kFp8 ? 1 : 2;                     // bytes of a cached element
-        constexpr int kStride = kFp8 ? 1 : kLoaders;            // items from one of this warp's to the next
         const uint32_t stride = (uint32_t)t.c.slot_stride * (uint32_t)kElem;   // bytes from slot to slot
         constexpr int kLanes = DP * kElem / 16, kAtOnce = 32 / kLanes;         // lanes of a row, rows at once
         constexpr int kSteps = (kFp8 ? kTile / kLoaders : kTile) / kAtOnce;
@@ -608,46 +622,56 @@ __global__ void __launch_bounds__(threads<kFp8>(), 1) attn_kernel(const __grid_c
         // rows of step k: e4m3 kAtOnce adjacent ones; else dr's own run of kSteps
         const int row0 = kFp8 ? lw * (kTile / kLoaders) + dr : dr * kSteps;
         const bool live = sub * (16 / kElem) < t.c.dim;
-        int i = kFp8 ? 0 : lw, base = 0, n = 0, ahead = 0;      // item of the segment, first tile, tiles, lead of K
-        bool ok = true, more = true;
+        const uint32_t bars = smem_u32(sh), empty = bars + offsetof(Shared, empty), described = bars + offsetof(Shared, info_full);
+        // items in order: per segment its first K tiles (lead of them), then V and K in turn
+        int kt = 0, vt = 0, k_left = 0, v_left = 0, lead = 0;   // next tiles of the CTA, left in the segment
+        bool ok = true, more = true, k_turn = false;
         long long head_at = 0;
-        auto described = [&](int ti) {
-            ok = __all_sync(0xffffffffu, wait_or_abort(&sh->info_full[ti % kInfo], (uint32_t)(ti / kInfo) & 1u, abort));
-        };
-        // the next item's source and slots; false past the last
         const uint8_t* src = nullptr;
         const int* slots = nullptr;
-        auto next = [&]() {
-            while (i >= 2 * n) {                                // on to the segment that holds the item
-                i -= 2 * n;
-                base += n;
-                n = 0;
-                if (base >= (int)count) return false;
-                described(base);
+        auto wait_described = [&](int tl) { return wait_at(described + 8 * (tl % kInfo), (uint32_t)(tl / kInfo) & 1u, abort); };
+        auto next = [&](bool mine) {                            // false past the last, or after a wait that gave up
+            if (v_left == 0) {
+                if (kt >= (int)count) return false;
+                ok = wait_described(kt);
                 if (!ok) return false;
-                const Info* f = info + base % kInfo;
-                n = f->tiles;
-                ahead = min(f->ahead, n);
+                const Info* f = info + kt % kInfo;
+                k_left = v_left = f->tiles;
+                lead = min(f->ahead, k_left);
                 head_at = kElem * (f->head * t.c.head_stride) + sub * 16;
             }
-            const int j = i - ahead, pairs = 2 * (n - ahead);
-            const bool is_k = j < 0 || ((j & 1) && j < pairs);
-            const int tl = base + (is_k ? (j < 0 ? i : ahead + (j >> 1)) : (j < pairs ? j >> 1 : j - (pairs >> 1)));
-            described(tl);
-            slots = info[tl % kInfo].slot + row0;
-            src = static_cast<const uint8_t*>(is_k ? t.c.k : t.c.v) + head_at;
-            i += kStride;
+            const bool is_k = lead > 0 || (k_turn && k_left > 0);
+            int tl;
+            if (is_k) {
+                tl = kt++;
+                --k_left;
+                lead = max(lead - 1, 0);
+                k_turn = false;
+            } else {
+                tl = vt++;
+                --v_left;
+                k_turn = true;
+            }
+            if (mine) {
+                // a warp that sees every item has waited for a V tile's description with its K tile
+                if (is_k || !kFp8) ok = wait_described(tl);
+                slots = info[tl % kInfo].slot + row0;
+                src = static_cast<const uint8_t*>(is_k ? t.c.k : t.c.v) + head_at;
+            }
             return ok;
         };
         if constexpr (!kFp8) {
             uint32_t s = lw, ph = 1;                            // stage, and the parity that says it is free
-            while (next()) {
-                ok = __all_sync(0xffffffffu, wait_or_abort(&sh->empty[s], ph, abort));
+            for (int item = 0;; ++item) {
+                const bool mine = item % kLoaders == lw;
+                if (!next(mine)) break;
+                if (!mine) continue;
+                ok = wait_at(empty + 8 * s, ph, abort);
                 if (!ok) break;
                 // chunk of row r: rows are 128 bytes apart, the chunk's place is xored with r & 7
                 const uint32_t dst = smem_u32(ring + s * L::kStage) + (sub >> 3) * kBlock + row0 * 128 + ((sub & 7) << 4);
                 if (live) {
-#pragma unroll
+#pragma unroll 2
                     for (int k = 0; k < kSteps; k += 4) {
                         const int4 four = *reinterpret_cast<const int4*>(slots + k);
                         cp16((dst ^ ((k & 7) << 4)) + k * 128, src + (uint64_t)(uint32_t)four.x * stride);
@@ -667,7 +691,7 @@ __global__ void __launch_bounds__(threads<kFp8>(), 1) attn_kernel(const __grid_c
             constexpr int kPart = L::kRawTile / kLoaders;       // this warp's rows of a raw tile
             uint8_t* mine_raw = raw + lw * kPart + dr * DP + sub * 16;
             auto load = [&](uint32_t r) {
-                more = more && next();
+                more = more && next(true);
                 if (more && live) {
                     const uint32_t dst = smem_u32(mine_raw + r * L::kRawTile);
 #pragma unroll
@@ -685,7 +709,7 @@ __global__ void __launch_bounds__(threads<kFp8>(), 1) attn_kernel(const __grid_c
                 if (!ok) break;
                 if (item < 0) continue;
                 cp_wait<kRaw - 1>();                            // this item's codes have landed
-                ok = __all_sync(0xffffffffu, wait_or_abort(&sh->empty[s], ph, abort));
+                ok = wait_at(empty + 8 * s, ph, abort);
                 if (!ok) break;
                 const uint8_t* from = mine_raw + r * L::kRawTile;
                 uint8_t* dst = ring + s * L::kStage;
@@ -873,7 +897,7 @@ __global__ void __launch_bounds__(threads<kFp8>(), 1) attn_kernel(const __grid_c
         mma_commit(smem_u32(drain));
         if (!mbar_wait_bounded(drain, 0)) *abort = 1;
         __syncwarp();
-    } else {
+    } else if (warp < 8) {
         // ---------------- softmax and epilogue: one row per thread ----------------
         const int s = warp >> 2, quarter = warp & 3, row = quarter * 32 + lane;
         const uint32_t lanes = (uint32_t)(quarter * 32) << 16;
@@ -970,9 +994,8 @@ __global__ void __launch_bounds__(threads<kFp8>(), 1) attn_kernel(const __grid_c
             for (int tl = both ? 0 : s; ok && tl < nt; tl += step, b ^= 1) {
                 const uint32_t ti = tile0 + tl, ts = tmem + lanes + s * 128 + b * kTile;
                 const Info* inf = info + ti % kInfo;
-                ok = wait_or_abort(&sh->info_full[ti % kInfo], (ti / kInfo) & 1u, abort) &&
-                     wait_or_abort(&sh->s_full[s][b], (ph >> b) & 1u, abort);
-                ok = __all_sync(0xffffffffu, ok);
+                ok = wait_at(smem_u32(&sh->info_full[ti % kInfo]), (ti / kInfo) & 1u, abort) &&
+                     wait_at(smem_u32(&sh->s_full[s][b]), (ph >> b) & 1u, abort);
                 if (!ok) break;
                 ph ^= 1u << b;
                 tc_fence_after();
@@ -1341,7 +1364,7 @@ int launch(const KernelArgs& a, int sms, cudaStream_t st) {
     if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess)
         return kLaunchFailed;
     const int grid = sms < kMaxCtas ? sms : kMaxCtas;
-    kern<<<grid, threads<kFp8>(), smem, st>>>(a);
+    kern<<<grid, kThreads, smem, st>>>(a);
     if (cudaGetLastError() != cudaSuccess) return kLaunchFailed;
     // items of one tile are never cut
     if ((long long)a.t.max_pages * a.t.page_size <= kTile) return kOk;
