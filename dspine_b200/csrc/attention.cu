@@ -671,13 +671,18 @@ __global__ void __launch_bounds__(kThreads, 1) attn_kernel(const __grid_constant
                 // chunk of row r: rows are 128 bytes apart, the chunk's place is xored with r & 7
                 const uint32_t dst = smem_u32(ring + s * L::kStage) + (sub >> 3) * kBlock + row0 * 128 + ((sub & 7) << 4);
                 if (live) {
+                    // slots four at a time, and the next four before the copies of these are issued
+                    // (loads do not move past the copies by themselves)
+                    int4 four = *reinterpret_cast<const int4*>(slots);
 #pragma unroll 2
                     for (int k = 0; k < kSteps; k += 4) {
-                        const int4 four = *reinterpret_cast<const int4*>(slots + k);
-                        cp16((dst ^ ((k & 7) << 4)) + k * 128, src + (uint64_t)(uint32_t)four.x * stride);
-                        cp16((dst ^ (((k + 1) & 7) << 4)) + (k + 1) * 128, src + (uint64_t)(uint32_t)four.y * stride);
-                        cp16((dst ^ (((k + 2) & 7) << 4)) + (k + 2) * 128, src + (uint64_t)(uint32_t)four.z * stride);
-                        cp16((dst ^ (((k + 3) & 7) << 4)) + (k + 3) * 128, src + (uint64_t)(uint32_t)four.w * stride);
+                        const int4 now = four;
+                        four = *reinterpret_cast<const int4*>(slots + (k + 4 < kSteps ? k + 4 : 0));
+                        const uint32_t at = dst ^ ((k & 4) << 4), to = k * 128;
+                        cp16(at + to, src + (uint64_t)(uint32_t)now.x * stride);
+                        cp16((at ^ 16) + to + 128, src + (uint64_t)(uint32_t)now.y * stride);
+                        cp16((at ^ 32) + to + 256, src + (uint64_t)(uint32_t)now.z * stride);
+                        cp16((at ^ 48) + to + 384, src + (uint64_t)(uint32_t)now.w * stride);
                     }
                 }
                 cp_arrive(&sh->full[s]);
@@ -694,9 +699,11 @@ __global__ void __launch_bounds__(kThreads, 1) attn_kernel(const __grid_constant
                 more = more && next(true);
                 if (more && live) {
                     const uint32_t dst = smem_u32(mine_raw + r * L::kRawTile);
+                    int slot[kSteps];
 #pragma unroll
-                    for (int k = 0; k < kSteps; ++k)
-                        cp16(dst + k * kAtOnce * DP, src + (uint64_t)(uint32_t)slots[k * kAtOnce] * stride);
+                    for (int k = 0; k < kSteps; ++k) slot[k] = slots[k * kAtOnce];
+#pragma unroll
+                    for (int k = 0; k < kSteps; ++k) cp16(dst + k * kAtOnce * DP, src + (uint64_t)(uint32_t)slot[k] * stride);
                 }
                 cp_commit();
             };
@@ -714,11 +721,13 @@ __global__ void __launch_bounds__(kThreads, 1) attn_kernel(const __grid_constant
                 const uint8_t* from = mine_raw + r * L::kRawTile;
                 uint8_t* dst = ring + s * L::kStage;
                 if (live) {
+                    uint4 x[kSteps];                            // all loads before the first store
+#pragma unroll
+                    for (int k = 0; k < kSteps; ++k) x[k] = *reinterpret_cast<const uint4*>(from + k * kAtOnce * DP);
 #pragma unroll
                     for (int k = 0; k < kSteps; ++k) {
                         const int row = row0 + k * kAtOnce;
-                        const uint4 x = *reinterpret_cast<const uint4*>(from + k * kAtOnce * DP);
-                        const uint32_t c4[4] = {x.x, x.y, x.z, x.w};
+                        const uint32_t c4[4] = {x[k].x, x[k].y, x[k].z, x[k].w};
                         uint32_t o[8];
 #pragma unroll
                         for (int q = 0; q < 8; ++q) {
@@ -841,27 +850,35 @@ __global__ void __launch_bounds__(kThreads, 1) attn_kernel(const __grid_constant
                 const uint32_t q0 = desc_low(smem_u32(sq), 16), k0 = desc_low(smem_u32(ring), 16);
                 ok = wait_at(bars + offsetof(Shared, q_full), seg & 1u, abort);
                 int left = ahead;                            // K tiles before the first V tile
-                for (int u = 0; ok && u < units; ++u) {
+                auto ready = [&](int u) {                    // K tile and score buffer of unit u
                     const uint32_t s = u & 1, sb = (s << 1) | ((u >> 1) & 1);
                     if (!(s & step)) ok = wait_at(full + 8 * st, sp, abort);
                     ok = ok && wait_at(s_free + 8 * sb, ((ph >> sb) & 1u) ^ 1u, abort);
-                    if (!ok) break;
                     ph ^= 1u << sb;
                     fence_proxy_async_smem();
                     tc_fence_after();
+                };
+                if (ok) ready(0);
+                for (int u = 0; ok && u < units; ++u) {
+                    const uint32_t s = u & 1, sb = (s << 1) | ((u >> 1) & 1), mine = st;
                     const uint32_t qa = q0 + (s & step) * (L::kQTile >> 4), kb = k0 + st * (L::kStage >> 4), d = tmem + sb * kTile;
-#pragma unroll
-                    for (int k = 0; k < DP / 16; ++k) {
+                    const bool last = (s & step) == step;    // the last use of the tile
+                    auto issue = [&](int k) {
                         const uint32_t col = (k & 3) * 2;
                         if (k < ksteps)
-                            mma_ss(d, desc(qa + (k >> 2) * (kQBlock >> 4) + col), desc(kb + (k >> 2) * (kBlock >> 4) + col),
-                                   kIdescS, k != 0);
-                    }
+                            mma_ss(d, desc(qa + (k >> 2) * (kQBlock >> 4) + col), desc(kb + (k >> 2) * (kBlock >> 4) + col), kIdescS,
+                                   k != 0);
+                    };
+#pragma unroll
+                    for (int k = 0; k < DP / 32; ++k) issue(k);
+                    // the next unit's waits while these execute
+                    if (last) skip(u == units - 1 ? ahead + 1 : (--left > 0 ? 1 : 2));
+                    if (u + 1 < units) ready(u + 1);
+                    if (!ok) break;
+#pragma unroll
+                    for (int k = DP / 32; k < DP / 16; ++k) issue(k);
                     mma_commit(s_full + 8 * sb);
-                    if ((s & step) == step) {                // the last use of the tile
-                        mma_commit(empty + 8 * st);
-                        skip(u == units - 1 ? ahead + 1 : (--left > 0 ? 1 : 2));
-                    }
+                    if (last) mma_commit(empty + 8 * mine);
                 }
             } else {
                 const uint32_t v0 = desc_low(smem_u32(ring), kBlock);
