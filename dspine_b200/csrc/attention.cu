@@ -19,6 +19,7 @@
 //                                  scores of a tile in registers
 //                     warps 8, 9   MMA issuers: scores (and TMEM allocation), accumulation
 //                     warp 10      index: slots, scales and validity of the tiles to come
+//                     warp 11      queries: the next segment's rows of q, while this one runs
 //                     warps 11..   loaders: K and V rows of a tile, slot by slot, into a ring of
 //                                  128-byte-swizzled shared-memory stages (e4m3: converted on the way)
 //                   S = Q K^T (kind::f16, both operands in shared memory) and O += P V (P from
@@ -74,8 +75,8 @@ constexpr float kSlack = 8.0f;             // log2 by which a maximum may outgro
 constexpr float kL2E = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
 
-// warps 0-7 softmax, 8 and 9 MMA issuers (scores, accumulation), 10 index, 11 idle, 12-15 loaders
-constexpr int kScoreWarp = 8, kAccumWarp = 9, kIndexWarp = 10, kFirstLoader = 12, kLoaders = 4, kThreads = 512;
+// warps 0-7 softmax, 8 and 9 MMA issuers (scores, accumulation), 10 index, 11 queries, 12-15 loaders
+constexpr int kScoreWarp = 8, kAccumWarp = 9, kIndexWarp = 10, kQueryWarp = 11, kFirstLoader = 12, kLoaders = 4, kThreads = 512;
 
 // a tile of keys, as the index warp describes it to the others
 struct alignas(16) TileInfoPlain {
@@ -114,7 +115,7 @@ struct Divisor {
 
 struct KernelArgs {
     TreeAttnArgs t;
-    Divisor page;           // by page_size
+    Divisor page, group;    // by page_size, by t.group
     int pages;              // of the cache
     int qt;                 // Q tiles of a row block
     Split* splits;          // [kMaxCtas]
@@ -262,7 +263,8 @@ struct alignas(16) Shared {
     uint64_t empty[kMaxStages];      // the matrix instructions that read it are done
     uint64_t info_full[kInfo];       // tile described
     uint64_t info_empty[kInfo];      // its last matrix instructions are done
-    uint64_t q_full;                 // Q of the segment in shared memory, last segment's TMEM read
+    uint64_t q_full[2];              // a segment and its Q in shared memory
+    uint64_t q_free[2];              // the segment is done with
     uint64_t s_full[2][2];           // scores of a stream's buffer in TMEM
     uint64_t p_full[2][2];           // weights of a stream's buffer in TMEM
     uint64_t s_free[2][2];           // the weights in a stream's buffer have been accumulated
@@ -274,24 +276,24 @@ struct alignas(16) Shared {
     int odd[2];                      // a drafted V element was not finite (by segment parity)
     long long scan[32];
     Walk start;                      // where this CTA starts on the line of tiles
-    Walk walk[kThreads / 32];        // where each warp is: here, not in registers, which the scores fill
+    Walk seg[2];                     // the segments whose Q is here; read in place, registers are full
+    Walk walk[2];                    // where the index and the query warp are
 };
 
 template <int DP, bool kFp8> struct Layout {
     static constexpr int kQTile = (DP / 64) * kQBlock;     // bytes of a Q tile
     static constexpr int kStage = (DP / 64) * kBlock;      // bytes of a K or V stage
     static constexpr int kRawTile = kFp8 ? kTile * DP : 0; // bytes of a tile of codes
-    static __host__ __device__ constexpr int stages(int qt) {
-        return kFp8 ? (DP == 128 ? 9 - 2 * qt : 8) : (DP == 128 ? 13 - 2 * qt : 12);
+    static __host__ __device__ constexpr int stages() {
+        return kFp8 ? (DP == 128 ? 5 : 8) : (DP == 128 ? 9 : 12);
     }
     static constexpr size_t info_bytes = sizeof(typename InfoOf<kFp8>::type) * kInfo;
-    static constexpr size_t smem(int qt) {
-        return (size_t)qt * kQTile + (size_t)stages(qt) * kStage + kRaw * kRawTile + sizeof(Shared) + info_bytes + (kFp8 ? 1024 : 0) + 1024;
+    static constexpr size_t smem() {
+        return (size_t)2 * kQTile + (size_t)stages() * kStage + kRaw * kRawTile + sizeof(Shared) + info_bytes + (kFp8 ? 1024 : 0) + 1024;
     }
 };
-static_assert(Layout<128, false>::smem(1) <= 232448 && Layout<128, false>::smem(2) <= 232448 &&
-                  Layout<128, true>::smem(1) <= 232448 && Layout<128, true>::smem(2) <= 232448 &&
-                  Layout<64, false>::smem(2) <= 232448 && Layout<64, true>::smem(2) <= 232448,
+static_assert(Layout<128, false>::smem() <= 232448 && Layout<128, true>::smem() <= 232448 && Layout<64, false>::smem() <= 232448 &&
+                  Layout<64, true>::smem() <= 232448,
               "shared memory of one CTA");
 
 // ---- PTX helpers ------------------------------------------------------------------------------
@@ -403,6 +405,9 @@ __device__ __forceinline__ void unpack2(uint32_t w, float& a, float& b, __half) 
     b = f.y;
 }
 
+__device__ __forceinline__ void cp16_or_zero(uint32_t dst, const void* src, bool ok) {   // nothing is read where !ok
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(ok ? 16 : 0) : "memory");
+}
 // 16 bytes global -> shared
 __device__ __forceinline__ void cp16(uint32_t dst, const void* src) {
     asm volatile("cp.async.cg.shared.global.L2::128B [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
@@ -486,10 +491,11 @@ __global__ void __launch_bounds__(kThreads, 1) attn_kernel(const __grid_constant
     using Info = typename InfoOf<kFp8>::type;
     using TO = typename std::conditional<kFp8, __half, TQ>::type;   // operands of the matrix instructions
     extern __shared__ uint8_t smem_raw[];
-    const int qt = a.qt, stages = L::stages(qt);
+    constexpr int stages = L::stages();
+    const int qt = a.qt, q_bufs = qt == 1 ? 2 : 1;         // segments whose Q is held at once
     uint8_t* base = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
-    uint8_t* sq = base;                                    // [qt][kQTile]
-    uint8_t* ring = base + qt * L::kQTile;                 // [stages][kStage]
+    uint8_t* sq = base;                                    // two Q tiles: of two segments, or of one with both streams' rows
+    uint8_t* ring = base + 2 * L::kQTile;                  // [stages][kStage]
     uint8_t* raw = ring + stages * L::kStage;              // e4m3: [kRaw][kRawTile]
     Shared* sh = reinterpret_cast<Shared*>(raw + (kFp8 ? kRaw * L::kRawTile : 0));
     Info* info = reinterpret_cast<Info*>(sh + 1);
@@ -575,8 +581,9 @@ __global__ void __launch_bounds__(kThreads, 1) attn_kernel(const __grid_constant
             mbar_init(&sh->info_full[i], kFp8 ? 33 : 1);
             mbar_init(&sh->info_empty[i], 1);
         }
-        mbar_init(&sh->q_full, 8);
         for (int i = 0; i < 2; ++i) {
+            mbar_init(&sh->q_full[i], kFp8 ? 1 : 33);
+            mbar_init(&sh->q_free[i], 8);
             for (int j = 0; j < 2; ++j) {
                 mbar_init(&sh->s_full[i][j], 1);
                 mbar_init(&sh->p_full[i][j], 4);
@@ -599,9 +606,6 @@ __global__ void __launch_bounds__(kThreads, 1) attn_kernel(const __grid_constant
     __syncthreads();
     tc_fence_after();
     constexpr uint32_t tmem = 0;                           // all 512 columns were allocated
-    Walk& w = sh->walk[warp];
-    if (lane == 0) w = sh->start;
-    __syncwarp();
     if (warp >= kFirstLoader) {
         // ---------------- loaders: rows of K and V by 16-byte copies of the lanes -----------------
         // fp16, bf16: a warp takes whole items (a tile of K or of V) in turn, straight into the
@@ -750,6 +754,9 @@ __global__ void __launch_bounds__(kThreads, 1) attn_kernel(const __grid_constant
         cp_wait_all();
     } else if (warp == kIndexWarp) {
         // ---------------- index: slots, scales and validity of the tiles to come ----------------
+        Walk& w = sh->walk[0];
+        if (lane == 0) w = sh->start;
+        __syncwarp();
         int ti = 0;
         bool ok = true;
         do {
@@ -816,6 +823,80 @@ __global__ void __launch_bounds__(kThreads, 1) attn_kernel(const __grid_constant
             }
         } while (ok && w.advance(a));
         if constexpr (kFp8) cp_wait_all();
+    } else if (warp == kQueryWarp) {
+        // ---------------- queries: the next segment and its rows of q, a segment ahead ------------
+        Walk& w = sh->walk[1];
+        if (lane == 0) w = sh->start;
+        __syncwarp();
+        constexpr int kLanes = DP / 8, kAtOnce = 32 / kLanes;   // lanes of a row (16-byte chunks), rows at once
+        const int sub = lane % kLanes, dr = lane / kLanes;
+        const bool live = sub * 8 < t.c.dim;
+        uint32_t seg = 0;
+        bool ok = true;
+        do {
+            const uint32_t buf = seg % q_bufs;
+            ok = wait_at(smem_u32(&sh->q_free[buf]), ((seg / q_bufs) & 1u) ^ 1u, abort);
+            if (!ok) break;
+            if (lane == 0) sh->seg[buf] = w;
+            const int nrows = w.rows(qt), row0 = w.first_row(qt);
+            const int filled = (nrows + 31) & ~31;              // whole warps of rows: zeros past the last
+            const int token0 = row0 / t.group, rem0 = row0 - token0 * t.group;
+            const TQ* q = static_cast<const TQ*>(t.q) + (long long)(w.r.lo + token0) * t.q_token_stride +
+                          (long long)(w.h * t.group) * t.q_head_stride + sub * 8;
+            uint8_t* dst = sq + buf * L::kQTile;
+            auto source = [&](int r) {
+                const int i = (int)a.group.divide(rem0 + r);
+                return q + i * t.q_token_stride + (rem0 + r - i * t.group) * t.q_head_stride;
+            };
+            if constexpr (!kFp8) {
+#pragma unroll 4
+                for (int r = dr; r < filled; r += kAtOnce) {
+                    const bool have = r < nrows && live;
+                    cp16_or_zero(smem_u32(dst + (r >> 7) * L::kQTile + chunk_at<kQBlock>(r & 127, sub)), have ? source(r) : q, have);
+                }
+                cp_arrive(&sh->q_full[buf]);
+            } else {
+#pragma unroll 1
+                for (int r0 = dr; r0 - dr < filled; r0 += 8 * kAtOnce) {
+                    uint4 x[8];
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) {
+                        const int r = r0 + i * kAtOnce;
+                        x[i] = make_uint4(0, 0, 0, 0);
+                        if (r < nrows && live) x[i] = __ldg(reinterpret_cast<const uint4*>(source(r)));
+                    }
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) {
+                        const int r = r0 + i * kAtOnce;
+                        float f[8];
+                        unpack2(x[i].x, f[0], f[1], TQ());
+                        unpack2(x[i].y, f[2], f[3], TQ());
+                        unpack2(x[i].z, f[4], f[5], TQ());
+                        unpack2(x[i].w, f[6], f[7], TQ());
+                        float m = 0.f;
+#pragma unroll
+                        for (int j = 0; j < 8; ++j) m = fmaxf(m, fabsf(f[j]));
+#pragma unroll
+                        for (int o = kLanes / 2; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+                        // a power of two that brings the row's largest value to [2^13, 2^14): products
+                        // stay exact, and values down to 2^-37 of the largest keep a place in fp16
+                        int e = (int)(__float_as_uint(m) >> 23) - 127;
+                        e = m > 0.f && e < 128 ? max(e, -100) : 13;
+                        const float up = __uint_as_float((uint32_t)(13 - e + 127) << 23);
+                        if (r < filled) {
+                            if (sub == 0) row_mul[buf * kRows + r] = __uint_as_float((uint32_t)(e - 13 + 127) << 23);
+                            *reinterpret_cast<uint4*>(dst + (r >> 7) * L::kQTile + chunk_at<kQBlock>(r & 127, sub)) =
+                                make_uint4(pack2(f[0] * up, f[1] * up, __half()), pack2(f[2] * up, f[3] * up, __half()),
+                                           pack2(f[4] * up, f[5] * up, __half()), pack2(f[6] * up, f[7] * up, __half()));
+                        }
+                    }
+                }
+            }
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&sh->q_full[buf]);
+            ++seg;
+        } while (w.advance(a));
+        if constexpr (!kFp8) cp_wait_all();
     } else if (warp == kScoreWarp || warp == kAccumWarp) {
         // ---------------- MMA issuers: one warp for S = Q K^T, one for O += P V ----------------
         // Two, because a unit costs the issuing warp more in waits, commits and issue than the
@@ -839,16 +920,18 @@ __global__ void __launch_bounds__(kThreads, 1) attn_kernel(const __grid_constant
         };
         do {
             // broadcasts: what the loop turns on is uniform, and so its operands stay in uniform registers
-            const bool both = __shfl_sync(0xffffffffu, (int)!w.shared_rows(qt), 0) != 0;   // both streams use every tile
-            const int nt = __shfl_sync(0xffffffffu, w.count(), 0);
+            const uint32_t buf = seg % q_bufs;
+            ok = wait_at(bars + offsetof(Shared, q_full) + 8 * buf, (seg / q_bufs) & 1u, abort);
+            if (!ok) break;
+            const bool both = __shfl_sync(0xffffffffu, (int)!sh->seg[buf].shared_rows(qt), 0) != 0;   // both streams use every tile
+            const int nt = __shfl_sync(0xffffffffu, sh->seg[buf].count(), 0);
             const int ahead = min(nt, both ? kAheadUnits / 2 : kAheadUnits);
             // unit u: stream u & 1, buffer (u >> 1) & 1; its tile u, or u >> 1 where both streams use it
             const uint32_t step = both ? 1u : 0u;
             const int units = nt << step;
             if (scores) {
                 const int ksteps = t.c.dim / 16;
-                const uint32_t q0 = desc_low(smem_u32(sq), 16), k0 = desc_low(smem_u32(ring), 16);
-                ok = wait_at(bars + offsetof(Shared, q_full), seg & 1u, abort);
+                const uint32_t q0 = desc_low(smem_u32(sq + buf * L::kQTile), 16), k0 = desc_low(smem_u32(ring), 16);
                 int left = ahead;                            // K tiles before the first V tile
                 auto ready = [&](int u) {                    // K tile and score buffer of unit u
                     const uint32_t s = u & 1, sb = (s << 1) | ((u >> 1) & 1);
@@ -858,7 +941,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_kernel(const __grid_constant
                     fence_proxy_async_smem();
                     tc_fence_after();
                 };
-                if (ok) ready(0);
+                ready(0);
                 for (int u = 0; ok && u < units; ++u) {
                     const uint32_t s = u & 1, sb = (s << 1) | ((u >> 1) & 1), mine = st;
                     const uint32_t qa = q0 + (s & step) * (L::kQTile >> 4), kb = k0 + st * (L::kStage >> 4), d = tmem + sb * kTile;
@@ -908,7 +991,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_kernel(const __grid_constant
             }
             tile0 += nt;
             ++seg;
-        } while (ok && __shfl_sync(0xffffffffu, (int)w.advance(a), 0) != 0);
+        } while (ok && tile0 < (uint32_t)count);
         // every instruction issued here is done before TMEM is released
         uint64_t* drain = &sh->drain[scores ? 0 : 1];
         mma_commit(smem_u32(drain));
@@ -921,9 +1004,6 @@ __global__ void __launch_bounds__(kThreads, 1) attn_kernel(const __grid_constant
         const uint32_t to = tmem + lanes + 256 + s * 128;
         constexpr int kLanes = DP / 8;                          // 16-byte chunks of a row
         constexpr int kStep = kSoftmaxThreads / kLanes;         // rows that the 256 threads move at once
-        const int sub = tid % kLanes, r_first = tid / kLanes;
-        const bool sub_live = sub * 8 < t.c.dim;
-        const uint32_t group_inv = (0xFFFFFFFFu / (uint32_t)t.group) + 1u;  // ceil(2^32 / group), 0 for 1
         uint32_t seg = 0, tile0 = 0, item = 0, jp = 0;          // jp: phases of `joined`
         uint32_t ph = 0;                                        // parity of each buffer
         bool ok = true;
@@ -934,75 +1014,23 @@ __global__ void __launch_bounds__(kThreads, 1) attn_kernel(const __grid_constant
             ++jp;
         };
         do {
+            const uint32_t buf = seg % q_bufs;
+            ok = wait_at(smem_u32(&sh->q_full[buf]), (seg / q_bufs) & 1u, abort);
+            if (!ok) break;
+            const Walk& w = sh->seg[buf];
+            uint8_t* sqb = sq + buf * L::kQTile;
             const bool both = !w.shared_rows(qt);
             const int nt = w.count(), nrows = w.rows(qt), row0 = w.first_row(qt);
             const int my = both ? s * kRows + row : row;        // row of the block
             const int token0 = row0 / t.group, rem0 = row0 - token0 * t.group;
-            // drafted token (from token0) and query head of the block's row r
-            auto token_of = [&](int r, int& gq) {
-                const uint32_t x = rem0 + r;
-                const int i = t.group == 1 ? (int)x : (int)__umulhi(x, group_inv);
-                gq = (int)x - i * t.group;
-                return i;
-            };
-            auto q_offset = [&](int r, long long ts_, long long hs) {
-                int gq;
-                const int i = token_of(r, gq);
-                return (long long)(w.r.lo + token0 + i) * ts_ + (long long)(w.h * t.group + gq) * hs;
-            };
-            // ---- Q into shared memory: whole warps of rows, zeros past the last
-            {
-                const int filled = (nrows + 31) & ~31;
-                const TQ* q = static_cast<const TQ*>(t.q) + sub * 8;
-#pragma unroll 1
-                for (int r0 = r_first; r0 - r_first < filled; r0 += 8 * kStep) {
-                    uint4 x[8];
-#pragma unroll
-                    for (int i = 0; i < 8; ++i) {
-                        const int r = r0 + i * kStep;
-                        x[i] = make_uint4(0, 0, 0, 0);
-                        if (r < nrows && sub_live)
-                            x[i] = __ldg(reinterpret_cast<const uint4*>(q + q_offset(r, t.q_token_stride, t.q_head_stride)));
-                    }
-#pragma unroll
-                    for (int i = 0; i < 8; ++i) {
-                        const int r = r0 + i * kStep;
-                        if constexpr (kFp8) {
-                            float f[8];
-                            unpack2(x[i].x, f[0], f[1], TQ());
-                            unpack2(x[i].y, f[2], f[3], TQ());
-                            unpack2(x[i].z, f[4], f[5], TQ());
-                            unpack2(x[i].w, f[6], f[7], TQ());
-                            float m = 0.f;
-#pragma unroll
-                            for (int j = 0; j < 8; ++j) m = fmaxf(m, fabsf(f[j]));
-#pragma unroll
-                            for (int o = kLanes / 2; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-                            // a power of two that brings the row's largest value to [2^13, 2^14): products
-                            // stay exact, and values down to 2^-37 of the largest keep a place in fp16
-                            int e = (int)(__float_as_uint(m) >> 23) - 127;
-                            e = m > 0.f && e < 128 ? max(e, -100) : 13;
-                            const float up = __uint_as_float((uint32_t)(13 - e + 127) << 23);
-                            if (sub == 0 && r < filled) row_mul[r] = __uint_as_float((uint32_t)(e - 13 + 127) << 23);
-                            x[i] = make_uint4(pack2(f[0] * up, f[1] * up, __half()), pack2(f[2] * up, f[3] * up, __half()),
-                                              pack2(f[4] * up, f[5] * up, __half()), pack2(f[6] * up, f[7] * up, __half()));
-                        }
-                        if (r < filled)
-                            *reinterpret_cast<uint4*>(sq + (r >> 7) * L::kQTile + chunk_at<kQBlock>(r & 127, sub)) = x[i];
-                    }
-                }
-                tc_fence_before();
-                __syncwarp();
-                if (lane == 0) mbar_arrive(&sh->q_full);
-                if constexpr (kFp8)                             // row_mul comes from all eight warps
-                    ok = __all_sync(0xffffffffu, ok && wait_or_abort(&sh->q_full, seg & 1u, abort));
-            }
             const bool any_row = (both ? s * kRows : 0) + quarter * 32 < nrows;  // this warp has rows
-            const float cm = t.scale * kL2E * (kFp8 && any_row ? row_mul[my] : 1.f);
+            const float cm = t.scale * kL2E * (kFp8 && any_row ? row_mul[buf * kRows + my] : 1.f);
             int token = 0, gq = 0;                              // this row's drafted token and head
             uint64_t bits = 0;
             if (my < nrows) {
-                token = token0 + token_of(my, gq);
+                token = (int)a.group.divide(rem0 + my);
+                gq = rem0 + my - token * t.group;
+                token += token0;
                 if (t.mask) bits = (uint64_t)__ldg(reinterpret_cast<const long long*>(t.mask) + w.r.lo + token);
             }
             float ref = -INFINITY, sum = 0.f, vmax = 0.f;
@@ -1191,7 +1219,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_kernel(const __grid_constant
             ok = __all_sync(0xffffffffu, ok && wait_or_abort(&sh->o_full, seg & 1u, abort));
             if (!ok) break;
             tc_fence_after();
-            float2* swap = reinterpret_cast<float2*>(sq);       // [2][128]: Q has been used
+            float2* swap = reinterpret_cast<float2*>(sqb);      // [2][128]: Q has been used
             if (!both) swap[s * kRows + row] = make_float2(ref, sum);
             join();
             if (!ok) break;
@@ -1216,7 +1244,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_kernel(const __grid_constant
                 const long long slot = 2 * blockIdx.x + (w.k0 == 0 ? 1 : 0);
                 const int per = kRows * qt;
                 float4* po = a.part_o + slot * (DP / 4) * per + my;
-                uint8_t* so = sq + (my >> 7) * L::kQTile;
+                uint8_t* so = sqb + (my >> 7) * L::kQTile;
                 const float inv = sum == 0.f ? 0.f : 1.0f / sum;
                 const int c0 = both ? 0 : s * (DP / 2), c1 = both ? DP : c0 + DP / 2;
 #pragma unroll 1
@@ -1283,24 +1311,29 @@ __global__ void __launch_bounds__(kThreads, 1) attn_kernel(const __grid_constant
                             sum == 0.f ? -INFINITY : (ref + log2f(sum)) * kLn2;
                 }
             }
+            tc_fence_before();
+            join();                                             // TMEM has been read, rows are staged
+            if (!ok) break;
             if (whole) {
-                // rows leave through shared memory, 16 bytes a thread and whole rows a warp; each
-                // thread later writes the next Q where it has read here
-                join();
-                if (!ok) break;
-                TQ* out = static_cast<TQ*>(t.out) + sub * 8;
-                if (sub_live) {
+                // rows leave through shared memory, 16 bytes a thread and whole rows a warp
+                const int sub = tid % kLanes;
+                if (sub * 8 < t.c.dim) {
+                    TQ* out = static_cast<TQ*>(t.out) + (long long)(w.r.lo + token0) * t.out_token_stride +
+                              (long long)(w.h * t.group) * t.out_head_stride + sub * 8;
 #pragma unroll 4
-                    for (int r = r_first; r < nrows; r += kStep)
-                        *reinterpret_cast<uint4*>(out + q_offset(r, t.out_token_stride, t.out_head_stride)) =
-                            *reinterpret_cast<const uint4*>(sq + (r >> 7) * L::kQTile + chunk_at<kQBlock>(r & 127, sub));
+                    for (int r = tid / kLanes; r < nrows; r += kStep) {
+                        const int i = (int)a.group.divide(rem0 + r);
+                        *reinterpret_cast<uint4*>(out + i * t.out_token_stride + (rem0 + r - i * t.group) * t.out_head_stride) =
+                            *reinterpret_cast<const uint4*>(sqb + (r >> 7) * L::kQTile + chunk_at<kQBlock>(r & 127, sub));
+                    }
                 }
             }
-            tc_fence_before();
             tile0 += nt;
             item += 2 * nt;
             ++seg;
-        } while (w.advance(a));
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&sh->q_free[buf]);
+        } while (tile0 < (uint32_t)count);
     }
 
     __syncthreads();
@@ -1377,7 +1410,7 @@ template <typename TQ, bool kFp8, int DP>
 int launch(const KernelArgs& a, int sms, cudaStream_t st) {
     using L = Layout<DP, kFp8>;
     auto kern = attn_kernel<TQ, kFp8, DP>;
-    const size_t smem = L::smem(a.qt);
+    const size_t smem = L::smem();
     if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess)
         return kLaunchFailed;
     const int grid = sms < kMaxCtas ? sms : kMaxCtas;
@@ -1414,6 +1447,7 @@ int launch_tree_attn(const TreeAttnArgs& t, int dtype, cudaStream_t st) {
     a.t = t;
     a.qt = q_tiles(t.group, t.width);
     a.page = divisor((uint32_t)t.page_size);
+    a.group = divisor((uint32_t)t.group);
     a.pages = (int)(t.c.slots / t.page_size);
     char* ws = static_cast<char*>(t.ws);
     a.splits = reinterpret_cast<Split*>(ws);
