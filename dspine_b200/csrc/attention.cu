@@ -68,7 +68,6 @@ constexpr int kQBlock = kRows * 128;       // bytes of a [128 rows][128 bytes] s
 constexpr int kBlock = kTile * 128;        // the same of a K or V tile
 constexpr int kMaxCtas = 148;              // SMs of a B200; partial results are laid out for these
 constexpr int kInfo = 16;                  // tiles that are described in shared memory at once
-constexpr int kAheadUnits = 4;             // score tiles in TMEM: two streams x two buffers
 constexpr int kSoftmaxThreads = 256;
 constexpr int kMinTiles = 4;               // tiles per CTA below which fewer CTAs take part
 constexpr float kSlack = 8.0f;             // log2 by which a maximum may outgrow the reference
@@ -82,7 +81,7 @@ constexpr int kScoreWarp = 8, kAccumWarp = 9, kIndexWarp = 10, kQueryWarp = 11, 
 struct alignas(16) TileInfoPlain {
     int slot[kTile];          // of each position; 0 where there is none or it cannot be read
     uint32_t valid[2];        // the positions with a slot
-    int head, tiles, ahead;   // of the segment: KV head, tiles, K tiles loaded before its first V tile
+    int head;                 // KV head
     int pad;
 };
 struct TileInfoScaled : TileInfoPlain {
@@ -188,7 +187,6 @@ struct Walk {
     int tiles;              // of the item
     int k0, k1;             // this segment's tiles
     long long left;         // tiles of this CTA after this segment
-    int next_k0;            // where the item goes on
 
     // tile in_b of request b0's tiles (per_head of them for each KV head)
     __device__ __forceinline__ void begin(const KernelArgs& a, int b0, const Request& r0, long long per_head, long long in_b,
@@ -255,12 +253,12 @@ struct Walk {
     __device__ __forceinline__ bool shared_rows(int qt) const { return rows(qt) <= kRows; }
 };
 
-constexpr int kMaxStages = 12;
-constexpr int kRaw = 6;                    // e4m3: tiles of codes in shared memory, all but one in flight
+constexpr int kMaxStages = 6;              // of the K ring, and of the V ring
+constexpr int kRaw = 2;                    // e4m3: tiles of codes that a loader warp holds, one of them in flight
 
 struct alignas(16) Shared {
-    uint64_t full[kMaxStages];       // stage holds a K or V tile
-    uint64_t empty[kMaxStages];      // the matrix instructions that read it are done
+    uint64_t full[2][kMaxStages];    // stage holds a K (first), a V tile
+    uint64_t empty[2][kMaxStages];   // the matrix instructions that read it are done
     uint64_t info_full[kInfo];       // tile described
     uint64_t info_empty[kInfo];      // its last matrix instructions are done
     uint64_t q_full[2];              // a segment and its Q in shared memory
@@ -274,6 +272,7 @@ struct alignas(16) Shared {
     uint32_t tmem;
     int abort;
     int odd[2];                      // a drafted V element was not finite (by segment parity)
+    int v_done[2];                   // e4m3: V tiles (even, odd) in their stages, as one past the last
     long long scan[32];
     Walk start;                      // where this CTA starts on the line of tiles
     Walk seg[2];                     // the segments whose Q is here; read in place, registers are full
@@ -284,12 +283,13 @@ template <int DP, bool kFp8> struct Layout {
     static constexpr int kQTile = (DP / 64) * kQBlock;     // bytes of a Q tile
     static constexpr int kStage = (DP / 64) * kBlock;      // bytes of a K or V stage
     static constexpr int kRawTile = kFp8 ? kTile * DP : 0; // bytes of a tile of codes
-    static __host__ __device__ constexpr int stages() {
-        return kFp8 ? (DP == 128 ? 5 : 8) : (DP == 128 ? 9 : 12);
-    }
+    // stages of the K ring, and of the V ring.  Even: two loader warps share a ring, and a stage is
+    // always filled by the same one and read by the same issuer, so that a wait on a stage's parity
+    // never meets a phase two behind.
+    static __host__ __device__ constexpr int stages() { return kFp8 ? (DP == 128 ? 2 : 4) : (DP == 128 ? 4 : 6); }
     static constexpr size_t info_bytes = sizeof(typename InfoOf<kFp8>::type) * kInfo;
     static constexpr size_t smem() {
-        return (size_t)2 * kQTile + (size_t)stages() * kStage + kRaw * kRawTile + sizeof(Shared) + info_bytes + (kFp8 ? 1024 : 0) + 1024;
+        return (size_t)2 * kQTile + (size_t)2 * stages() * kStage + kLoaders * kRaw * kRawTile + sizeof(Shared) + info_bytes + (kFp8 ? 1024 : 0) + 1024;
     }
 };
 static_assert(Layout<128, false>::smem() <= 232448 && Layout<128, true>::smem() <= 232448 && Layout<64, false>::smem() <= 232448 &&
@@ -462,6 +462,20 @@ __device__ __noinline__ bool wait_slow_at(uint32_t bar, uint32_t parity, volatil
         }
     }
 }
+// until *at is past `value`
+__device__ __noinline__ bool wait_past(volatile int* at, int value, volatile int* abort) {
+    const uint64_t t0 = globaltimer_ns();
+    for (uint32_t i = 1; *at <= value; ++i) {
+        if (i % 32 != 0) continue;
+        if (*abort) return false;
+        if (globaltimer_ns() - t0 > 2000000000ull) {
+            *abort = 1;
+            return false;
+        }
+    }
+    __threadfence_block();
+    return true;
+}
 __device__ __forceinline__ bool wait_at(uint32_t bar, uint32_t parity, volatile int* abort) {
     if (__all_sync(0xffffffffu, try_wait_at(bar, parity))) return true;
     return __all_sync(0xffffffffu, wait_slow_at(bar, parity, abort));
@@ -473,15 +487,8 @@ __device__ __forceinline__ uint32_t chunk_at(int row, int c) {
     return (uint32_t)((c >> 3) * block + row * 128 + (((c ^ row) & 7) << 4));
 }
 
-// ---- the order of the tiles ---------------------------------------------------------------------
-// A unit is one stream's share of a tile: unit u belongs to stream u & 1 and uses its score buffer
-// (u >> 1) & 1; its tile is u, or u >> 1 where both streams use every tile.  The scores of unit
-// u + 4 are issued behind the accumulation of unit u, so that two score tiles of each stream are in
-// work; K tiles are therefore loaded `ahead` tiles before V: K0 .. K(ahead-1), V0, K(ahead), V1, ...
-__device__ __forceinline__ int item_of_k(int t, int ahead) { return t < ahead ? t : 2 * t - ahead + 1; }
-__device__ __forceinline__ int item_of_v(int t, int n, int ahead) {
-    return n <= ahead ? n + t : ahead + t + min(t, n - ahead);
-}
+// A unit is one stream's share of a tile: unit u of a segment belongs to stream u & 1 and uses its
+// score buffer (u >> 1) & 1; its tile is u, or u >> 1 where both streams use every tile.
 
 // ---- the kernel ---------------------------------------------------------------------------------
 
@@ -495,9 +502,9 @@ __global__ void __launch_bounds__(kThreads, 1) attn_kernel(const __grid_constant
     const int qt = a.qt, q_bufs = qt == 1 ? 2 : 1;         // segments whose Q is held at once
     uint8_t* base = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
     uint8_t* sq = base;                                    // two Q tiles: of two segments, or of one with both streams' rows
-    uint8_t* ring = base + 2 * L::kQTile;                  // [stages][kStage]
-    uint8_t* raw = ring + stages * L::kStage;              // e4m3: [kRaw][kRawTile]
-    Shared* sh = reinterpret_cast<Shared*>(raw + (kFp8 ? kRaw * L::kRawTile : 0));
+    uint8_t* ring = base + 2 * L::kQTile;                  // [K, V][stages][kStage]
+    uint8_t* raw = ring + 2 * stages * L::kStage;              // e4m3: [kLoaders][kRaw][kRawTile]
+    Shared* sh = reinterpret_cast<Shared*>(raw + (kFp8 ? kLoaders * kRaw * L::kRawTile : 0));
     Info* info = reinterpret_cast<Info*>(sh + 1);
     float* row_mul = reinterpret_cast<float*>(info + kInfo);        // e4m3: [128 qt] power of two of a row of q
     volatile int* abort = &sh->abort;
@@ -574,8 +581,10 @@ __global__ void __launch_bounds__(kThreads, 1) attn_kernel(const __grid_constant
 
     if (tid == 0) {
         for (int s = 0; s < stages; ++s) {
-            mbar_init(&sh->full[s], kFp8 ? kLoaders : 32);
-            mbar_init(&sh->empty[s], 1);
+            for (int i = 0; i < 2; ++i) {
+                mbar_init(&sh->full[i][s], kFp8 ? 1 : 32);
+                mbar_init(&sh->empty[i][s], 1);
+            }
         }
         for (int i = 0; i < kInfo; ++i) {
             mbar_init(&sh->info_full[i], kFp8 ? 33 : 1);
@@ -595,6 +604,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_kernel(const __grid_constant
         mbar_init(&sh->joined, 8);
         sh->abort = 0;
         sh->odd[0] = sh->odd[1] = 0;
+        sh->v_done[0] = sh->v_done[1] = 0;
         fence_mbar_init();
     }
     if (warp == kScoreWarp) {
@@ -608,9 +618,9 @@ __global__ void __launch_bounds__(kThreads, 1) attn_kernel(const __grid_constant
     constexpr uint32_t tmem = 0;                           // all 512 columns were allocated
     if (warp >= kFirstLoader) {
         // ---------------- loaders: rows of K and V by 16-byte copies of the lanes -----------------
-        // fp16, bf16: a warp takes whole items (a tile of K or of V) in turn, straight into the
-        // swizzled stage.  e4m3: each warp takes its 16 rows of every item, as codes into its own
-        // part of a raw ring (kRaw - 1 items in flight), and from there as fp16 into the stage.
+        // Two warps for K tiles, two for V, every other tile each.  fp16, bf16: straight into the
+        // swizzled stage.  e4m3: as codes into a raw tile of its own, the next one's on the way
+        // while each lane brings what it has copied into the stage as fp16.
         // Copies of a lane, not TMA: one warp of them reaches 5.6 TB/s, two 6.7, whatever the page
         // size; gathers of four rows and bulk copies of one stay at 2.2 and 1.3 (scattered rows of
         // 256 bytes, nothing else running).
@@ -618,62 +628,45 @@ __global__ void __launch_bounds__(kThreads, 1) attn_kernel(const __grid_constant
         constexpr int kElem = kFp8 ? 1 : 2;                     // bytes of a cached element
         const uint32_t stride = (uint32_t)t.c.slot_stride * (uint32_t)kElem;   // bytes from slot to slot
         constexpr int kLanes = DP * kElem / 16, kAtOnce = 32 / kLanes;         // lanes of a row, rows at once
-        constexpr int kSteps = (kFp8 ? kTile / kLoaders : kTile) / kAtOnce;
+        constexpr int kSteps = kTile / kAtOnce;
         // e4m3: a row of codes becomes up to two blocks of fp16; four lanes of one row then stand beside
         // four of the next, so that their stores of eight hit eight different groups of banks
         const int sub = kFp8 && DP == 128 ? (lane & 3) | ((lane >> 1) & 4) : lane % kLanes;
         const int dr = kFp8 && DP == 128 ? ((lane >> 2) & 1) | ((lane >> 3) & 2) : lane / kLanes;
         // rows of step k: e4m3 kAtOnce adjacent ones; else dr's own run of kSteps
-        const int row0 = kFp8 ? lw * (kTile / kLoaders) + dr : dr * kSteps;
+        const int row0 = kFp8 ? dr : dr * kSteps;
         const bool live = sub * (16 / kElem) < t.c.dim;
-        const uint32_t bars = smem_u32(sh), empty = bars + offsetof(Shared, empty), described = bars + offsetof(Shared, info_full);
-        // items in order: per segment its first K tiles (lead of them), then V and K in turn
-        int kt = 0, vt = 0, k_left = 0, v_left = 0, lead = 0;   // next tiles of the CTA, left in the segment
-        bool ok = true, more = true, k_turn = false;
-        long long head_at = 0;
+        const int which = lw >> 1;                              // 0: K, 1: V
+        const uint32_t bars = smem_u32(sh), empty = bars + offsetof(Shared, empty) + which * (kMaxStages * 8);
+        uint64_t* full = sh->full[which];
+        uint8_t* stage0 = ring + which * (stages * L::kStage);
+        const uint8_t* rows = static_cast<const uint8_t*>(which ? t.c.v : t.c.k) + sub * 16;
+        int tl = (lw & 1) - 2;                                  // this warp's tile
+        bool ok = true;
         const uint8_t* src = nullptr;
         const int* slots = nullptr;
-        auto wait_described = [&](int tl) { return wait_at(described + 8 * (tl % kInfo), (uint32_t)(tl / kInfo) & 1u, abort); };
-        auto next = [&](bool mine) {                            // false past the last, or after a wait that gave up
-            if (v_left == 0) {
-                if (kt >= (int)count) return false;
-                ok = wait_described(kt);
-                if (!ok) return false;
-                const Info* f = info + kt % kInfo;
-                k_left = v_left = f->tiles;
-                lead = min(f->ahead, k_left);
-                head_at = kElem * (f->head * t.c.head_stride) + sub * 16;
-            }
-            const bool is_k = lead > 0 || (k_turn && k_left > 0);
-            int tl;
-            if (is_k) {
-                tl = kt++;
-                --k_left;
-                lead = max(lead - 1, 0);
-                k_turn = false;
-            } else {
-                tl = vt++;
-                --v_left;
-                k_turn = true;
-            }
-            if (mine) {
-                // a warp that sees every item has waited for a V tile's description with its K tile
-                if (is_k || !kFp8) ok = wait_described(tl);
-                slots = info[tl % kInfo].slot + row0;
-                src = static_cast<const uint8_t*>(is_k ? t.c.k : t.c.v) + head_at;
-            }
+        auto next = [&]() {                                     // false past the last, or after a wait that gave up
+            tl += 2;
+            if (tl >= (int)count) return false;
+            ok = wait_at(bars + offsetof(Shared, info_full) + 8 * (tl % kInfo), (uint32_t)(tl / kInfo) & 1u, abort);
+            slots = info[tl % kInfo].slot + row0;
+            src = rows + kElem * (info[tl % kInfo].head * t.c.head_stride);
             return ok;
         };
+        uint32_t s = lw & 1, ph = 1;                            // stage, and the parity that says it is free
+        auto step_stage = [&]() {
+            s += 2;
+            if (s >= (uint32_t)stages) {
+                s -= stages;
+                ph ^= 1u;
+            }
+        };
         if constexpr (!kFp8) {
-            uint32_t s = lw, ph = 1;                            // stage, and the parity that says it is free
-            for (int item = 0;; ++item) {
-                const bool mine = item % kLoaders == lw;
-                if (!next(mine)) break;
-                if (!mine) continue;
+            while (next()) {
                 ok = wait_at(empty + 8 * s, ph, abort);
                 if (!ok) break;
                 // chunk of row r: rows are 128 bytes apart, the chunk's place is xored with r & 7
-                const uint32_t dst = smem_u32(ring + s * L::kStage) + (sub >> 3) * kBlock + row0 * 128 + ((sub & 7) << 4);
+                const uint32_t dst = smem_u32(stage0 + s * L::kStage) + (sub >> 3) * kBlock + row0 * 128 + ((sub & 7) << 4);
                 if (live) {
                     // slots four at a time, and the next four before the copies of these are issued
                     // (loads do not move past the copies by themselves)
@@ -689,66 +682,73 @@ __global__ void __launch_bounds__(kThreads, 1) attn_kernel(const __grid_constant
                         cp16((at ^ 48) + to + 384, src + (uint64_t)(uint32_t)now.w * stride);
                     }
                 }
-                cp_arrive(&sh->full[s]);
-                s += kLoaders;
-                if (s >= (uint32_t)stages) {
-                    s -= stages;
-                    ph ^= 1u;
-                }
+                cp_arrive(full + s);
+                step_stage();
             }
         } else {
-            constexpr int kPart = L::kRawTile / kLoaders;       // this warp's rows of a raw tile
-            uint8_t* mine_raw = raw + lw * kPart + dr * DP + sub * 16;
-            auto load = [&](uint32_t r) {
-                more = more && next(true);
-                if (more && live) {
-                    const uint32_t dst = smem_u32(mine_raw + r * L::kRawTile);
-                    int slot[kSteps];
-#pragma unroll
-                    for (int k = 0; k < kSteps; ++k) slot[k] = slots[k * kAtOnce];
-#pragma unroll
-                    for (int k = 0; k < kSteps; ++k) cp16(dst + k * kAtOnce * DP, src + (uint64_t)(uint32_t)slot[k] * stride);
-                }
-                cp_commit();
-            };
-            const long long items = 2 * count;
-            uint32_t s = 0, ph = 1, r = 0, ahead_r = 0;
+            uint8_t* own = raw + lw * (kRaw * L::kRawTile) + dr * DP + sub * 16;
+            auto fetch = [&](uint32_t r) {                      // this warp's next tile on its way to raw tile r
+                if (!next()) return false;
+                if (live) {
+                    const uint32_t dst = smem_u32(own + r * L::kRawTile);
 #pragma unroll 1
-            for (long long item = 1 - kRaw; item < items; ++item) {
-                load(ahead_r);                                  // item + kRaw - 1
-                if (++ahead_r == (uint32_t)kRaw) ahead_r = 0;
+                    for (int k = 0; k < kSteps; k += 8) {
+                        int slot[8];
+#pragma unroll
+                        for (int q = 0; q < 8; ++q) slot[q] = slots[(k + q) * kAtOnce];
+#pragma unroll
+                        for (int q = 0; q < 8; ++q)
+                            cp16(dst + (k + q) * kAtOnce * DP, src + (uint64_t)(uint32_t)slot[q] * stride);
+                    }
+                }
+                return true;
+            };
+            uint32_t r = 0;
+            int done = lw & 1;                                  // the tile being converted
+            bool have = fetch(0);
+            cp_commit();
+#pragma unroll 1
+            while (have) {
+                have = fetch(r ^ 1);
+                cp_commit();
                 if (!ok) break;
-                if (item < 0) continue;
-                cp_wait<kRaw - 1>();                            // this item's codes have landed
+                cp_wait<1>();                                   // this tile's codes have landed
                 ok = wait_at(empty + 8 * s, ph, abort);
                 if (!ok) break;
-                const uint8_t* from = mine_raw + r * L::kRawTile;
-                uint8_t* dst = ring + s * L::kStage;
+                const uint8_t* from = own + r * L::kRawTile;
+                uint8_t* dst = stage0 + s * L::kStage;
                 if (live) {
-                    uint4 x[kSteps];                            // all loads before the first store
+#pragma unroll 1
+                    for (int k0 = 0; k0 < kSteps; k0 += 4) {
+                        uint4 x[4];                             // all loads before the first store
 #pragma unroll
-                    for (int k = 0; k < kSteps; ++k) x[k] = *reinterpret_cast<const uint4*>(from + k * kAtOnce * DP);
+                        for (int k = 0; k < 4; ++k) x[k] = *reinterpret_cast<const uint4*>(from + (k0 + k) * kAtOnce * DP);
 #pragma unroll
-                    for (int k = 0; k < kSteps; ++k) {
-                        const int row = row0 + k * kAtOnce;
-                        const uint32_t c4[4] = {x[k].x, x[k].y, x[k].z, x[k].w};
-                        uint32_t o[8];
+                        for (int k = 0; k < 4; ++k) {
+                            const int row = row0 + (k0 + k) * kAtOnce;
+                            const uint32_t c4[4] = {x[k].x, x[k].y, x[k].z, x[k].w};
+                            uint32_t o[8];
 #pragma unroll
-                        for (int q = 0; q < 8; ++q) {
-                            const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2((uint16_t)(c4[q >> 1] >> (16 * (q & 1))), __NV_E4M3);
-                            o[q] = (uint32_t)h.x | ((uint32_t)h.y << 16);
+                            for (int q = 0; q < 8; ++q) {
+                                const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2((uint16_t)(c4[q >> 1] >> (16 * (q & 1))), __NV_E4M3);
+                                o[q] = (uint32_t)h.x | ((uint32_t)h.y << 16);
+                            }
+                            *reinterpret_cast<uint4*>(dst + chunk_at<kBlock>(row, 2 * sub)) = make_uint4(o[0], o[1], o[2], o[3]);
+                            *reinterpret_cast<uint4*>(dst + chunk_at<kBlock>(row, 2 * sub + 1)) = make_uint4(o[4], o[5], o[6], o[7]);
                         }
-                        *reinterpret_cast<uint4*>(dst + chunk_at<kBlock>(row, 2 * sub)) = make_uint4(o[0], o[1], o[2], o[3]);
-                        *reinterpret_cast<uint4*>(dst + chunk_at<kBlock>(row, 2 * sub + 1)) = make_uint4(o[4], o[5], o[6], o[7]);
                     }
                 }
                 __syncwarp();
-                if (lane == 0) mbar_arrive(&sh->full[s]);
-                if (++s == (uint32_t)stages) {
-                    s = 0;
-                    ph ^= 1u;
+                if (lane == 0) {
+                    if (which) {
+                        __threadfence_block();
+                        *(volatile int*)&sh->v_done[lw & 1] = done + 1;
+                    }
+                    mbar_arrive(full + s);
                 }
-                if (++r == (uint32_t)kRaw) r = 0;
+                done += 2;
+                step_stage();
+                r ^= 1;
             }
         }
         cp_wait_all();
@@ -760,7 +760,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_kernel(const __grid_constant
         int ti = 0;
         bool ok = true;
         do {
-            const int nt = w.count(), ahead = w.shared_rows(qt) ? kAheadUnits : kAheadUnits / 2;
+            const int nt = w.count();
             const int* table = t.table + (long long)w.b * t.table_stride;
             // a tile's page table entries are fetched one round of two tiles ahead
             auto entry_of = [&](int tl, int e) {
@@ -813,8 +813,6 @@ __global__ void __launch_bounds__(kThreads, 1) attn_kernel(const __grid_constant
                         f->valid[0] = valid[0];
                         f->valid[1] = valid[1];
                         f->head = w.h;
-                        f->tiles = nt;
-                        f->ahead = ahead;
                     }
                     __syncwarp();
                     if (lane == 0) mbar_arrive(&sh->info_full[at]);
@@ -904,17 +902,17 @@ __global__ void __launch_bounds__(kThreads, 1) attn_kernel(const __grid_constant
         constexpr uint32_t kFormat = std::is_same<TO, __nv_bfloat16>::value ? 1u : 0u;
         constexpr uint32_t kCommon = (1u << 4) | (kFormat << 7) | (kFormat << 10) | ((uint32_t)(kRows >> 4) << 24);
         constexpr uint32_t kIdescS = kCommon | ((uint32_t)(kTile >> 3) << 17);
-        const uint32_t bars = smem_u32(sh), full = bars + offsetof(Shared, full), empty = bars + offsetof(Shared, empty),
+        const bool scores = warp == kScoreWarp;
+        const uint32_t bars = smem_u32(sh), full = bars + offsetof(Shared, full) + (scores ? 0 : kMaxStages * 8),
+                       empty = bars + offsetof(Shared, empty) + (scores ? 0 : kMaxStages * 8),
                        s_full = bars + offsetof(Shared, s_full), p_full = bars + offsetof(Shared, p_full),
                        s_free = bars + offsetof(Shared, s_free);
-        const bool scores = warp == kScoreWarp;
         uint32_t seg = 0, tile0 = 0, ph = 0;                 // ph: parity of each (stream, buffer)
-        uint32_t st = 0, sp = 0;                             // stage of the ring, and its parity
+        uint32_t st = 0, sp = 0;                             // stage of the warp's ring, and its parity
         bool ok = true;
-        auto skip = [&](uint32_t n) {                        // n items on
-            st += n;
-            if (st >= (uint32_t)stages) {
-                st -= stages;
+        auto step_stage = [&]() {
+            if (++st == (uint32_t)stages) {
+                st = 0;
                 sp ^= 1u;
             }
         };
@@ -925,14 +923,11 @@ __global__ void __launch_bounds__(kThreads, 1) attn_kernel(const __grid_constant
             if (!ok) break;
             const bool both = __shfl_sync(0xffffffffu, (int)!sh->seg[buf].shared_rows(qt), 0) != 0;   // both streams use every tile
             const int nt = __shfl_sync(0xffffffffu, sh->seg[buf].count(), 0);
-            const int ahead = min(nt, both ? kAheadUnits / 2 : kAheadUnits);
-            // unit u: stream u & 1, buffer (u >> 1) & 1; its tile u, or u >> 1 where both streams use it
             const uint32_t step = both ? 1u : 0u;
             const int units = nt << step;
             if (scores) {
                 const int ksteps = t.c.dim / 16;
                 const uint32_t q0 = desc_low(smem_u32(sq + buf * L::kQTile), 16), k0 = desc_low(smem_u32(ring), 16);
-                int left = ahead;                            // K tiles before the first V tile
                 auto ready = [&](int u) {                    // K tile and score buffer of unit u
                     const uint32_t s = u & 1, sb = (s << 1) | ((u >> 1) & 1);
                     if (!(s & step)) ok = wait_at(full + 8 * st, sp, abort);
@@ -955,7 +950,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_kernel(const __grid_constant
 #pragma unroll
                     for (int k = 0; k < DP / 32; ++k) issue(k);
                     // the next unit's waits while these execute
-                    if (last) skip(u == units - 1 ? ahead + 1 : (--left > 0 ? 1 : 2));
+                    if (last) step_stage();
                     if (u + 1 < units) ready(u + 1);
                     if (!ok) break;
 #pragma unroll
@@ -964,10 +959,8 @@ __global__ void __launch_bounds__(kThreads, 1) attn_kernel(const __grid_constant
                     if (last) mma_commit(empty + 8 * mine);
                 }
             } else {
-                const uint32_t v0 = desc_low(smem_u32(ring), kBlock);
+                const uint32_t v0 = desc_low(smem_u32(ring + stages * L::kStage), kBlock);
                 const uint32_t idesc_o = kCommon | (1u << 16) | ((uint32_t)(t.c.dim >> 3) << 17);  // B: MN-major
-                int pairs = nt - ahead;                      // V tiles with a K tile behind them
-                skip(ahead);
                 for (int u = 0; ok && u < units; ++u) {
                     const uint32_t s = u & 1, sb = (s << 1) | ((u >> 1) & 1);
                     if (!(s & step)) ok = wait_at(full + 8 * st, sp, abort);
@@ -984,7 +977,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_kernel(const __grid_constant
                     if ((s & step) == step) {
                         mma_commit(empty + 8 * st);
                         mma_commit(bars + offsetof(Shared, info_empty) + 8 * ((tile0 + (u >> step)) % kInfo));
-                        skip(pairs-- > 0 ? 2 : 1);
+                        step_stage();
                     }
                 }
                 if (ok) mma_commit(bars + offsetof(Shared, o_full));
@@ -1004,7 +997,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_kernel(const __grid_constant
         const uint32_t to = tmem + lanes + 256 + s * 128;
         constexpr int kLanes = DP / 8;                          // 16-byte chunks of a row
         constexpr int kStep = kSoftmaxThreads / kLanes;         // rows that the 256 threads move at once
-        uint32_t seg = 0, tile0 = 0, item = 0, jp = 0;          // jp: phases of `joined`
+        uint32_t seg = 0, tile0 = 0, jp = 0;                    // jp: phases of `joined`
         uint32_t ph = 0;                                        // parity of each buffer
         bool ok = true;
         auto join = [&]() {                                     // both warpgroups have come here
@@ -1034,7 +1027,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_kernel(const __grid_constant
                 if (t.mask) bits = (uint64_t)__ldg(reinterpret_cast<const long long*>(t.mask) + w.r.lo + token);
             }
             float ref = -INFINITY, sum = 0.f, vmax = 0.f;
-            const int step = both ? 1 : 2, ahead = min(nt, both ? kAheadUnits / 2 : kAheadUnits);
+            const int step = both ? 1 : 2;
             int b = 0;
             for (int tl = both ? 0 : s; ok && tl < nt; tl += step, b ^= 1) {
                 const uint32_t ti = tile0 + tl, ts = tmem + lanes + s * 128 + b * kTile;
@@ -1052,13 +1045,18 @@ __global__ void __launch_bounds__(kThreads, 1) attn_kernel(const __grid_constant
                     // V rows of positions that do not exist are zeroed (another slot's row was loaded);
                     // elements of drafted tokens that are not finite too, and added to the rows that
                     // see them at the end
-                    const uint32_t it = item + item_of_v(tl, nt, ahead), st = it % stages;
-                    ok = __all_sync(0xffffffffu, wait_or_abort(&sh->full[st], (it / stages) & 1u, abort));
+                    // (S of tile ti is there, so V of tile ti - 4 has been used: with four stages the parity
+                    // of V's barrier says which phase it is; a shorter ring has a counter beside it)
+                    const uint32_t st = ti % stages;
+                    if constexpr (stages >= 4)
+                        ok = wait_at(smem_u32(&sh->full[1][st]), (ti / stages) & 1u, abort);
+                    else
+                        ok = __all_sync(0xffffffffu, wait_past(&sh->v_done[ti & 1], (int)ti, abort));
                     if (!ok) break;
                     const int key = row & (kTile - 1);          // two threads a key
                     const bool gone = !(((key & 32 ? valid.y : valid.x) >> (key & 31)) & 1u);
                     if (gone || kb + key >= w.r.p0) {
-                        uint8_t* v = ring + st * L::kStage;
+                        uint8_t* v = ring + (stages + st) * L::kStage;
                         constexpr uint32_t kExp = std::is_same<TO, __nv_bfloat16>::value ? 0x7F80u : 0x7C00u;
                         bool found = false;
 #pragma unroll 1
@@ -1329,7 +1327,6 @@ __global__ void __launch_bounds__(kThreads, 1) attn_kernel(const __grid_constant
                 }
             }
             tile0 += nt;
-            item += 2 * nt;
             ++seg;
             __syncwarp();
             if (lane == 0) mbar_arrive(&sh->q_free[buf]);
