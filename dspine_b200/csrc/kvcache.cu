@@ -121,6 +121,36 @@ __device__ __forceinline__ V16 decode16(const uint4& c, float s) {
     return v;
 }
 
+__device__ __forceinline__ uint32_t codes4(float a, float b, float c, float d) {
+    return (uint32_t)__nv_cvt_float2_to_fp8x2(make_float2(a, b), __NV_SATFINITE, __NV_E4M3) |
+           (uint32_t)__nv_cvt_float2_to_fp8x2(make_float2(c, d), __NV_SATFINITE, __NV_E4M3) << 16;
+}
+
+// The codes of x / s, IEEE quotients rounded to e4m3.  In a row of finite values a quotient takes a
+// product with r = 1 / s and two corrections by its exact residual (P. Markstein, "Computation of
+// elementary functions on the IBM RISC System/6000 processor", 1990: with r rounded correctly, the
+// first leaves a quotient off by less than a step, the second rounds that one correctly).  |s|
+// within 2^-100 and 2^100 keeps r normal; where x is so small that its residual is not exact, the
+// quotient is far below half of the smallest code.  The residual is taken as q s - x, so that -0
+// stays -0.
+__device__ __forceinline__ void encode(const V16& v, float s, bool finite, uint32_t (&w)[4]) {
+    float y[16];
+    if (finite && s > 7.8886e-31f && s < 1.2676e30f) {
+        const float r = __frcp_rn(s);
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+            y[i] = __fmul_rn(v.x[i], r);
+            y[i] = __fmaf_rn(-__fmaf_rn(y[i], s, -v.x[i]), r, y[i]);
+            y[i] = __fmaf_rn(-__fmaf_rn(y[i], s, -v.x[i]), r, y[i]);
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < 16; ++i) y[i] = __fdiv_rn(v.x[i], s);
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) w[i] = codes4(y[4 * i], y[4 * i + 1], y[4 * i + 2], y[4 * i + 3]);
+}
+
 __device__ __forceinline__ long long slot_at(const void* slots, int is64, long long n) {
     return is64 ? __ldg(static_cast<const long long*>(slots) + n)
                 : (long long)__ldg(static_cast<const int*>(slots) + n);
@@ -167,17 +197,7 @@ __global__ void __launch_bounds__(kThreads) write_kernel(KvRowsArgs a) {
             const float s = amax > 0.f ? __fdiv_rn(amax, 448.0f) : 1.0f;
             if (ok && live) {
                 uint32_t w[4];
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    uint32_t u = 0;
-#pragma unroll
-                    for (int j = 0; j < 2; ++j) {
-                        const float2 q = make_float2(__fdiv_rn(v.x[4 * i + 2 * j], s),
-                                                     __fdiv_rn(v.x[4 * i + 2 * j + 1], s));
-                        u |= (uint32_t)__nv_cvt_float2_to_fp8x2(q, __NV_SATFINITE, __NV_E4M3) << (16 * j);
-                    }
-                    w[i] = u;
-                }
+                encode(v, s, amax < INFINITY, w);
                 *reinterpret_cast<uint4*>(static_cast<uint8_t*>(is_v ? a.c.v : a.c.k) + at) =
                     make_uint4(w[0], w[1], w[2], w[3]);
                 if (sub == 0) (is_v ? a.c.v_scale : a.c.k_scale)[slot * a.c.scale_stride + h] = s;
