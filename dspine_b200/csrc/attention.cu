@@ -949,14 +949,16 @@ __global__ void __launch_bounds__(kThreads, 1) attn_kernel(const __grid_constant
                     };
 #pragma unroll
                     for (int k = 0; k < DP / 32; ++k) issue(k);
-                    // the next unit's waits while these execute
                     if (last) step_stage();
-                    if (u + 1 < units) ready(u + 1);
+                    // the next unit's waits while these execute; not with a ring of two, where the
+                    // next tile's warp may be waiting for this stage
+                    if (stages > 2 && u + 1 < units) ready(u + 1);
                     if (!ok) break;
 #pragma unroll
                     for (int k = DP / 32; k < DP / 16; ++k) issue(k);
                     mma_commit(s_full + 8 * sb);
                     if (last) mma_commit(empty + 8 * mine);
+                    if (stages <= 2 && u + 1 < units) ready(u + 1);
                 }
             } else {
                 const uint32_t v0 = desc_low(smem_u32(ring + stages * L::kStage), kBlock);
