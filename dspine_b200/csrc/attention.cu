@@ -338,6 +338,9 @@ __device__ __forceinline__ void mma_commit(uint32_t bar) {
         "@one tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}" ::"r"(bar)
         : "memory");
 }
+__device__ __forceinline__ void mbar_arrive_n(uint32_t bar, uint32_t n) {
+    asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(n) : "memory");
+}
 __device__ __forceinline__ void mbar_arrive(uint64_t* bar) {
     asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(bar)) : "memory");
 }
@@ -487,6 +490,76 @@ __device__ __forceinline__ uint32_t chunk_at(int row, int c) {
     return (uint32_t)((c >> 3) * block + row * 128 + (((c ^ row) & 7) << 4));
 }
 
+// Rows of q of a segment into a Q tile, by `warps` warps of which this is `warp`.  bf16, fp16: copies
+// on their way.  e4m3: done on return, as fp16 with a power of two per row, whose inverse goes to mul.
+template <typename TQ, bool kFp8, int DP>
+__device__ __noinline__ void bring_queries(const KernelArgs& a, const Walk& w, uint8_t* dst, float* mul, int warp, int warps) {
+    constexpr int kTileBytes = (DP / 64) * kQBlock;
+    constexpr int kLanes = DP / 8, kAtOnce = 32 / kLanes;       // lanes of a row (16-byte chunks), rows at once
+    constexpr int kRun = 8 * kAtOnce;                           // adjacent rows of a warp
+    const TreeAttnArgs& t = a.t;
+    const int lane = threadIdx.x & 31, sub = lane % kLanes, dr = lane / kLanes;
+    const bool live = sub * 8 < t.c.dim;
+    const int nrows = w.rows(a.qt), row0 = w.first_row(a.qt);
+    const int filled = (nrows + 31) & ~31;                      // whole warps of rows: zeros past the last
+    const int token0 = row0 / t.group, rem0 = row0 - token0 * t.group;
+    const TQ* q = static_cast<const TQ*>(t.q) + (long long)(w.r.lo + token0) * t.q_token_stride +
+                  (long long)(w.h * t.group) * t.q_head_stride + sub * 8;
+    auto place = [&](int r) { return dst + (r >> 7) * kTileBytes + chunk_at<kQBlock>(r & 127, sub); };
+    for (int r0 = warp * kRun + dr; r0 - dr < filled; r0 += warps * kRun) {
+#pragma unroll 4
+        for (int k = 0; k < 8; ++k) {
+            const int r = r0 + k * kAtOnce, i = (int)a.group.divide(rem0 + r);
+            const bool have = r < nrows && live;
+            cp16_or_zero(smem_u32(place(r)), have ? q + i * t.q_token_stride + (rem0 + r - i * t.group) * t.q_head_stride : q, have);
+        }
+    }
+    if constexpr (kFp8) {
+        // to fp16 in place, each lane what it has copied
+        cp_wait_all();
+#pragma unroll 1
+        for (int r0 = warp * kRun + dr; r0 - dr < filled; r0 += warps * kRun) {
+            uint4 x[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) x[i] = *reinterpret_cast<const uint4*>(place(r0 + i * kAtOnce));
+            // the largest size in each row, as bits without the sign (ordered as the values are); all
+            // rows before the first store, so that the shuffles overlap
+            uint32_t top[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const uint32_t sizes = __vmaxu2(__vmaxu2(x[i].x & 0x7FFF7FFFu, x[i].y & 0x7FFF7FFFu),
+                                                __vmaxu2(x[i].z & 0x7FFF7FFFu, x[i].w & 0x7FFF7FFFu));
+                top[i] = max(sizes >> 16, sizes & 0xFFFFu);
+            }
+#pragma unroll
+            for (int o = kLanes / 2; o > 0; o >>= 1) {
+#pragma unroll
+                for (int i = 0; i < 8; ++i) top[i] = max(top[i], __shfl_xor_sync(0xffffffffu, top[i], o));
+            }
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const int r = r0 + i * kAtOnce;
+                float f[8], m, none;
+                unpack2(x[i].x, f[0], f[1], TQ());
+                unpack2(x[i].y, f[2], f[3], TQ());
+                unpack2(x[i].z, f[4], f[5], TQ());
+                unpack2(x[i].w, f[6], f[7], TQ());
+                unpack2(top[i], m, none, TQ());
+                // a power of two that brings the row's largest value to [2^13, 2^14): products
+                // stay exact, and values down to 2^-37 of the largest keep a place in fp16.  A
+                // row with a NaN or an infinity is left as it is: its scores are NaN or infinite
+                int e = (int)(__float_as_uint(m) >> 23) - 127;
+                e = m > 0.f && e < 128 ? max(e, -100) : 13;
+                const float up = __uint_as_float((uint32_t)(13 - e + 127) << 23);
+                if (sub == 0) mul[r] = __uint_as_float((uint32_t)(e - 13 + 127) << 23);
+                *reinterpret_cast<uint4*>(place(r)) =
+                    make_uint4(pack2(f[0] * up, f[1] * up, __half()), pack2(f[2] * up, f[3] * up, __half()),
+                               pack2(f[4] * up, f[5] * up, __half()), pack2(f[6] * up, f[7] * up, __half()));
+            }
+        }
+    }
+}
+
 // A unit is one stream's share of a tile: unit u of a segment belongs to stream u & 1 and uses its
 // score buffer (u >> 1) & 1; its tile is u, or u >> 1 where both streams use every tile.
 
@@ -591,7 +664,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_kernel(const __grid_constant
             mbar_init(&sh->info_empty[i], 1);
         }
         for (int i = 0; i < 2; ++i) {
-            mbar_init(&sh->q_full[i], kFp8 ? 1 : 33);
+            mbar_init(&sh->q_full[i], kFp8 ? kSoftmaxThreads / 32 : 33);
             mbar_init(&sh->q_free[i], 8);
             for (int j = 0; j < 2; ++j) {
                 mbar_init(&sh->s_full[i][j], 1);
@@ -823,77 +896,24 @@ __global__ void __launch_bounds__(kThreads, 1) attn_kernel(const __grid_constant
         if constexpr (kFp8) cp_wait_all();
     } else if (warp == kQueryWarp) {
         // ---------------- queries: the next segment and its rows of q, a segment ahead ------------
+        // (e4m3: the softmax warps bring those of the first)
         Walk& w = sh->walk[1];
         if (lane == 0) w = sh->start;
         __syncwarp();
-        constexpr int kLanes = DP / 8, kAtOnce = 32 / kLanes;   // lanes of a row (16-byte chunks), rows at once
-        const int sub = lane % kLanes, dr = lane / kLanes;
-        const bool live = sub * 8 < t.c.dim;
-        uint32_t seg = 0;
-        bool ok = true;
-        do {
+        uint32_t seg = kFp8 ? 1 : 0;
+        bool ok = true, more = !kFp8 || w.advance(a);
+        while (more) {
             const uint32_t buf = seg % q_bufs;
             ok = wait_at(smem_u32(&sh->q_free[buf]), ((seg / q_bufs) & 1u) ^ 1u, abort);
             if (!ok) break;
             if (lane == 0) sh->seg[buf] = w;
-            const int nrows = w.rows(qt), row0 = w.first_row(qt);
-            const int filled = (nrows + 31) & ~31;              // whole warps of rows: zeros past the last
-            const int token0 = row0 / t.group, rem0 = row0 - token0 * t.group;
-            const TQ* q = static_cast<const TQ*>(t.q) + (long long)(w.r.lo + token0) * t.q_token_stride +
-                          (long long)(w.h * t.group) * t.q_head_stride + sub * 8;
-            uint8_t* dst = sq + buf * L::kQTile;
-            auto source = [&](int r) {
-                const int i = (int)a.group.divide(rem0 + r);
-                return q + i * t.q_token_stride + (rem0 + r - i * t.group) * t.q_head_stride;
-            };
-            if constexpr (!kFp8) {
-#pragma unroll 4
-                for (int r = dr; r < filled; r += kAtOnce) {
-                    const bool have = r < nrows && live;
-                    cp16_or_zero(smem_u32(dst + (r >> 7) * L::kQTile + chunk_at<kQBlock>(r & 127, sub)), have ? source(r) : q, have);
-                }
-                cp_arrive(&sh->q_full[buf]);
-            } else {
-#pragma unroll 1
-                for (int r0 = dr; r0 - dr < filled; r0 += 8 * kAtOnce) {
-                    uint4 x[8];
-#pragma unroll
-                    for (int i = 0; i < 8; ++i) {
-                        const int r = r0 + i * kAtOnce;
-                        x[i] = make_uint4(0, 0, 0, 0);
-                        if (r < nrows && live) x[i] = __ldg(reinterpret_cast<const uint4*>(source(r)));
-                    }
-#pragma unroll
-                    for (int i = 0; i < 8; ++i) {
-                        const int r = r0 + i * kAtOnce;
-                        float f[8];
-                        unpack2(x[i].x, f[0], f[1], TQ());
-                        unpack2(x[i].y, f[2], f[3], TQ());
-                        unpack2(x[i].z, f[4], f[5], TQ());
-                        unpack2(x[i].w, f[6], f[7], TQ());
-                        float m = 0.f;
-#pragma unroll
-                        for (int j = 0; j < 8; ++j) m = fmaxf(m, fabsf(f[j]));
-#pragma unroll
-                        for (int o = kLanes / 2; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-                        // a power of two that brings the row's largest value to [2^13, 2^14): products
-                        // stay exact, and values down to 2^-37 of the largest keep a place in fp16
-                        int e = (int)(__float_as_uint(m) >> 23) - 127;
-                        e = m > 0.f && e < 128 ? max(e, -100) : 13;
-                        const float up = __uint_as_float((uint32_t)(13 - e + 127) << 23);
-                        if (r < filled) {
-                            if (sub == 0) row_mul[buf * kRows + r] = __uint_as_float((uint32_t)(e - 13 + 127) << 23);
-                            *reinterpret_cast<uint4*>(dst + (r >> 7) * L::kQTile + chunk_at<kQBlock>(r & 127, sub)) =
-                                make_uint4(pack2(f[0] * up, f[1] * up, __half()), pack2(f[2] * up, f[3] * up, __half()),
-                                           pack2(f[4] * up, f[5] * up, __half()), pack2(f[6] * up, f[7] * up, __half()));
-                        }
-                    }
-                }
-            }
+            bring_queries<TQ, kFp8, DP>(a, w, sq + buf * L::kQTile, row_mul + buf * kRows, 0, 1);
+            if constexpr (!kFp8) cp_arrive(&sh->q_full[buf]);
             __syncwarp();
-            if (lane == 0) mbar_arrive(&sh->q_full[buf]);
+            if (lane == 0) mbar_arrive_n(smem_u32(&sh->q_full[buf]), kFp8 ? kSoftmaxThreads / 32 : 1);
             ++seg;
-        } while (w.advance(a));
+            more = w.advance(a);
+        }
         if constexpr (!kFp8) cp_wait_all();
     } else if (warp == kScoreWarp || warp == kAccumWarp) {
         // ---------------- MMA issuers: one warp for S = Q K^T, one for O += P V ----------------
@@ -1008,6 +1028,14 @@ __global__ void __launch_bounds__(kThreads, 1) attn_kernel(const __grid_constant
             ok = __all_sync(0xffffffffu, ok && wait_or_abort(&sh->joined, jp & 1u, abort));
             ++jp;
         };
+        if constexpr (kFp8) {
+            // The first segment's queries.  The query warp alone took 19 thousand cycles for 128 rows
+            // with the loaders' copies in front of its own.
+            if (tid == 0) sh->seg[0] = sh->start;
+            bring_queries<TQ, kFp8, DP>(a, sh->start, sq, row_mul, warp, kSoftmaxThreads / 32);
+            __syncwarp();
+            if (lane == 0) mbar_arrive_n(smem_u32(&sh->q_full[0]), 1);
+        }
         do {
             const uint32_t buf = seg % q_bufs;
             ok = wait_at(smem_u32(&sh->q_full[buf]), (seg / q_bufs) & 1u, abort);
