@@ -266,6 +266,7 @@ struct alignas(16) Shared {
     uint64_t s_full[2][2];           // scores of a stream's buffer in TMEM
     uint64_t p_full[2][2];           // weights of a stream's buffer in TMEM
     uint64_t s_free[2][2];           // the weights in a stream's buffer have been accumulated
+    uint64_t described;              // the segment's walk is there, its Q is not yet
     uint64_t o_full;                 // the segment's accumulators are complete
     uint64_t joined;                 // both warpgroups have written what the other reads
     uint64_t drain[2];
@@ -490,8 +491,8 @@ __device__ __forceinline__ uint32_t chunk_at(int row, int c) {
     return (uint32_t)((c >> 3) * block + row * 128 + (((c ^ row) & 7) << 4));
 }
 
-// Rows of q of a segment into a Q tile, by `warps` warps of which this is `warp`.  bf16, fp16: copies
-// on their way.  e4m3: done on return, as fp16 with a power of two per row, whose inverse goes to mul.
+// Rows of q of a segment into a Q tile, by `warps` warps of which this is `warp`.  e4m3: as fp16 with a
+// power of two per row, whose inverse goes to mul.
 template <typename TQ, bool kFp8, int DP>
 __device__ __noinline__ void bring_queries(const KernelArgs& a, const Walk& w, uint8_t* dst, float* mul, int warp, int warps) {
     constexpr int kTileBytes = (DP / 64) * kQBlock;
@@ -514,9 +515,9 @@ __device__ __noinline__ void bring_queries(const KernelArgs& a, const Walk& w, u
             cp16_or_zero(smem_u32(place(r)), have ? q + i * t.q_token_stride + (rem0 + r - i * t.group) * t.q_head_stride : q, have);
         }
     }
+    cp_wait_all();
     if constexpr (kFp8) {
         // to fp16 in place, each lane what it has copied
-        cp_wait_all();
 #pragma unroll 1
         for (int r0 = warp * kRun + dr; r0 - dr < filled; r0 += warps * kRun) {
             uint4 x[8];
@@ -664,7 +665,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_kernel(const __grid_constant
             mbar_init(&sh->info_empty[i], 1);
         }
         for (int i = 0; i < 2; ++i) {
-            mbar_init(&sh->q_full[i], kFp8 ? kSoftmaxThreads / 32 : 33);
+            mbar_init(&sh->q_full[i], kSoftmaxThreads / 32);
             mbar_init(&sh->q_free[i], 8);
             for (int j = 0; j < 2; ++j) {
                 mbar_init(&sh->s_full[i][j], 1);
@@ -673,6 +674,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_kernel(const __grid_constant
             }
             mbar_init(&sh->drain[i], 1);
         }
+        mbar_init(&sh->described, 1);
         mbar_init(&sh->o_full, 1);
         mbar_init(&sh->joined, 8);
         sh->abort = 0;
@@ -896,25 +898,25 @@ __global__ void __launch_bounds__(kThreads, 1) attn_kernel(const __grid_constant
         if constexpr (kFp8) cp_wait_all();
     } else if (warp == kQueryWarp) {
         // ---------------- queries: the next segment and its rows of q, a segment ahead ------------
-        // (e4m3: the softmax warps bring those of the first)
+        // (the softmax warps bring the first segment's, and all where there is no room for two)
         Walk& w = sh->walk[1];
         if (lane == 0) w = sh->start;
         __syncwarp();
-        uint32_t seg = kFp8 ? 1 : 0;
-        bool ok = true, more = !kFp8 || w.advance(a);
-        while (more) {
+        uint32_t seg = 1;
+        while (w.advance(a)) {
             const uint32_t buf = seg % q_bufs;
-            ok = wait_at(smem_u32(&sh->q_free[buf]), ((seg / q_bufs) & 1u) ^ 1u, abort);
-            if (!ok) break;
+            if (!wait_at(smem_u32(&sh->q_free[buf]), ((seg / q_bufs) & 1u) ^ 1u, abort)) break;
             if (lane == 0) sh->seg[buf] = w;
-            bring_queries<TQ, kFp8, DP>(a, w, sq + buf * L::kQTile, row_mul + buf * kRows, 0, 1);
-            if constexpr (!kFp8) cp_arrive(&sh->q_full[buf]);
+            if (q_bufs > 1) bring_queries<TQ, kFp8, DP>(a, w, sq + buf * L::kQTile, row_mul + buf * kRows, 0, 1);
             __syncwarp();
-            if (lane == 0) mbar_arrive_n(smem_u32(&sh->q_full[buf]), kFp8 ? kSoftmaxThreads / 32 : 1);
+            if (lane == 0) {
+                if (q_bufs > 1)
+                    mbar_arrive_n(smem_u32(&sh->q_full[buf]), kSoftmaxThreads / 32);
+                else
+                    mbar_arrive(&sh->described);
+            }
             ++seg;
-            more = w.advance(a);
         }
-        if constexpr (!kFp8) cp_wait_all();
     } else if (warp == kScoreWarp || warp == kAccumWarp) {
         // ---------------- MMA issuers: one warp for S = Q K^T, one for O += P V ----------------
         // Two, because a unit costs the issuing warp more in waits, commits and issue than the
@@ -1028,16 +1030,21 @@ __global__ void __launch_bounds__(kThreads, 1) attn_kernel(const __grid_constant
             ok = __all_sync(0xffffffffu, ok && wait_or_abort(&sh->joined, jp & 1u, abort));
             ++jp;
         };
-        if constexpr (kFp8) {
-            // The first segment's queries.  The query warp alone took 19 thousand cycles for 128 rows
-            // with the loaders' copies in front of its own.
-            if (tid == 0) sh->seg[0] = sh->start;
-            bring_queries<TQ, kFp8, DP>(a, sh->start, sq, row_mul, warp, kSoftmaxThreads / 32);
-            __syncwarp();
-            if (lane == 0) mbar_arrive_n(smem_u32(&sh->q_full[0]), 1);
-        }
         do {
             const uint32_t buf = seg % q_bufs;
+            if (seg == 0 || q_bufs == 1) {
+                // Queries that could not be brought ahead: by eight warps, as copies behind those of the
+                // loaders are slow to issue (one warp took 27 thousand cycles for 256 rows)
+                if (seg == 0) {
+                    if (tid == 0) sh->seg[0] = sh->start;
+                } else {
+                    ok = wait_at(smem_u32(&sh->described), (seg - 1) & 1u, abort);
+                    if (!ok) break;
+                }
+                bring_queries<TQ, kFp8, DP>(a, seg == 0 ? sh->start : sh->seg[0], sq, row_mul, warp, kSoftmaxThreads / 32);
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&sh->q_full[0]);
+            }
             ok = wait_at(smem_u32(&sh->q_full[buf]), (seg / q_bufs) & 1u, abort);
             if (!ok) break;
             const Walk& w = sh->seg[buf];
