@@ -952,10 +952,12 @@ __global__ void __launch_bounds__(kThreads, 1) attn_kernel(const __grid_constant
                 const uint32_t q0 = desc_low(smem_u32(sq + buf * L::kQTile), 16), k0 = desc_low(smem_u32(ring), 16);
                 auto ready = [&](int u) {                    // K tile and score buffer of unit u
                     const uint32_t s = u & 1, sb = (s << 1) | ((u >> 1) & 1);
-                    if (!(s & step)) ok = wait_at(full + 8 * st, sp, abort);
+                    if (!(s & step)) {
+                        ok = wait_at(full + 8 * st, sp, abort);
+                        fence_proxy_async_smem();
+                    }
                     ok = ok && wait_at(s_free + 8 * sb, ((ph >> sb) & 1u) ^ 1u, abort);
                     ph ^= 1u << sb;
-                    fence_proxy_async_smem();
                     tc_fence_after();
                 };
                 ready(0);
@@ -991,7 +993,8 @@ __global__ void __launch_bounds__(kThreads, 1) attn_kernel(const __grid_constant
                     ok = ok && wait_at(p_full + 8 * sb, (ph >> sb) & 1u, abort);
                     if (!ok) break;
                     ph ^= 1u << sb;
-                    fence_proxy_async_smem();
+                    // V, and the zeros that each warpgroup has put into all of it; so once a tile
+                    if (!(s & step)) fence_proxy_async_smem();
                     tc_fence_after();
                     const uint32_t vb = v0 + st * (L::kStage >> 4), d = tmem + 256 + s * 128, p = tmem + sb * kTile;
 #pragma unroll
