@@ -92,13 +92,11 @@ class TreeAccept:
 
     @staticmethod
     def allocate(batch: int, width: int, device, *, slots=True) -> "TreeAccept":
-        """Outputs for `batch` requests, parts of two allocations."""
-        n = batch * width
-        bonus, output = torch.empty(batch + n, dtype=torch.int64, device=device).split((batch, n))
-        small = torch.empty(3 * batch + (2 if slots else 1) * n, dtype=torch.int32, device=device)
-        accept, commit, new_seq, path, *kept = small.split((batch, batch, batch, n, n) if slots else (batch, batch, batch, n))
-        shape = (batch, width)
-        return TreeAccept(accept, commit, bonus, output.view(shape), path.view(shape), kept[0].view(shape) if slots else None, new_seq)
+        """Outputs for `batch` requests."""
+        accept, commit, new_seq = torch.empty((3, batch), dtype=torch.int32, device=device).unbind()
+        path, *kept = torch.empty((2 if slots else 1, batch, width), dtype=torch.int32, device=device).unbind()
+        return TreeAccept(accept, commit, torch.empty(batch, dtype=torch.int64, device=device),
+                          torch.empty((batch, width), dtype=torch.int64, device=device), path, kept[0] if slots else None, new_seq)
 
     def _check(self, batch, width, dev, slots):
         for x, shape, dtype in ((self.accept, (batch,), torch.int32), (self.commit, (batch,), torch.int32), (self.bonus, (batch,), torch.int64),
