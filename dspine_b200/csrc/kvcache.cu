@@ -9,9 +9,13 @@
 //   write_kernel  one group of lanes per (token, head) row, 16 elements per lane
 //   read_kernel   the inverse: code * s in fp32, rounded once to the output type
 //
-// Both are bound by memory (a row is read once and written once).  A lane holds 16 elements
-// because 16 codes are one 16-byte access of the cache: the widest there is, and rows of 128
-// elements then need 8 lanes, so a warp moves 4 rows at a time.
+// A row is read once and written once.  A lane holds 16 elements because 16 codes are one 16-byte
+// access of the cache: the widest there is, and rows of 128 elements then need 8 lanes, so a warp
+// moves 4 rows at a time.  Measured with 8 heads of 128, e4m3, bf16 rows: 131072 tokens read in
+// 147 us (5.5 TB/s, bound by memory); 32749 written in 51.5 us (4.0 TB/s, bound by issue: 318
+// instructions for the 16 elements of a lane, schedulers 75% busy.  The next row's loads ahead of this
+// one's arithmetic took the same time; arithmetic on pairs took fewer instructions but more
+// registers, 53 us).
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_fp8.h>

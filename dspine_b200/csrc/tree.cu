@@ -9,7 +9,9 @@
 //
 //   accept_kernel   one warp per request, two nodes per lane: the agreement of all nodes is one
 //                   64-bit ballot, after which "all ancestors agree" is one AND per node, so no
-//                   walk over the tree is needed.  The cost is the latency of two dependent loads.
+//                   walk over the tree is needed.  The cost is the latency of two dependent loads: 256
+//                   trees of up to 64 nodes take as long as 4 of 16 (26 us as called from Python,
+//                   nearly all of it the host's).
 #include <cuda_runtime.h>
 #include <stdint.h>
 

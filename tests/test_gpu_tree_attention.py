@@ -126,6 +126,23 @@ def test_long_chains(width, length, cache):
     c.check(c.run())
 
 
+@pytest.mark.parametrize("most,tree", [(3, False), (64, True)])
+@pytest.mark.parametrize("cache,page", [("bf16", 16), ("e4m3", 1)])
+def test_many_short_segments(cache, page, most, tree):
+    """More requests than CTAs have room for at once: every CTA goes from segment to segment, and every
+    wait of every call has to end."""
+    g = torch.Generator().manual_seed(most)
+    widths = torch.randint(0, most + 1, (90,), generator=g).tolist()
+    lengths = [w + int(n) for w, n in zip(widths, torch.randint(0, 200, (90,), generator=g))]
+    c = Case(widths, lengths, heads=32, kv_heads=8, dim=128, page=page, cache=cache, tree=tree, seed=most)
+    want, err = c.want(), torch.zeros(1, dtype=torch.int32, device="cuda")
+    a, k = c.args()
+    for _ in range(20):
+        got = attention.tree_attention(*a, **k, max_width=most, err=err)
+    assert int(err) == 0
+    c.check(got, want)
+
+
 def test_the_layout_bound_does_not_change_what_is_computed():
     c = Case([40, 2, 17], [300, 700, 17], heads=16, kv_heads=2, dim=64, seed=4)
     want = c.want()
