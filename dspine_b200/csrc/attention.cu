@@ -56,11 +56,13 @@
 //       warps' exponentials (a unit of 64 keys: 1700 cycles, 512 of them at least for the ex2 of its
 //       warp, twice for two warps a scheduler; its matrix instructions: 640)
 //   64 requests x 16 tokens, up to 4096 cached, e4m3, pages of 1    245 us, and 1 x 16 tokens, 131071
-//       cached, 4 KV heads 86 us: shared memory, which for each tile of 64 keys takes the codes, their
-//       conversion to fp16, Q, K and V for the matrix instructions and the scales for every
-//       softmax warp, about 1400 cycles of the 1800 to 2100 that a tile takes
-//   1 request x 1 token, 333 cached                                 24 us as called from Python, of which
-//       the kernels take 8
+//       cached, 4 KV heads 86 us: the loaders' conversion (two warps for K, two for V: 1550 cycles a
+//       tile of the 1800 to 2100 that one takes), beside it the integer pipe (half busy) and shared
+//       memory (970 wavefronts a tile by its threads, 510 more for the matrix operands).  64 x 16 loses a fifth
+//       to segment switches besides
+//   1 request x 1 token, 333 cached                                 24 us as called from Python, 19 of them in
+//       attn_kernel when its code comes from a cold cache: the chain of waits from the plan to the
+//       join
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_fp8.h>
