@@ -61,7 +61,7 @@ def tree_attention(q, k_cache, v_cache, page_table, kv_lens, *, page_size=1, q_i
     multiple of kv_heads.  Request b owns rows [q_indptr[b], q_indptr[b+1]) (int32 [B+1]; None:
     rows / B each) and kv_lens[b] (int32) cached positions, its drafted tokens the last of them:
     their K and V are written before the call.  Position p is slot page_table[b, p // page_size]
-    * page_size + p % page_size (page_table int32 [B, pages]).
+    * page_size + p % page_size (page_table int32 [B, pages], pages * page_size < 2^31 - 255).
 
     Row i of a request sees every position before its drafted tokens, and drafted token j where
     bit j of tree_mask[row] (int64 [rows]) is set, or without a tree_mask where j <= i.  The result is

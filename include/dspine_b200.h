@@ -464,7 +464,8 @@ int dsv_kv_read(int64_t tokens, const void* slots, int32_t slots_int64, const ds
  * nothing gets zeros and -inf.  Query head hq reads KV head hq / (q_heads / heads)
  * (at most 4096 of them each).
  * dtype (q and out) DSV_BF16 or DSV_F16; the cache has the same type or is e4m3; dim a multiple
- * of 16, at most 128; cache->slots a multiple of page_size; scale positive and finite.  `width`
+ * of 16, at most 128; cache->slots a multiple of page_size; max_pages * page_size at most
+ * 0x7fffff00; scale positive and finite.  `width`
  * is with q_indptr a bound on the rows of a request, by which the work is laid out (a request
  * with more rows is computed all the same).
  * Bits of *err (a device word, may be NULL): bit 1: a page outside the cache, or a length above

@@ -225,3 +225,16 @@ def test_c_entries_refuse_before_launch(lib):
         assert tree(**bad) == 1, bad
     assert tree(tokens=None) == 3 and tree(slots=None) == 3 and tree(out=None) == 3
     assert tree(tokens=12) == 4 and tree(out=12) == 4 and tree(ind=18) == 4
+
+
+def test_positions_near_the_end_of_32_bits_are_refused(lib):
+    """A tile past the last position would not be told from one at its start."""
+    c = _lib.KvCache(k=16, v=16, k_scale=None, v_scale=None, slots=64, slot_stride=128, head_stride=64, scale_stride=2, heads=2,
+                     dim=64, dtype=0)
+
+    def attend(pages, page):
+        return lib.dsv_tree_attention(1, 1, 4, 0, 16, 256, 64, c, 16, pages, pages, page, 16, 16, 1, None, 0.1, 16, 256, 64, None,
+                                      None, 16, 0, None)
+
+    assert attend((1 << 27) - 1, 16) == 1 and attend((1 << 31) - 1, 1) == 1
+    assert attend((1 << 27) - 16, 16) == 6                  # the positions are taken: the workspace is too small
