@@ -133,13 +133,13 @@ __device__ __forceinline__ uint32_t codes4(float a, float b, float c, float d) {
 // The codes of x / s, IEEE quotients rounded to e4m3.  In a row of finite values a quotient takes a
 // product with r = 1 / s and two corrections by its exact residual (P. Markstein, "Computation of
 // elementary functions on the IBM RISC System/6000 processor", 1990: with r rounded correctly, the
-// first leaves a quotient off by less than a step, the second rounds that one correctly).  |s|
-// within 2^-100 and 2^100 keeps r normal; where x is so small that its residual is not exact, the
-// quotient is far below half of the smallest code.  The residual is taken as q s - x, so that -0
+// first leaves a quotient off by less than a step, the second rounds that one correctly).  s
+// within 2^-60 and 2^100 keeps r normal and the residuals of all quotients from 2^-42 on exact (they
+// are multiples of 2^-47 s y); smaller ones are far below half of the smallest code, 2^-10.  The residual is taken as q s - x, so that -0
 // stays -0.
 __device__ __forceinline__ void encode(const V16& v, float s, bool finite, uint32_t (&w)[4]) {
     float y[16];
-    if (finite && s > 7.8886e-31f && s < 1.2676e30f) {
+    if (finite && s > 8.6737e-19f && s < 1.2676e30f) {
         const float r = __frcp_rn(s);
 #pragma unroll
         for (int i = 0; i < 16; ++i) {

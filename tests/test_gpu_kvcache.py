@@ -100,6 +100,27 @@ def test_random_fp32_rows_are_quantised_like_the_rule():
         assert torch.equal(scale.cpu(), scales) and torch.equal(_codes(cache), codes.view(torch.uint8))
 
 
+@pytest.mark.parametrize("kind", ["bf16", "fp32"])
+def test_rows_of_every_size_are_quantised_like_the_rule(kind):
+    """Row maxima from the smallest subnormals to the largest values: scales on every side of the
+    range in which quotients come from a reciprocal, and quotients down to nothing."""
+    g = torch.Generator().manual_seed(12)
+    powers = torch.arange(-150, 127).repeat_interleave(8).double()
+    n = len(powers)
+    x = torch.randn(n, 1, 128, generator=g).double().clamp(-1.9, 1.9)
+    x = x * torch.exp2(powers[:, None, None] - 12 * torch.rand(x.shape, generator=g).double())
+    x = x.float().to(TYPES[kind])
+    kc, vc, ks, vs = kvcache.allocate_kv(n, 1, 128, dtype=E4M3)
+    kvcache.write_kv(x.cuda(), -x.cuda(), kc, vc, torch.arange(n, device="cuda"), k_scale=ks, v_scale=vs)
+    for y, cache, scale in ((x, kc, ks), (-x, vc, vs)):
+        codes, scales = quantise(y)
+        assert torch.equal(scale.cpu(), scales)
+        got, want = _codes(cache), codes.view(torch.uint8)
+        # a scale that underflows to 0 makes 0 / 0, a NaN whose sign IEEE leaves open (0x7F and 0xFF are both NaN)
+        both_nan = ((got & 0x7F) == 0x7F) & ((want & 0x7F) == 0x7F)
+        assert bool(((got == want) | both_nan).all())
+
+
 def test_rows_with_nan_infinity_and_tiny_values():
     x = torch.zeros(6, 1, 32)
     x[0, 0, 3], x[0, 0, 4] = math.nan, 2.0                 # scale 1, the NaN stays one

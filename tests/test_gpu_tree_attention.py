@@ -143,6 +143,17 @@ def test_many_short_segments(cache, page, most, tree):
     c.check(got, want)
 
 
+@pytest.mark.parametrize("tree", [False, True])
+def test_more_requests_than_threads(tree):
+    """1100 requests, some without rows, some with fewer cached positions than rows."""
+    g = torch.Generator().manual_seed(5)
+    widths = torch.randint(0, 4, (1100,), generator=g).tolist()
+    lengths = torch.randint(0, 150, (1100,), generator=g).tolist()
+    lengths[7], widths[7], lengths[8], widths[8] = 0, 3, 2, 3
+    c = Case(widths, lengths, heads=2, kv_heads=2, dim=16, page=4, tree=tree, seed=5)
+    c.check(c.run())
+
+
 def test_the_layout_bound_does_not_change_what_is_computed():
     c = Case([40, 2, 17], [300, 700, 17], heads=16, kv_heads=2, dim=64, seed=4)
     want = c.want()
