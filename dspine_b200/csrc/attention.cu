@@ -60,9 +60,8 @@
 //       tile of the 1800 to 2100 that one takes), beside it the integer pipe (half busy) and shared
 //       memory (970 wavefronts a tile by its threads, 510 more for the matrix operands).  64 x 16 loses a fifth
 //       to segment switches besides
-//   1 request x 1 token, 333 cached                                 24 us as called from Python, 19 of them in
-//       attn_kernel when its code comes from a cold cache: the chain of waits from the plan to the
-//       join
+//   1 request x 1 token, 333 cached                                 24 us a call from Python, the host's time (19 us
+//       in attn_kernel when all caches are cold: the chain of waits from the plan to the join)
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_fp8.h>
