@@ -810,11 +810,18 @@ __global__ void __launch_bounds__(kThreads, 1) attn_kernel(const __grid_constant
                 const uint8_t* from = own + r * L::kRawTile;
                 uint8_t* dst = stage0 + s * L::kStage;
                 if (live) {
+                    uint4 next4[4];                             // loads ahead of the stores of those before
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) next4[k] = *reinterpret_cast<const uint4*>(from + k * kAtOnce * DP);
 #pragma unroll 1
                     for (int k0 = 0; k0 < kSteps; k0 += 4) {
-                        uint4 x[4];                             // all loads before the first store
+                        uint4 x[4];
 #pragma unroll
-                        for (int k = 0; k < 4; ++k) x[k] = *reinterpret_cast<const uint4*>(from + (k0 + k) * kAtOnce * DP);
+                        for (int k = 0; k < 4; ++k) x[k] = next4[k];
+                        if (k0 + 4 < kSteps) {
+#pragma unroll
+                            for (int k = 0; k < 4; ++k) next4[k] = *reinterpret_cast<const uint4*>(from + (k0 + 4 + k) * kAtOnce * DP);
+                        }
 #pragma unroll
                         for (int k = 0; k < 4; ++k) {
                             const int row = row0 + (k0 + k) * kAtOnce;
