@@ -708,7 +708,11 @@ __global__ void __launch_bounds__(kThreads, 1) attn_kernel(const __grid_constant
     __syncthreads();
     tc_fence_after();
     constexpr uint32_t tmem = 0;                           // all 512 columns were allocated
-    if (warp >= kFirstLoader) {
+    // Up to 64 rows only the softmax warps of schedulers 0 and 1 have any: the loaders there change
+    // places with the index and the query warp (64 x 16 e4m3, 64 rows: 243.2 us from 246.0; 64 x 1 bf16, 4 rows:
+    // 215.3 from 216.0).  With more rows they would meet on schedulers 2 and 3 alone.
+    const int role = t.group * t.width <= 64 && warp >= kIndexWarp && warp < kFirstLoader + 2 ? warp ^ 6 : warp;
+    if (role >= kFirstLoader) {
         // ---------------- loaders: rows of K and V by 16-byte copies of the lanes -----------------
         // Two warps for K tiles, two for V, every other tile each.  fp16, bf16: straight into the
         // swizzled stage.  e4m3: as codes into a raw tile of its own, the next one's on the way
@@ -716,7 +720,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_kernel(const __grid_constant
         // Copies of a lane, not TMA: one warp of them reaches 5.6 TB/s, two 6.7, whatever the page
         // size; gathers of four rows and bulk copies of one stay at 2.2 and 1.3 (scattered rows of
         // 256 bytes, nothing else running).
-        const int lw = warp - kFirstLoader;
+        const int lw = role - kFirstLoader;
         constexpr int kElem = kFp8 ? 1 : 2;                     // bytes of a cached element
         const uint32_t stride = (uint32_t)t.c.slot_stride * (uint32_t)kElem;   // bytes from slot to slot
         constexpr int kLanes = DP * kElem / 16, kAtOnce = 32 / kLanes;         // lanes of a row, rows at once
@@ -851,7 +855,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_kernel(const __grid_constant
             }
         }
         cp_wait_all();
-    } else if (warp == kIndexWarp) {
+    } else if (role == kIndexWarp) {
         // ---------------- index: slots, scales and validity of the tiles to come ----------------
         Walk& w = sh->walk[0];
         if (lane == 0) w = sh->start;
@@ -920,7 +924,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_kernel(const __grid_constant
             }
         } while (ok && w.advance(a));
         if constexpr (kFp8) cp_wait_all();
-    } else if (warp == kQueryWarp) {
+    } else if (role == kQueryWarp) {
         // ---------------- queries: the next segment and its rows of q, a segment ahead ------------
         // (the softmax warps bring the first segment's, and all where there is no room for two)
         Walk& w = sh->walk[1];
