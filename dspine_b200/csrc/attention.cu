@@ -55,9 +55,9 @@
 //   16 requests x trees of up to 64, 64 query heads, up to 16384    365 us, 0.62 PFLOP/s: the softmax
 //       warps' exponentials (a unit of 64 keys: 1700 cycles, 512 of them at least for the ex2 of its
 //       warp, twice for two warps a scheduler; its matrix instructions: 640)
-//   64 requests x 16 tokens, up to 4096 cached, e4m3, pages of 1    245 us, and 1 x 16 tokens, 131071
-//       cached, 4 KV heads 86 us: the loaders' conversion (two warps for K, two for V: 1550 cycles a
-//       tile of the 1800 to 2100 that one takes), beside it the integer pipe (half busy) and shared
+//   64 requests x 16 tokens, up to 4096 cached, e4m3, pages of 1    243 us, and 1 x 16 tokens, 131071
+//       cached, 4 KV heads 84 us: the loaders' conversion (two warps for K, two for V: 1500 cycles a
+//       tile of the 1750 to 2100 that one takes), beside it the integer pipe (half busy) and shared
 //       memory (970 wavefronts a tile by its threads, 510 more for the matrix operands).  64 x 16 loses a fifth
 //       to segment switches besides
 //   1 request x 1 token, 333 cached                                 24 us a call from Python, the host's time (19 us
