@@ -652,7 +652,8 @@ int dsv_tree_attention(int32_t batch, int64_t rows, int32_t q_heads, int32_t dty
     if (a.c.dtype != DSV_E4M3 && a.c.dtype != dtype) return DSV_BAD_DTYPE;
     if (batch < 0 || rows < 0 || rows > 0x7fffffff || q_heads < 1 || q_heads % a.c.heads != 0 ||
         page_size < 1 || a.c.slots % page_size != 0 || max_pages < 0 || table_stride < max_pages ||
-        width < 1 || (int64_t)max_pages * page_size > 0x7fffff00 || q_heads / a.c.heads > 4096)
+        width < 1 || (int64_t)max_pages * page_size > 0x7fffff00 || q_heads / a.c.heads > 4096 ||
+        rows * (q_heads / a.c.heads) > 0x7fffff00)
         return DSV_BAD_SHAPE;
     if (q_indptr == nullptr && rows != (int64_t)batch * width) return DSV_BAD_SHAPE;
     if (tree_mask != nullptr && q_indptr == nullptr && width > 64) return DSV_BAD_SHAPE;

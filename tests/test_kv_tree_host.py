@@ -238,3 +238,15 @@ def test_positions_near_the_end_of_32_bits_are_refused(lib):
 
     assert attend((1 << 27) - 1, 16) == 1 and attend((1 << 31) - 1, 1) == 1
     assert attend((1 << 27) - 16, 16) == 6                  # the positions are taken: the workspace is too small
+
+
+def test_rows_of_queries_past_32_bits_are_refused(lib):
+    c = _lib.KvCache(k=16, v=16, k_scale=None, v_scale=None, slots=64, slot_stride=16, head_stride=16, scale_stride=1, heads=1,
+                     dim=16, dtype=0)
+
+    def attend(rows, heads):
+        return lib.dsv_tree_attention(1, rows, heads, 0, 16, 16, 16, c, 16, 4, 4, 16, 16, 16, 1, None, 0.1, 16, 16, 16, None, None,
+                                      16, 0, None)
+
+    assert attend(1 << 30, 2) == 1 and attend((1 << 31) - 1, 1) == 1 and attend(1 << 20, 4096) == 1
+    assert attend((1 << 30) - 128, 2) == 6                  # taken: the workspace is too small
