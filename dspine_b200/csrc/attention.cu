@@ -41,8 +41,17 @@
 //
 // e4m3 caches: codes are exact in fp16, so they are converted between two rings in shared memory
 // and the matrix instructions run on fp16.  q goes to fp16 with a power of two per row.  K
-// scales multiply the scores; V scales multiply the weights, and the reference moves by the running
-// maximum of the V scales (a power of two) so that weight x scale stays within fp16.
+// scales multiply the scores; V scales multiply the weights.  The products are what is rounded to
+// fp16, so the reference follows the row's largest product: the maximum, over the keys that the row
+// sees, of s c + e, 2^e the first power of two above the key's V scale.  Where the V scales of a tile
+// lie within 2^kNear of each other and of the last tile's (nearly always; one vote), one e serves for
+// all its keys, at most kNear too large, so that the row's largest product lies in [2, 2^14]: products
+// keep fp16's full precision down to 2^-15 of it and are off by at most 2^-26 of it below.  Other
+// tiles take an e a key, in a function of its own (far_unit).  e is held within [-90, 120], so that
+// sums of the weights themselves stay within fp32.
+//
+// A near tile costs what it did with one e for the whole context (64 x 16 245 us, 1 x 16 long 87 from 84: the
+// rare forms are calls, as any code beside the loop slowed it, run or not; an e a key for every tile: 277 and 93).
 //
 // Masked positions: scores of unseen keys are replaced by -inf, rows of unreadable positions are
 // zeros in shared memory.  A V element of a drafted token that is not finite would reach rows that
@@ -88,6 +97,10 @@ constexpr int kSoftmaxThreads = 256;
 // positions (8 items of 6 tiles): 1 tile 16.9 us, 2 16.4, 4 18.4, 8 23.5
 constexpr int kMinTiles = 2;
 constexpr float kSlack = 8.0f;             // log2 by which a maximum may outgrow the reference
+constexpr int kNear = 4;                   // e4m3: powers of two between V scales that one e serves
+constexpr int kFar = 0x10000;              // a biased exponent near to none
+constexpr int kSpan = 60;                  // see far_unit
+constexpr float kReach = 120.0f, kFarthest = 400.0f;   // log2 of a step of scaling; beyond kFarthest nothing is left in any case
 constexpr float kL2E = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
 
@@ -290,6 +303,7 @@ struct alignas(16) Shared {
     uint32_t tmem;
     int abort;
     int odd[2];                      // a drafted V element was not finite (by segment parity)
+    int e_eff[8];                    // e4m3, a softmax warp each: see far_unit
     int v_done[2];                   // e4m3: V tiles (even, odd) in their stages, as one past the last
     long long scan[32];
     Walk start;                      // where this CTA starts on the line of tiles
@@ -383,6 +397,14 @@ __device__ __forceinline__ void tmem_wait_ld(uint32_t (&r)[32]) {
     asm volatile("tcgen05.wait::ld.sync.aligned;" : DSV_R16(DSV_IO, 0), DSV_R16(DSV_IO, 16)::"memory");
 #undef DSV_IO
 }
+// 8 columns, and the wait for them
+__device__ __forceinline__ void tmem_ld8(uint32_t taddr, uint32_t (&r)[8]) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];\n\ttcgen05.wait::ld.sync.aligned;"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7])
+        : "r"(taddr)
+        : "memory");
+}
 __device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t (&r)[32]) {
 #define DSV_IN(y) "r"(y)
@@ -399,6 +421,16 @@ __device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&r)[16
         "r"(taddr)
         : "memory");
 #undef DSV_IN
+}
+__device__ __forceinline__ void tmem_st8(uint32_t taddr, const uint32_t (&r)[8]) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%8], {%0, %1, %2, %3, %4, %5, %6, %7};\n\ttcgen05.wait::st.sync.aligned;" ::"r"(r[0]),
+                 "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(taddr)
+                 : "memory");
+}
+__device__ __forceinline__ void tmem_st4(uint32_t taddr, const uint32_t (&r)[4]) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x4.b32 [%4], {%0, %1, %2, %3};\n\ttcgen05.wait::st.sync.aligned;" ::"r"(r[0]), "r"(r[1]),
+                 "r"(r[2]), "r"(r[3]), "r"(taddr)
+                 : "memory");
 }
 #undef DSV_R16
 
@@ -576,6 +608,159 @@ __device__ __noinline__ void bring_queries(const KernelArgs& a, const Walk& w, u
             }
         }
     }
+}
+
+// columns [c, end) of this thread's TMEM lane times f
+__device__ __noinline__ void scale_columns(uint32_t taddr, int c, int end, float f) {
+#pragma unroll 1
+    for (; c < end; c += 8) {
+        uint32_t x[8];
+        tmem_ld8(taddr + c, x);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) x[i] = __float_as_uint(__uint_as_float(x[i]) * f);
+        tmem_st8(taddr + c, x);
+    }
+}
+
+// e4m3: of two accumulators 128 columns apart the one with the lower reference (by kReach to kFarthest) is
+// scaled towards the other, in columns [c, end)
+__device__ __noinline__ float4 bring_nearer(uint32_t taddr, int c, int end, float2 x, float2 y) {
+    for (int k = 0; k < 3; ++k) {
+        const float apart = x.x - y.x, by = 7.5231638e-37f;     // 2^-120
+        const bool low_x = apart < -kReach && apart > -kFarthest, low_y = apart > kReach && apart < kFarthest;
+        if (!__any_sync(0xffffffffu, low_x || low_y)) break;
+        scale_columns(taddr, c, end, low_x ? by : 1.f);
+        scale_columns(taddr + 128, c, end, low_y ? by : 1.f);
+        if (low_x) x = make_float2(x.x + kReach, x.y * by);
+        if (low_y) y = make_float2(y.x + kReach, y.y * by);
+    }
+    return make_float4(x.x, x.y, y.x, y.y);
+}
+
+// e4m3: NaN into the columns [c, end) of a row's accumulator where a V element of a drafted token that the row sees is one
+// (the tile's own have been zeroed); by whole warps, `mine` where the lane has a row
+__device__ __noinline__ void add_nan(const KernelArgs& a, const Walk& w, uint32_t taddr, int c, int end, int token, uint64_t bits, bool mine) {
+    const TreeAttnArgs& t = a.t;
+    const int n0 = max(max(0, w.k0 * kTile - w.r.p0), -w.r.p0), n1 = min(w.r.len, w.k1 * kTile) - w.r.p0;
+#pragma unroll 1
+    for (; c < end; c += 8) {
+        uint32_t x[8];
+        tmem_ld8(taddr + c, x);
+        for (int j = n0; j < n1; ++j) {
+            if (!mine || !(t.mask ? j < 64 && ((bits >> j) & 1) : j <= token)) continue;
+            const int pos = w.r.p0 + j;
+            const int page = __ldg(t.table + (long long)w.b * t.table_stride + pos / t.page_size);
+            if (page < 0 || page >= a.pages) continue;
+            const uint2 q = *reinterpret_cast<const uint2*>(static_cast<const uint8_t*>(t.c.v) +
+                                                            (long long)(page * t.page_size + pos % t.page_size) * t.c.slot_stride +
+                                                            (long long)w.h * t.c.head_stride + c);
+#pragma unroll
+            for (int d = 0; d < 8; ++d)
+                if ((((d < 4 ? q.x : q.y) >> (8 * (d & 3))) & 0x7F) == 0x7F) x[d] = 0x7fffffffu;
+        }
+        __syncwarp();
+        tmem_st8(taddr + c, x);
+    }
+}
+
+// where V scales have to lie to be near those of a tile (biased; e within [-90, 120])
+__device__ __noinline__ int first_window(const float* vs, const uint32_t* valid) {
+    const int lane = threadIdx.x & 31;
+    int most = -1;
+#pragma unroll
+    for (int e = 0; e < 2; ++e)
+        if ((valid[e] >> lane) & 1u) most = max(most, (int)(__float_as_uint(fabsf(vs[e * 32 + lane])) >> 23));
+    most = __reduce_max_sync(0xffffffffu, most);
+    return most < 0 || most > 246 ? kFar : max(36, most + 1 - kNear);
+}
+
+struct FarResult {
+    float ref, sum;
+    int e_low;                // -1 after a wait that gave up
+};
+
+// e4m3: a unit whose V scales lie far apart, from its scores to its weights in TMEM, with an e for each key.
+//
+// A reference may rise by the whole range of e here, more than one factor in fp32 bridges, so
+// accumulator and sum follow in steps of 2^-kReach (three at most; scores that differ by kFarthest
+// leave nothing).  The tiles between scale in one step.  What that flushes to zero (factors below
+// 2^-126) has to be nothing beside the new sum.  A sum is at most (keys) x 2^(14 - e_eff), e_eff the least
+// that e has added to the maximum of a row's scores so far, and the new one at least 2^(2 - e): with
+// 2^31 keys and e <= e_eff + kSpan, 2^(31 + 14 - 2 + kSpan - 126) = 2^-23 of it, and 2^-37 with 2^17
+// keys.  So where the V scales have risen by more than kSpan above e_eff, the tiles to come are far
+// as well.
+__device__ __noinline__ FarResult far_unit(uint32_t ts, uint32_t to, int dim, float cm, uint2 vis, const float* ks, const float* vs, float ref,
+                                           float sum, int e_low, volatile int* e_eff, uint64_t* used, uint32_t parity, volatile int* abort) {
+    auto power = [](float scale) {                              // e of a scale; of one that is not finite the least
+        const uint32_t x = __float_as_uint(fabsf(scale));
+        return x >= 0x7f800000u ? -90 : max(-90, min(120, (int)(x >> 23) - 126));
+    };
+    float target = -INFINITY, top = -INFINITY;
+    int most = -90;
+#pragma unroll 1
+    for (int j = 0; j < kTile; j += 8) {
+        uint32_t x[8];
+        tmem_ld8(ts + j, x);
+        const uint32_t seen = (j & 32 ? vis.y : vis.x) >> (j & 31);
+#pragma unroll
+        for (int i = 0; i < 8; i += 4) {
+            const float4 k4 = *reinterpret_cast<const float4*>(ks + j + i), v4 = *reinterpret_cast<const float4*>(vs + j + i);
+            const float kk[4] = {k4.x, k4.y, k4.z, k4.w}, vv[4] = {v4.x, v4.y, v4.z, v4.w};
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                const int e = power(vv[k]);
+                const float s = __uint_as_float(x[i + k]) * kk[k];
+                most = max(most, e);
+                if ((seen >> (i + k)) & 1u) {
+                    top = fmaxf(top, s * cm);
+                    target = fmaxf(target, fmaf(s, cm, (float)e));
+                }
+            }
+        }
+    }
+    int least = min(*e_eff, e_low == kFar ? kFar : e_low - 126);
+    least = min(least, __reduce_min_sync(0xffffffffu, target > -INFINITY && top < INFINITY ? (int)floorf(target - top) : kFar));
+    __syncwarp();
+    *e_eff = least;                                             // every lane the same
+    most += 127 - kNear;                                        // biased; room for one power above these
+    e_low = max(most, 36) - 126 > least + kSpan - kNear ? kFar : max(most, 36);
+    target -= 6.0f;
+    for (int k = 0; k < 4 && __any_sync(0xffffffffu, target > ref + kSlack); ++k) {
+        float to_ref = fmaxf(ref, target);
+        if (k < 3 && to_ref < ref + kFarthest) to_ref = fminf(to_ref, ref + kReach);
+        if (used) {                                             // the accumulator holds something
+            if (!__all_sync(0xffffffffu, wait_or_abort(used, parity, abort))) return {ref, sum, -1};
+            tc_fence_after();
+            const float f = ref == -INFINITY ? 1.0f : ex2(ref - to_ref);
+            sum *= f;
+            scale_columns(to, 0, dim, f);
+        }
+        ref = to_ref;
+    }
+    const float nref = ref == -INFINITY ? 0.f : -ref;
+    float part = 0.f;
+#pragma unroll 1
+    for (int j = 0; j < kTile; j += 8) {
+        uint32_t x[8], p[4];
+        tmem_ld8(ts + j, x);
+        const uint32_t seen = (j & 32 ? vis.y : vis.x) >> (j & 31);
+#pragma unroll
+        for (int i = 0; i < 8; i += 4) {
+            const float4 k4 = *reinterpret_cast<const float4*>(ks + j + i), v4 = *reinterpret_cast<const float4*>(vs + j + i);
+            const float kk[4] = {k4.x, k4.y, k4.z, k4.w}, vv[4] = {v4.x, v4.y, v4.z, v4.w};
+            float w[4];
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                w[k] = (seen >> (i + k)) & 1u ? ex2(fmaf(__uint_as_float(x[i + k]) * kk[k], cm, nref)) : 0.f;
+                part += w[k];
+                w[k] *= vv[k];
+            }
+            p[i / 2] = pack2(w[0], w[1], __half());
+            p[i / 2 + 1] = pack2(w[2], w[3], __half());
+        }
+        tmem_st4(ts + j / 2, p);                                // over scores that have been read
+    }
+    return {ref, sum + part, e_low};
 }
 
 // A unit is one stream's share of a tile: unit u of a segment belongs to stream u & 1 and uses its
@@ -1053,6 +1238,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_kernel(const __grid_constant
         constexpr int kLanes = DP / 8;                          // 16-byte chunks of a row
         constexpr int kStep = kSoftmaxThreads / kLanes;         // rows that the 256 threads move at once
         uint32_t seg = 0, tile0 = 0, jp = 0;                    // jp: phases of `joined`
+        [[maybe_unused]] int e_low = kFar;                      // e4m3: V scales with biased exponents in [e_low, e_low + kNear] are near
         uint32_t ph = 0;                                        // parity of each buffer
         bool ok = true;
         auto join = [&]() {                                     // both warpgroups have come here
@@ -1075,6 +1261,13 @@ __global__ void __launch_bounds__(kThreads, 1) attn_kernel(const __grid_constant
                 bring_queries<TQ, kFp8, DP>(a, seg == 0 ? sh->start : sh->seg[0], sq, row_mul, warp, kSoftmaxThreads / 32);
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&sh->q_full[0]);
+                if constexpr (kFp8) {
+                    if (seg == 0) {                             // V scales like those of the first tile are near
+                        ok = wait_at(smem_u32(&sh->info_full[0]), 0, abort);
+                        if (!ok) break;
+                        e_low = first_window(info[0].vs, info[0].valid);
+                    }
+                }
             }
             ok = wait_at(smem_u32(&sh->q_full[buf]), (seg / q_bufs) & 1u, abort);
             if (!ok) break;
@@ -1094,7 +1287,8 @@ __global__ void __launch_bounds__(kThreads, 1) attn_kernel(const __grid_constant
                 token += token0;
                 if (t.mask) bits = (uint64_t)__ldg(reinterpret_cast<const long long*>(t.mask) + w.r.lo + token);
             }
-            float ref = -INFINITY, sum = 0.f, vmax = 0.f;
+            float ref = -INFINITY, sum = 0.f;
+            if (kFp8 && lane == 0) sh->e_eff[warp] = kFar;
             const int step = both ? 1 : 2;
             int b = 0;
             for (int tl = both ? 0 : s; ok && tl < nt; tl += step, b ^= 1) {
@@ -1156,23 +1350,21 @@ __global__ void __launch_bounds__(kThreads, 1) attn_kernel(const __grid_constant
                     tmem_ld32(ts, v[0]);
                     tmem_ld32(ts + 32, v[1]);
                     uint32_t vis[2] = {~0u, ~0u};
+                    bool far = false;
                     if constexpr (kFp8) {
-                        // the largest V scale; a token whose V scale is not finite gets a K scale of NaN (the
-                        // rows that see it become NaN) and a V scale of 0 (the others do not); every warp
-                        // writes the same
-                        uint32_t top = 0;
+                        // a token whose V scale is not finite gets a K scale of NaN (the rows that see it become NaN)
+                        // and a V scale of 0 (the others do not); every warp writes the same
+                        bool near = true;
 #pragma unroll
                         for (int e = 0; e < 2; ++e) {
                             const uint32_t x = __float_as_uint(fabsf(inf->vs[e * 32 + lane]));
                             if (x >= 0x7f800000u) {
                                 const_cast<Info*>(inf)->ks[e * 32 + lane] = __int_as_float(0x7fffffff);
                                 const_cast<Info*>(inf)->vs[e * 32 + lane] = 0.f;
-                            } else {
-                                top = max(top, x);              // finite sizes: ordered as their bits
                             }
+                            near &= !(((e ? valid.y : valid.x) >> lane) & 1u) || (uint32_t)((int)(x >> 23) - e_low) <= (uint32_t)kNear;
                         }
-                        vmax = fmaxf(vmax, __uint_as_float(__reduce_max_sync(0xffffffffu, top)));
-                        __syncwarp();
+                        far = !__all_sync(0xffffffffu, near);
                     }
                     if (masked) {
 #pragma unroll
@@ -1190,91 +1382,106 @@ __global__ void __launch_bounds__(kThreads, 1) attn_kernel(const __grid_constant
                             vis[i] = m & (i ? valid.y : valid.x);
                         }
                     }
-                    float mx[2];
+                    if constexpr (kFp8) {
+                        if (far) {
+                            __syncwarp();
+                            tmem_wait_ld(v[0]);
+                            tmem_wait_ld(v[1]);
+                            const FarResult r = far_unit(ts, to, t.c.dim, cm, make_uint2(vis[0], vis[1]), inf->ks, inf->vs, ref, sum, e_low,
+                                                         &sh->e_eff[warp], tl >= step ? &sh->s_free[s][b ^ 1] : nullptr,
+                                                         ((ph >> (b ^ 1)) & 1u) ^ 1u, abort);
+                            ref = r.ref;
+                            sum = r.sum;
+                            e_low = r.e_low;
+                            ok = e_low >= 0;
+                            if (!ok) break;
+                        }
+                    }
+                    if (!kFp8 || !far) {
+                        float mx[2];
 #pragma unroll
-                    for (int c = 0; c < 2; ++c) {
-                        tmem_wait_ld(v[c]);
-                        if constexpr (kFp8) {
+                        for (int c = 0; c < 2; ++c) {
+                            tmem_wait_ld(v[c]);
+                            if constexpr (kFp8) {
+#pragma unroll
+                                for (int j = 0; j < 32; j += 4) {
+                                    const float4 k4 = *reinterpret_cast<const float4*>(&inf->ks[c * 32 + j]);
+                                    const float2 lo = __fmul2_rn(make_float2(__uint_as_float(v[c][j]), __uint_as_float(v[c][j + 1])),
+                                                                 make_float2(k4.x, k4.y));
+                                    const float2 hi = __fmul2_rn(make_float2(__uint_as_float(v[c][j + 2]), __uint_as_float(v[c][j + 3])),
+                                                                 make_float2(k4.z, k4.w));
+                                    v[c][j] = __float_as_uint(lo.x);
+                                    v[c][j + 1] = __float_as_uint(lo.y);
+                                    v[c][j + 2] = __float_as_uint(hi.x);
+                                    v[c][j + 3] = __float_as_uint(hi.y);
+                                }
+                            }
+                            if (masked) {
+#pragma unroll
+                                for (int j = 0; j < 32; ++j)
+                                    if (!((vis[c] >> j) & 1u)) v[c][j] = 0xFF800000u;
+                            }
+                            float a0 = -INFINITY, a1 = -INFINITY;
 #pragma unroll
                             for (int j = 0; j < 32; j += 4) {
-                                const float4 k4 = *reinterpret_cast<const float4*>(&inf->ks[c * 32 + j]);
-                                const float2 lo = __fmul2_rn(make_float2(__uint_as_float(v[c][j]), __uint_as_float(v[c][j + 1])),
-                                                             make_float2(k4.x, k4.y));
-                                const float2 hi = __fmul2_rn(make_float2(__uint_as_float(v[c][j + 2]), __uint_as_float(v[c][j + 3])),
-                                                             make_float2(k4.z, k4.w));
-                                v[c][j] = __float_as_uint(lo.x);
-                                v[c][j + 1] = __float_as_uint(lo.y);
-                                v[c][j + 2] = __float_as_uint(hi.x);
-                                v[c][j + 3] = __float_as_uint(hi.y);
+                                a0 = fmaxf(a0, fmaxf(__uint_as_float(v[c][j]), __uint_as_float(v[c][j + 1])));
+                                a1 = fmaxf(a1, fmaxf(__uint_as_float(v[c][j + 2]), __uint_as_float(v[c][j + 3])));
                             }
+                            mx[c] = fmaxf(a0, a1);
                         }
-                        if (masked) {
-#pragma unroll
-                            for (int j = 0; j < 32; ++j)
-                                if (!((vis[c] >> j) & 1u)) v[c][j] = 0xFF800000u;
+                        float target = fmaxf(mx[0], mx[1]) * cm;
+                        if constexpr (kFp8) {
+                            target += (float)(e_low + kNear - 126 - 6);
+                        } else if constexpr (std::is_same<TO, __half>::value) {
+                            target -= 6.0f;
                         }
-                        float a0 = -INFINITY, a1 = -INFINITY;
-#pragma unroll
-                        for (int j = 0; j < 32; j += 4) {
-                            a0 = fmaxf(a0, fmaxf(__uint_as_float(v[c][j]), __uint_as_float(v[c][j + 1])));
-                            a1 = fmaxf(a1, fmaxf(__uint_as_float(v[c][j + 2]), __uint_as_float(v[c][j + 3])));
-                        }
-                        mx[c] = fmaxf(a0, a1);
-                    }
-                    float target = fmaxf(mx[0], mx[1]) * cm;
-                    if constexpr (kFp8) {
-                        // 2^ev is the first power of two above the V scales so far
-                        const int ev = max(-90, min(120, (int)(__float_as_uint(vmax) >> 23) - 126));
-                        target += (float)(ev - 6);
-                    } else if constexpr (std::is_same<TO, __half>::value) {
-                        target -= 6.0f;
-                    }
-                    if (__any_sync(0xffffffffu, target > ref + kSlack)) {
-                        const float to_ref = fmaxf(ref, target);
-                        if (tl >= step) {                       // the accumulator holds something
-                            ok = __all_sync(0xffffffffu, wait_or_abort(&sh->s_free[s][b ^ 1], ((ph >> (b ^ 1)) & 1u) ^ 1u, abort));
-                            if (!ok) break;
-                            tc_fence_after();
-                            const float f = ref == -INFINITY ? 1.0f : ex2(ref - to_ref);
-                            sum *= f;
+                        if (__any_sync(0xffffffffu, target > ref + kSlack)) {
+                            const float to_ref = fmaxf(ref, target);
+                            if (tl >= step) {                       // the accumulator holds something
+                                ok = __all_sync(0xffffffffu, wait_or_abort(&sh->s_free[s][b ^ 1], ((ph >> (b ^ 1)) & 1u) ^ 1u, abort));
+                                if (!ok) break;
+                                tc_fence_after();
+                                const float f = ref == -INFINITY ? 1.0f : ex2(ref - to_ref);
+                                sum *= f;
 #pragma unroll 1
-                            for (int c = 0; c < t.c.dim; c += 32) {
-                                uint32_t o[32];
-                                tmem_ld32(to + c, o);
-                                tmem_wait_ld(o);
+                                for (int c = 0; c < t.c.dim; c += 32) {
+                                    uint32_t o[32];
+                                    tmem_ld32(to + c, o);
+                                    tmem_wait_ld(o);
 #pragma unroll
-                                for (int j = 0; j < 32; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * f);
-                                tmem_st32(to + c, o);
+                                    for (int j = 0; j < 32; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * f);
+                                    tmem_st32(to + c, o);
+                                }
                             }
+                            ref = to_ref;
                         }
-                        ref = to_ref;
-                    }
-                    const float nref = ref == -INFINITY ? 0.f : -ref;
-                    const float2 cm2 = make_float2(cm, cm), nref2 = make_float2(nref, nref);
-                    float2 part0 = make_float2(0.f, 0.f), part1 = part0;
+                        const float nref = ref == -INFINITY ? 0.f : -ref;
+                        const float2 cm2 = make_float2(cm, cm), nref2 = make_float2(nref, nref);
+                        float2 part0 = make_float2(0.f, 0.f), part1 = part0;
 #pragma unroll
-                    for (int c = 0; c < 2; ++c) {
-                        uint32_t p[16];
+                        for (int c = 0; c < 2; ++c) {
+                            uint32_t p[16];
 #pragma unroll
-                        for (int j = 0; j < 32; j += 4) {
-                            float2 lo = __ffma2_rn(make_float2(__uint_as_float(v[c][j]), __uint_as_float(v[c][j + 1])), cm2, nref2);
-                            float2 hi = __ffma2_rn(make_float2(__uint_as_float(v[c][j + 2]), __uint_as_float(v[c][j + 3])), cm2, nref2);
-                            lo = make_float2(ex2(lo.x), ex2(lo.y));
-                            hi = make_float2(ex2(hi.x), ex2(hi.y));
-                            part0 = __fadd2_rn(part0, lo);
-                            part1 = __fadd2_rn(part1, hi);
-                            if constexpr (kFp8) {
-                                const float4 v4 = *reinterpret_cast<const float4*>(&inf->vs[c * 32 + j]);
-                                lo = __fmul2_rn(lo, make_float2(v4.x, v4.y));
-                                hi = __fmul2_rn(hi, make_float2(v4.z, v4.w));
+                            for (int j = 0; j < 32; j += 4) {
+                                float2 lo = __ffma2_rn(make_float2(__uint_as_float(v[c][j]), __uint_as_float(v[c][j + 1])), cm2, nref2);
+                                float2 hi = __ffma2_rn(make_float2(__uint_as_float(v[c][j + 2]), __uint_as_float(v[c][j + 3])), cm2, nref2);
+                                lo = make_float2(ex2(lo.x), ex2(lo.y));
+                                hi = make_float2(ex2(hi.x), ex2(hi.y));
+                                part0 = __fadd2_rn(part0, lo);
+                                part1 = __fadd2_rn(part1, hi);
+                                if constexpr (kFp8) {
+                                    const float4 v4 = *reinterpret_cast<const float4*>(&inf->vs[c * 32 + j]);
+                                    lo = __fmul2_rn(lo, make_float2(v4.x, v4.y));
+                                    hi = __fmul2_rn(hi, make_float2(v4.z, v4.w));
+                                }
+                                p[j / 2] = pack2(lo.x, lo.y, TO());
+                                p[j / 2 + 1] = pack2(hi.x, hi.y, TO());
                             }
-                            p[j / 2] = pack2(lo.x, lo.y, TO());
-                            p[j / 2 + 1] = pack2(hi.x, hi.y, TO());
+                            tmem_st16(ts + c * 16, p);              // over scores that have been read
                         }
-                        tmem_st16(ts + c * 16, p);              // over scores that have been read
+                        sum += (part0.x + part0.y) + (part1.x + part1.y);
+                        tmem_wait_st();
                     }
-                    sum += (part0.x + part0.y) + (part1.x + part1.y);
-                    tmem_wait_st();
                 }
                 tc_fence_before();
                 __syncwarp();
@@ -1291,11 +1498,19 @@ __global__ void __launch_bounds__(kThreads, 1) attn_kernel(const __grid_constant
             if (!ok) break;
             float f0 = 1.f, f1 = 0.f;                           // factors of the two accumulators
             if (!both) {
-                const float2 x = swap[row];
+                float2 x = swap[row];
                 ref = x.x;
                 sum = x.y;
                 if (nt > 1) {
-                    const float2 y = swap[kRows + row];
+                    float2 y = swap[kRows + row];
+                    if constexpr (kFp8) {
+                        // references further apart than one factor bridges
+                        if (any_row && __any_sync(0xffffffffu, fabsf(x.x - y.x) > kReach)) {
+                            const float4 xy = bring_nearer(tmem + lanes + 256, s * (DP / 2), min((s + 1) * (DP / 2), t.c.dim), x, y);
+                            x = make_float2(xy.x, xy.y);
+                            y = make_float2(xy.z, xy.w);
+                        }
+                    }
                     ref = fmaxf(x.x, y.x);
                     f0 = ref == -INFINITY ? 1.f : ex2(x.x - ref);
                     f1 = ref == -INFINITY ? 1.f : ex2(y.x - ref);
@@ -1313,6 +1528,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_kernel(const __grid_constant
                 uint8_t* so = sqb + (my >> 7) * L::kQTile;
                 const float inv = sum == 0.f ? 0.f : 1.0f / sum;
                 const int c0 = both ? 0 : s * (DP / 2), c1 = both ? DP : c0 + DP / 2;
+                if (kFp8 && odd) add_nan(a, w, tmem + lanes + 256 + (both ? s * 128 : 0), c0, min(c1, t.c.dim), token, bits, my < nrows);
 #pragma unroll 1
                 for (int c = c0; c < c1 && c < t.c.dim; c += 32) {
                     uint32_t v[32];
@@ -1328,7 +1544,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_kernel(const __grid_constant
                     } else {
                         tmem_wait_ld(v);
                     }
-                    if (odd && my < nrows) {
+                    if (!kFp8 && odd && my < nrows) {
                         const int pages = (int)(t.c.slots / t.page_size);
                         const int n0 = max(max(0, w.k0 * kTile - w.r.p0), -w.r.p0), n1 = min(w.r.len, w.k1 * kTile) - w.r.p0;
                         for (int j = n0; j < n1; ++j) {
@@ -1341,14 +1557,8 @@ __global__ void __launch_bounds__(kThreads, 1) attn_kernel(const __grid_constant
 #pragma unroll
                             for (int d = 0; d < 32; ++d) {
                                 if (c + d >= t.c.dim) break;
-                                float x;
-                                if constexpr (kFp8) {
-                                    const uint8_t q8 = static_cast<const uint8_t*>(t.c.v)[at + d];
-                                    x = (q8 & 0x7F) == 0x7F ? __int_as_float(0x7fffffff) : 0.f;
-                                } else {
-                                    x = (float)static_cast<const TQ*>(t.c.v)[at + d];
-                                    if (fabsf(x) < __int_as_float(0x7f800000)) x = 0.f;
-                                }
+                                float x = (float)static_cast<const TQ*>(t.c.v)[at + d];
+                                if (fabsf(x) < __int_as_float(0x7f800000)) x = 0.f;
                                 v[d] = __float_as_uint(__uint_as_float(v[d]) + x);
                             }
                         }
@@ -1438,12 +1648,13 @@ __global__ void __launch_bounds__(kCombineThreads) combine_kernel(const __grid_c
         for (int p = 0; p < parts; ++p) {
             const float2 m = __ldcg(ml + slot_of(p) * per);
             const float4 x = __ldcg(po + slot_of(p) * (DP / 4) * per);
-            const float f = top == -INFINITY ? 1.f : ex2(m.x - top);
-            sum = fmaf(m.y, f, sum);
-            acc[0] = fmaf(x.x, f, acc[0]);
-            acc[1] = fmaf(x.y, f, acc[1]);
-            acc[2] = fmaf(x.z, f, acc[2]);
-            acc[3] = fmaf(x.w, f, acc[3]);
+            // in two factors, as references may lie further apart than one bridges (see kReach)
+            const float d = top == -INFINITY ? 0.f : m.x - top, near = fmaxf(d, -kReach), f = ex2(near), g = ex2(d - near);
+            sum = fmaf(m.y * g, f, sum);
+            acc[0] = fmaf(x.x * g, f, acc[0]);
+            acc[1] = fmaf(x.y * g, f, acc[1]);
+            acc[2] = fmaf(x.z * g, f, acc[2]);
+            acc[3] = fmaf(x.w * g, f, acc[3]);
         }
         const int token = (row0 + row) / t.group;
         const long long qrow = r.lo + token;
