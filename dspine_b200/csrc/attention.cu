@@ -679,7 +679,7 @@ struct FarResult {
     int e_low;                // -1 after a wait that gave up
 };
 
-// e4m3: a unit whose V scales lie far apart, from its scores to its weights in TMEM, with an e for each key.
+// e4m3: a unit whose V scales lie far apart or are not finite, from its scores to its weights in TMEM, with an e for each key.
 //
 // A reference may rise by the whole range of e here, more than one factor in fp32 bridges, so
 // accumulator and sum follow in steps of 2^-kReach (three at most; scores that differ by kFarthest
@@ -751,9 +751,10 @@ __device__ __noinline__ FarResult far_unit(uint32_t ts, uint32_t to, int dim, fl
             float w[4];
 #pragma unroll
             for (int k = 0; k < 4; ++k) {
-                w[k] = (seen >> (i + k)) & 1u ? ex2(fmaf(__uint_as_float(x[i + k]) * kk[k], cm, nref)) : 0.f;
+                const bool sees = (seen >> (i + k)) & 1u;
+                w[k] = sees ? ex2(fmaf(__uint_as_float(x[i + k]) * kk[k], cm, nref)) : 0.f;
                 part += w[k];
-                w[k] *= vv[k];
+                w[k] = sees ? w[k] * vv[k] : 0.f;              // a scale that is not finite: the rows that see it alone
             }
             p[i / 2] = pack2(w[0], w[1], __half());
             p[i / 2 + 1] = pack2(w[2], w[3], __half());
@@ -1352,19 +1353,10 @@ __global__ void __launch_bounds__(kThreads, 1) attn_kernel(const __grid_constant
                     uint32_t vis[2] = {~0u, ~0u};
                     bool far = false;
                     if constexpr (kFp8) {
-                        // a token whose V scale is not finite gets a K scale of NaN (the rows that see it become NaN)
-                        // and a V scale of 0 (the others do not); every warp writes the same
-                        bool near = true;
-#pragma unroll
-                        for (int e = 0; e < 2; ++e) {
-                            const uint32_t x = __float_as_uint(fabsf(inf->vs[e * 32 + lane]));
-                            if (x >= 0x7f800000u) {
-                                const_cast<Info*>(inf)->ks[e * 32 + lane] = __int_as_float(0x7fffffff);
-                                const_cast<Info*>(inf)->vs[e * 32 + lane] = 0.f;
-                            }
-                            near &= !(((e ? valid.y : valid.x) >> lane) & 1u) || (uint32_t)((int)(x >> 23) - e_low) <= (uint32_t)kNear;
-                        }
-                        far = !__all_sync(0xffffffffu, near);
+                        const uint32_t x0 = __float_as_uint(fabsf(inf->vs[lane])) >> 23, x1 = __float_as_uint(fabsf(inf->vs[32 + lane])) >> 23;
+                        const uint32_t out0 = __ballot_sync(0xffffffffu, x0 - (uint32_t)e_low > (uint32_t)kNear) & valid.x,
+                                       out1 = __ballot_sync(0xffffffffu, x1 - (uint32_t)e_low > (uint32_t)kNear) & valid.y;
+                        far = (out0 | out1) != 0;
                     }
                     if (masked) {
 #pragma unroll
@@ -1384,7 +1376,6 @@ __global__ void __launch_bounds__(kThreads, 1) attn_kernel(const __grid_constant
                     }
                     if constexpr (kFp8) {
                         if (far) {
-                            __syncwarp();
                             tmem_wait_ld(v[0]);
                             tmem_wait_ld(v[1]);
                             const FarResult r = far_unit(ts, to, t.c.dim, cm, make_uint2(vis[0], vis[1]), inf->ks, inf->vs, ref, sum, e_low,

@@ -121,3 +121,31 @@ def test_scales_of_zero():
     c.vs[_slots(c, 0, torch.arange(0, 200, 2))] = 0.0
     c.vs[_slots(c, 1, torch.arange(70))] = 0.0
     _check(c, c.run())
+
+
+@pytest.mark.parametrize("value", [math.inf, -math.inf, math.nan])
+@pytest.mark.parametrize("dim,group", [(64, 4), (128, 20)])
+def test_v_scales_that_are_not_finite_reach_the_rows_that_see_them(value, dim, group):
+    """A drafted token with such a V scale: out of the rows that see it, no other row, and no logsumexp (which is K's)."""
+    c = Case([6, 40, 2], [150, 60, 200], heads=2 * group, kv_heads=2, dim=dim, page=16, cache="e4m3", tree=True, seed=8, size=0.3)
+    c.masks[:6] = torch.tensor([0b1, 0b11, 0b101, 0b1011, 0b10101, 0b100001])
+    c.vs[_slots(c, 0, [146]), 0] = value                   # node 2: rows 2 and 4
+    c.vs[_slots(c, 1, [59]), 1] = value                    # node 39: itself, unless another row names it
+    c.vs[_slots(c, 2, [3]), 0] = value                     # the context: every row
+    c.masks[6:45] &= (1 << 39) - 1
+    out, lse = (x.double().cpu() for x in c.run())
+    want = c.want()
+    _, lse_bound = R.attention_bounds(*want, dim=dim, out_dtype=c.kind, weight_half_step=2.0 ** -11)
+    assert bool(torch.isfinite(lse).all()) and bool(((lse - want[1]).abs() <= lse_bound).all())
+    touched = torch.zeros(48, 2, dtype=torch.bool)
+    touched[[2, 4, 46, 47], 0] = True
+    touched[45, 1] = True
+    touched = touched.repeat_interleave(group, 1)
+    assert torch.equal(~torch.isfinite(want[0]).all(-1), touched)
+    same = out.nan_to_num(1.0, 2.0, 3.0) == want[0].nan_to_num(1.0, 2.0, 3.0)
+    assert bool(same[touched].all())
+    # the other rows' bounds, from a cache in which those tokens hold zeros (they do not see them)
+    c.vs = torch.where(torch.isfinite(c.vs), c.vs, torch.zeros_like(c.vs))
+    clean = c.want()
+    bound, _ = R.attention_bounds(*clean, dim=dim, out_dtype=c.kind, weight_half_step=2.0 ** -11)
+    assert bool(((out - clean[0]).abs() <= bound + _products_bound(c))[~touched].all())
