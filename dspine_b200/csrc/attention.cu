@@ -157,7 +157,7 @@ struct KernelArgs {
 
 struct Request {
     int lo, n;              // rows of q
-    int len, p0;            // cached positions, the first drafted one
+    int len, p0;            // cached positions that the page table reaches, the first drafted one
     int rows, blocks;       // n x group, row blocks
 };
 
@@ -173,12 +173,11 @@ __device__ __forceinline__ Request request_of(const TreeAttnArgs& a, int qt, int
         lo = (long long)b * a.width;
         hi = lo + a.width;
     }
-    const int cap = a.max_pages * a.page_size;
-    const int len = __ldg(a.lens + b);
+    const int len = max(0, __ldg(a.lens + b));
     r.lo = (int)lo;
     r.n = (int)(hi - lo);
-    r.len = len < 0 ? 0 : (len > cap ? cap : len);
-    r.p0 = r.len - r.n;
+    r.len = min(len, a.max_pages * a.page_size);            // positions past the table are unseen,
+    r.p0 = len - r.n;                                       // which moves no drafted token
     r.rows = r.n * a.group;
     r.blocks = (r.rows + kRows * qt - 1) / (kRows * qt);
     return r;

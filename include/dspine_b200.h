@@ -471,7 +471,7 @@ int dsv_kv_read(int64_t tokens, const void* slots, int32_t slots_int64, const ds
  * is with q_indptr a bound on the rows of a request, by which the work is laid out (a request
  * with more rows is computed all the same).
  * Bits of *err (a device word, may be NULL): bit 1: a page outside the cache, or a length above
- * max_pages * page_size (those positions are unseen); bit 2: a wait inside the kernel timed out
+ * max_pages * page_size (those positions are unseen, drafted tokens among them); bit 2: a wait inside the kernel timed out
  * (outputs not valid).  The workspace needs no initialisation; calls that may overlap need one
  * each. */
 int dsv_tree_attention_workspace_size(int32_t q_heads, int32_t kv_heads, int32_t dim,

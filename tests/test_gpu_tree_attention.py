@@ -441,3 +441,22 @@ def test_one_serving_round():
         at = torch.tensor([b * T + i for i in path])
         assert torch.equal(rk.view(B, T, kv_heads, dim)[b, :c].cpu(), codes.float()[at] * sc[at][..., None])
         assert not bool(rk.view(B, T, kv_heads, dim)[b, c:].any())
+
+
+@pytest.mark.parametrize("tree", [False, True])
+@pytest.mark.parametrize("length", [129, 130, 133, 200, 100000, (1 << 31) - 1])
+def test_a_length_past_the_table_leaves_the_drafted_tokens_where_they_are(length, tree):
+    """The drafted tokens are the last of kv_lens also where the page table ends before them: the context keeps
+    its positions, those past the table are unseen."""
+    c = Case([5, 2], [128, 100], heads=8, kv_heads=2, dim=64, tree=tree, seed=21)
+    if tree:
+        c.masks[:5] = torch.tensor([0b1, 0b10, 0b100, 0b1001, 0b10000])
+    c.lengths = [length, 100]
+    c.table = c.table[:, :8].contiguous()                  # 128 positions
+    err = torch.zeros(1, dtype=torch.int32, device="cuda")
+    got = c.run(err=err)
+    assert int(err) == 2
+    # the same call with a table that goes on, with pages that are none (length: any at which all of it is context)
+    c.lengths = [min(length, 300), 100]
+    c.table = torch.cat([c.table, torch.full((2, 12), 1 << 30, dtype=torch.int32)], 1)
+    c.check(got)
