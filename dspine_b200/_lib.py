@@ -141,6 +141,7 @@ _SIGNATURES = {
                            ctypes.POINTER(KvCache), c_void_p, c_int64, c_int32, c_int32, c_void_p,
                            c_void_p, c_int32, c_void_p, ctypes.c_float, c_void_p, c_int64, c_int64,
                            c_void_p, c_void_p, c_void_p, c_size_t, c_void_p],
+    "dsv_tree_attention_waits": [c_int32, c_int32],
     "dsv_accept_tree": [c_int32, c_int64, c_void_p, c_void_p, c_void_p, c_void_p, c_int32,
                         c_void_p, c_void_p, c_int32, c_void_p, c_void_p, c_void_p, c_void_p,
                         c_void_p, c_void_p, c_void_p, c_void_p],

@@ -73,8 +73,9 @@ def tree_attention(q, k_cache, v_cache, page_table, kv_lens, *, page_size=1, q_i
     workspace: uint8 scratch of `workspace_bytes` (allocated for the call unless given); calls that may
     overlap need one each.  err (int32 [1], optional) collects bit 1: a page outside the cache or
     a length past the page table (those positions are unseen, drafted tokens among them; no token
-    moves), bit 2: a wait that timed out.  A masked position's K may hold anything; V of positions that some row of the request sees
-    reaches the rows that see it alone, infinities and NaN included."""
+    moves), bit 2: a wait that timed out, whose rows are NaN.  A masked position's K may hold
+    anything; V of positions that some row of the request sees reaches the rows that see it alone,
+    infinities and NaN included."""
     c = describe(k_cache, v_cache, k_scale, v_scale)
     dev = k_cache.device
     shape = q.shape

@@ -78,6 +78,7 @@
 #include <stddef.h>
 #include <stdint.h>
 
+#include <atomic>
 #include <type_traits>
 
 #include "dsv_common.cuh"
@@ -146,6 +147,7 @@ struct KernelArgs {
     TreeAttnArgs t;
     Divisor page, group;    // by page_size, by t.group
     int pages;              // of the cache
+    int wait_us, hold;      // limit of a wait; tile of a CTA that is never described (tests of that limit), -1
     int qt;                 // Q tiles of a row block
     Split* splits;          // [kMaxCtas]
     float2* part_ml;        // [2 * kMaxCtas][128 qt] (reference, sum)
@@ -300,9 +302,9 @@ struct alignas(16) Shared {
     uint64_t joined;                 // both warpgroups have written what the other reads
     uint64_t drain[2];
     uint32_t tmem;
-    int abort;
+    int abort, wait_us;              // a wait has given up, and after how long: see wait_limit
     int odd[2];                      // a drafted V element was not finite (by segment parity)
-    int e_eff[8];                    // e4m3, a softmax warp each: see far_unit
+    int e_low[8], e_eff[8];          // e4m3, a softmax warp each: see far_unit
     int v_done[2];                   // e4m3: V tiles (even, odd) in their stages, as one past the last
     long long scan[32];
     Walk start;                      // where this CTA starts on the line of tiles
@@ -475,6 +477,9 @@ __device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_grou
 template <int N> __device__ __forceinline__ void cp_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
 __device__ __forceinline__ void cp_wait_all() { asm volatile("cp.async.wait_all;" ::: "memory"); }
 
+// ns after which a wait gives up; Shared holds the limit beside the word that says that one has
+__device__ __forceinline__ uint64_t wait_limit(volatile int* abort) { return (uint64_t)abort[1] * 1000u; }
+
 // bounded wait that also gives up when another warp of the CTA has given up
 __device__ __noinline__ bool wait_slow(uint64_t* bar, uint32_t parity, volatile int* abort) {
     const uint64_t t0 = globaltimer_ns();
@@ -482,7 +487,7 @@ __device__ __noinline__ bool wait_slow(uint64_t* bar, uint32_t parity, volatile 
         if (mbar_try_wait(bar, parity)) return true;
         if (i % 32 != 0) continue;
         if (*abort) return false;
-        if (globaltimer_ns() - t0 > 2000000000ull) {
+        if (globaltimer_ns() - t0 > wait_limit(abort)) {
             *abort = 1;
             return false;
         }
@@ -508,7 +513,7 @@ __device__ __noinline__ bool wait_slow_at(uint32_t bar, uint32_t parity, volatil
         if (try_wait_at(bar, parity)) return true;
         if (i % 32 != 0) continue;
         if (*abort) return false;
-        if (globaltimer_ns() - t0 > 2000000000ull) {
+        if (globaltimer_ns() - t0 > wait_limit(abort)) {
             *abort = 1;
             return false;
         }
@@ -520,7 +525,7 @@ __device__ __noinline__ bool wait_past(volatile int* at, int value, volatile int
     for (uint32_t i = 1; *at <= value; ++i) {
         if (i % 32 != 0) continue;
         if (*abort) return false;
-        if (globaltimer_ns() - t0 > 2000000000ull) {
+        if (globaltimer_ns() - t0 > wait_limit(abort)) {
             *abort = 1;
             return false;
         }
@@ -663,7 +668,7 @@ __device__ __noinline__ void add_nan(const KernelArgs& a, const Walk& w, uint32_
 }
 
 // where V scales have to lie to be near those of a tile (biased; e within [-90, 120])
-__device__ __noinline__ int first_window(const float* vs, const uint32_t* valid) {
+__device__ __forceinline__ int first_window(const float* vs, const uint32_t* valid) {
     const int lane = threadIdx.x & 31;
     int most = -1;
 #pragma unroll
@@ -688,8 +693,10 @@ struct FarResult {
 // 2^31 keys and e <= e_eff + kSpan, 2^(31 + 14 - 2 + kSpan - 126) = 2^-23 of it, and 2^-37 with 2^17
 // keys.  So where the V scales have risen by more than kSpan above e_eff, the tiles to come are far
 // as well.
-__device__ __noinline__ FarResult far_unit(uint32_t ts, uint32_t to, int dim, float cm, uint2 vis, const float* ks, const float* vs, float ref,
-                                           float sum, int e_low, volatile int* e_eff, uint64_t* used, uint32_t parity, volatile int* abort) {
+__device__ __noinline__ FarResult far_unit(uint32_t ts, uint32_t to, int dim, float cm, uint2 vis, const TileInfoScaled& inf, float ref,
+                                           float sum, int e_low, Shared* sh, uint64_t* used, uint32_t parity) {
+    const float *ks = inf.ks, *vs = inf.vs;
+    volatile int *e_eff = &sh->e_eff[threadIdx.x >> 5], *abort = &sh->abort;
     auto power = [](float scale) {                              // e of a scale; of one that is not finite the least
         const uint32_t x = __float_as_uint(fabsf(scale));
         return x >= 0x7f800000u ? -90 : max(-90, min(120, (int)(x >> 23) - 126));
@@ -761,6 +768,32 @@ __device__ __noinline__ FarResult far_unit(uint32_t ts, uint32_t to, int dim, fl
         tmem_st4(ts + j / 2, p);                                // over scores that have been read
     }
     return {ref, sum + part, e_low};
+}
+
+// A wait has given up: NaN for all rows of this CTA's segments, so that none passes for a result.  By one warp.
+__device__ __noinline__ void give_up(const KernelArgs& a, Shared* sh) {
+    Walk& w = sh->walk[0];
+    const TreeAttnArgs& t = a.t;
+    const int lane = threadIdx.x & 31, per = kRows * a.qt;
+    const float nan = __int_as_float(0x7fffffff);
+    if (lane == 0) {
+        w = sh->start;
+        if (t.err) atomicOr(t.err, 4u);
+    }
+    __syncwarp();
+    do {
+        const bool whole = w.k0 == 0 && w.k1 == w.tiles;
+        for (int r = lane; r < w.rows(a.qt); r += 32) {
+            const int token = (w.first_row(a.qt) + r) / t.group, hq = w.h * t.group + (w.first_row(a.qt) + r) - token * t.group;
+            if (!whole) {                                       // the join makes NaN of it
+                a.part_ml[(long long)(2 * blockIdx.x + (w.k0 == 0 ? 1 : 0)) * per + r] = make_float2(nan, nan);
+                continue;
+            }
+            uint16_t* out = static_cast<uint16_t*>(t.out) + (w.r.lo + token) * t.out_token_stride + hq * t.out_head_stride;
+            for (int d = 0; d < t.c.dim; ++d) out[d] = 0x7fff;  // NaN of either type
+            if (t.lse) t.lse[(long long)(w.r.lo + token) * t.q_heads + hq] = nan;
+        }
+    } while (w.advance(a));
 }
 
 // A unit is one stream's share of a tile: unit u of a segment belongs to stream u & 1 and uses its
@@ -880,6 +913,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_kernel(const __grid_constant
         mbar_init(&sh->o_full, 1);
         mbar_init(&sh->joined, 8);
         sh->abort = 0;
+        sh->wait_us = a.wait_us;
         sh->odd[0] = sh->odd[1] = 0;
         sh->v_done[0] = sh->v_done[1] = 0;
         fence_mbar_init();
@@ -1073,7 +1107,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_kernel(const __grid_constant
                 for (int k = 0; k < 2; ++k) {
                     if (t0 + k >= nt) break;
                     const int at = ti % kInfo;
-                    ok = __all_sync(0xffffffffu,
+                    ok = __all_sync(0xffffffffu, ti != a.hold &&
                                     wait_or_abort(&sh->info_empty[at], ((uint32_t)(ti / kInfo) & 1u) ^ 1u, abort));
                     if (!ok) break;
                     Info* f = info + at;
@@ -1238,7 +1272,6 @@ __global__ void __launch_bounds__(kThreads, 1) attn_kernel(const __grid_constant
         constexpr int kLanes = DP / 8;                          // 16-byte chunks of a row
         constexpr int kStep = kSoftmaxThreads / kLanes;         // rows that the 256 threads move at once
         uint32_t seg = 0, tile0 = 0, jp = 0;                    // jp: phases of `joined`
-        [[maybe_unused]] int e_low = kFar;                      // e4m3: V scales with biased exponents in [e_low, e_low + kNear] are near
         uint32_t ph = 0;                                        // parity of each buffer
         bool ok = true;
         auto join = [&]() {                                     // both warpgroups have come here
@@ -1265,7 +1298,9 @@ __global__ void __launch_bounds__(kThreads, 1) attn_kernel(const __grid_constant
                     if (seg == 0) {                             // V scales like those of the first tile are near
                         ok = wait_at(smem_u32(&sh->info_full[0]), 0, abort);
                         if (!ok) break;
-                        e_low = first_window(info[0].vs, info[0].valid);
+                        const int from = first_window(info[0].vs, info[0].valid);
+                        if (lane == 0) sh->e_low[warp] = from;
+                        __syncwarp();
                     }
                 }
             }
@@ -1351,7 +1386,9 @@ __global__ void __launch_bounds__(kThreads, 1) attn_kernel(const __grid_constant
                     tmem_ld32(ts + 32, v[1]);
                     uint32_t vis[2] = {~0u, ~0u};
                     bool far = false;
+                    [[maybe_unused]] int e_low = 0;
                     if constexpr (kFp8) {
+                        e_low = *(volatile int*)&sh->e_low[warp];
                         const uint32_t x0 = __float_as_uint(fabsf(inf->vs[lane])) >> 23, x1 = __float_as_uint(fabsf(inf->vs[32 + lane])) >> 23;
                         const uint32_t out0 = __ballot_sync(0xffffffffu, x0 - (uint32_t)e_low > (uint32_t)kNear) & valid.x,
                                        out1 = __ballot_sync(0xffffffffu, x1 - (uint32_t)e_low > (uint32_t)kNear) & valid.y;
@@ -1377,13 +1414,13 @@ __global__ void __launch_bounds__(kThreads, 1) attn_kernel(const __grid_constant
                         if (far) {
                             tmem_wait_ld(v[0]);
                             tmem_wait_ld(v[1]);
-                            const FarResult r = far_unit(ts, to, t.c.dim, cm, make_uint2(vis[0], vis[1]), inf->ks, inf->vs, ref, sum, e_low,
-                                                         &sh->e_eff[warp], tl >= step ? &sh->s_free[s][b ^ 1] : nullptr,
-                                                         ((ph >> (b ^ 1)) & 1u) ^ 1u, abort);
+                            const FarResult r = far_unit(ts, to, t.c.dim, cm, make_uint2(vis[0], vis[1]), *inf, ref, sum, e_low, sh,
+                                                         tl >= step ? &sh->s_free[s][b ^ 1] : nullptr, ((ph >> (b ^ 1)) & 1u) ^ 1u);
                             ref = r.ref;
                             sum = r.sum;
-                            e_low = r.e_low;
-                            ok = e_low >= 0;
+                            ok = r.e_low >= 0;
+                            if (lane == 0) sh->e_low[warp] = r.e_low;
+                            __syncwarp();
                             if (!ok) break;
                         }
                     }
@@ -1602,7 +1639,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_kernel(const __grid_constant
     }
 
     __syncthreads();
-    if (tid == 0 && *abort && t.err) atomicOr(t.err, 4u);
+    if (warp == 0 && *abort) give_up(a, sh);
     if (warp == kScoreWarp) {
         tc_fence_after();
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(sh->tmem) : "memory");
@@ -1701,6 +1738,12 @@ int launch(const KernelArgs& a, int sms, cudaStream_t st) {
 
 }  // namespace attn
 
+static std::atomic<int> g_wait_us{2000000}, g_hold{-1};
+void tree_attn_waits(int wait_us, int hold) {
+    g_wait_us = wait_us;
+    g_hold = hold;
+}
+
 size_t tree_attn_workspace_bytes(int q_heads, int kv_heads, int dim, int width) {
     const int qt = attn::q_tiles(q_heads / kv_heads, width);
     return attn::kSplitBytes + attn::kMlBytes(qt) +
@@ -1715,6 +1758,8 @@ int launch_tree_attn(const TreeAttnArgs& t, int dtype, cudaStream_t st) {
     a.page = divisor((uint32_t)t.page_size);
     a.group = divisor((uint32_t)t.group);
     a.pages = (int)(t.c.slots / t.page_size);
+    a.wait_us = g_wait_us;
+    a.hold = g_hold;
     char* ws = static_cast<char*>(t.ws);
     a.splits = reinterpret_cast<Split*>(ws);
     a.part_ml = reinterpret_cast<float2*>(ws + kSplitBytes);

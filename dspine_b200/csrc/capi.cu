@@ -694,6 +694,12 @@ int dsv_tree_attention(int32_t batch, int64_t rows, int32_t q_heads, int32_t dty
     return counted(dsv::launch_tree_attn(a, dtype, (cudaStream_t)stream), 1);
 }
 
+int dsv_tree_attention_waits(int32_t wait_us, int32_t hold) {
+    if (wait_us < 1 || wait_us > 2000000 || hold < -1) return DSV_BAD_SHAPE;
+    dsv::tree_attn_waits(wait_us, hold);
+    return DSV_OK;
+}
+
 int dsv_accept_tree(int32_t batch, int64_t rows, const int64_t* tokens, const int64_t* top1,
                     const int64_t* tree_mask, const int32_t* q_indptr, int32_t nodes,
                     const int32_t* prefix, const int32_t* slots, int32_t width, int32_t* accept,

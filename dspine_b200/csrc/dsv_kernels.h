@@ -440,6 +440,7 @@ struct TreeAttnArgs {
 };
 size_t tree_attn_workspace_bytes(int q_heads, int kv_heads, int dim, int width);
 int launch_tree_attn(const TreeAttnArgs& a, int dtype, cudaStream_t stream);
+void tree_attn_waits(int wait_us, int hold);
 
 // ---- greedy acceptance over draft trees (tree.cu) -----------------------------------------
 struct TreeAcceptArgs {

@@ -472,7 +472,7 @@ int dsv_kv_read(int64_t tokens, const void* slots, int32_t slots_int64, const ds
  * with more rows is computed all the same).
  * Bits of *err (a device word, may be NULL): bit 1: a page outside the cache, or a length above
  * max_pages * page_size (those positions are unseen, drafted tokens among them); bit 2: a wait inside the kernel timed out
- * (outputs not valid).  The workspace needs no initialisation; calls that may overlap need one
+ * (2 s; the rows that were to come of it are NaN, in out and lse).  The workspace needs no initialisation; calls that may overlap need one
  * each. */
 int dsv_tree_attention_workspace_size(int32_t q_heads, int32_t kv_heads, int32_t dim,
                                       int32_t width, size_t* bytes);
@@ -484,6 +484,12 @@ int dsv_tree_attention(int32_t batch, int64_t rows, int32_t q_heads, int32_t dty
                        int64_t out_token_stride, int64_t out_head_stride, float* lse,
                        uint32_t* err, void* workspace, size_t workspace_bytes,
                        dsv_stream_t stream);
+
+/* For tests of that limit: in the dsv_tree_attention calls of this process from here on, waits give
+ * up after wait_us microseconds (1 to 2000000, the default), and tile `hold` of the keys of each
+ * thread block, with those after it, is never announced (-1, the default: all are), so that the
+ * waits for it run out. */
+int dsv_tree_attention_waits(int32_t wait_us, int32_t hold);
 
 /* ---- greedy acceptance over draft trees ----------------------------------------------------
  * The tree form of dsv_accept_greedy (verification/caps.py:32-59 _accept_capped).  Request b owns

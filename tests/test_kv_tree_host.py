@@ -250,3 +250,9 @@ def test_rows_of_queries_past_32_bits_are_refused(lib):
 
     assert attend(1 << 30, 2) == 1 and attend((1 << 31) - 1, 1) == 1 and attend(1 << 20, 4096) == 1
     assert attend((1 << 30) - 128, 2) == 6                  # taken: the workspace is too small
+
+
+def test_limits_of_waits_that_are_refused(lib):
+    for bad in ((0, -1), (-1, -1), (2000001, -1), (1000, -2)):
+        assert lib.dsv_tree_attention_waits(*bad) == 1
+    assert lib.dsv_tree_attention_waits(2000000, -1) == 0
