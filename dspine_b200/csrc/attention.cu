@@ -1706,6 +1706,8 @@ Divisor divisor(uint32_t d) {
 int q_tiles(int group, int width) { return (long long)group * width > kRows ? 2 : 1; }
 int padded_dim(int dim) { return dim <= 64 ? 64 : 128; }
 
+bool joins(const TreeAttnArgs& t) { return (long long)t.max_pages * t.page_size > kTile; }   // items of one tile are never cut
+
 constexpr size_t kSplitBytes = sizeof(Split) * kMaxCtas;
 constexpr size_t kMlBytes(int qt) { return sizeof(float2) * 2 * kMaxCtas * kRows * qt; }
 
@@ -1719,8 +1721,7 @@ int launch(const KernelArgs& a, int sms, cudaStream_t st) {
     const int grid = sms < kMaxCtas ? sms : kMaxCtas;
     kern<<<grid, kThreads, smem, st>>>(a);
     if (cudaGetLastError() != cudaSuccess) return kLaunchFailed;
-    // items of one tile are never cut
-    if ((long long)a.t.max_pages * a.t.page_size <= kTile) return kOk;
+    if (!joins(a.t)) return kOk;
     cudaLaunchConfig_t cfg = {};
     // two units of four columns a thread where an item is cut in two
     const long long rows = (long long)a.t.group * a.t.width;
@@ -1749,6 +1750,8 @@ size_t tree_attn_workspace_bytes(int q_heads, int kv_heads, int dim, int width) 
     return attn::kSplitBytes + attn::kMlBytes(qt) +
            sizeof(float) * 2 * attn::kMaxCtas * attn::kRows * qt * attn::padded_dim(dim);
 }
+
+int tree_attn_kernels(const TreeAttnArgs& t) { return attn::joins(t) ? 2 : 1; }
 
 int launch_tree_attn(const TreeAttnArgs& t, int dtype, cudaStream_t st) {
     using namespace attn;

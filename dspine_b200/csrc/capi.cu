@@ -691,7 +691,7 @@ int dsv_tree_attention(int32_t batch, int64_t rows, int32_t q_heads, int32_t dty
     a.scale = scale;
     a.err = err;
     a.ws = workspace;
-    return counted(dsv::launch_tree_attn(a, dtype, (cudaStream_t)stream), 1);
+    return counted(dsv::launch_tree_attn(a, dtype, (cudaStream_t)stream), dsv::tree_attn_kernels(a));
 }
 
 int dsv_tree_attention_waits(int32_t wait_us, int32_t hold) {

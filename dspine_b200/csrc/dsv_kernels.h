@@ -439,6 +439,7 @@ struct TreeAttnArgs {
     void* ws;
 };
 size_t tree_attn_workspace_bytes(int q_heads, int kv_heads, int dim, int width);
+int tree_attn_kernels(const TreeAttnArgs& a);   // that launch_tree_attn enqueues
 int launch_tree_attn(const TreeAttnArgs& a, int dtype, cudaStream_t stream);
 void tree_attn_waits(int wait_us, int hold);
 

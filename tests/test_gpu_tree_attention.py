@@ -460,3 +460,16 @@ def test_a_length_past_the_table_leaves_the_drafted_tokens_where_they_are(length
     c.lengths = [min(length, 300), 100]
     c.table = torch.cat([c.table, torch.full((2, 12), 1 << 30, dtype=torch.int32)], 1)
     c.check(got)
+
+
+@pytest.mark.parametrize("length,page,kernels", [(64, 64, 1), (30, 16, 1), (65, 16, 2), (700, 16, 2)])
+def test_the_kernels_of_a_call_are_counted(length, page, kernels):
+    """One, and the one that joins items of more than one tile."""
+    from dspine_b200 import _lib
+
+    c = Case([1], [length], page=page, seed=22)
+    a, k = c.args()
+    table = a[3][:, :-(-length // page)].contiguous()
+    before = _lib.load().dsv_launch_count()
+    attention.tree_attention(a[0], a[1], a[2], table, a[4], **k)
+    assert _lib.load().dsv_launch_count() - before == kernels
