@@ -713,7 +713,8 @@ int dsv_accept_tree(int32_t batch, int64_t rows, const int64_t* tokens, const in
         !path || !new_seq)
         return DSV_BAD_POINTER;
     if (!aligned(tokens, 8) || !aligned(top1, 8) || !aligned(tree_mask, 8) || !aligned(q_indptr, 4) ||
-        !aligned(prefix, 4) || !aligned(slots, 4) || !aligned(bonus, 8) || !aligned(output, 8))
+        !aligned(prefix, 4) || !aligned(slots, 4) || !aligned(bonus, 8) || !aligned(output, 8) ||
+        !aligned(accept, 4) || !aligned(commit, 4) || !aligned(path, 4) || !aligned(kept, 4) || !aligned(new_seq, 4))
         return DSV_BAD_ALIGNMENT;
     dsv::TreeAcceptArgs t = {batch, rows, tokens, top1, tree_mask, q_indptr, nodes, prefix, slots,
                              width, accept, commit, bonus, output, path, kept,

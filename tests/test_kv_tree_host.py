@@ -256,3 +256,17 @@ def test_limits_of_waits_that_are_refused(lib):
     for bad in ((0, -1), (-1, -1), (2000001, -1), (1000, -2)):
         assert lib.dsv_tree_attention_waits(*bad) == 1
     assert lib.dsv_tree_attention_waits(2000000, -1) == 0
+
+
+@pytest.mark.parametrize("name", ["accept", "commit", "bonus", "output", "path", "kept", "new_seq"])
+def test_every_output_of_accept_tree_has_to_be_aligned(lib, name):
+    size = {"bonus": 8, "output": 8}.get(name, 4)
+    out = dict(accept=16, commit=16, bonus=16, output=16, path=16, kept=16, new_seq=16)
+
+    def tree(**more):
+        o = {**out, **more}
+        return lib.dsv_accept_tree(1, 3, 16, 16, 16, 16, 3, None, 16, 8, o["accept"], o["commit"], o["bonus"], o["output"], o["path"],
+                                   o["kept"], o["new_seq"], None)
+
+    for off in range(1, size):
+        assert tree(**{name: 16 + off}) == 4, off
