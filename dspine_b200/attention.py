@@ -10,6 +10,7 @@ Argument errors raise ValueError before anything is launched.
 from __future__ import annotations
 
 import ctypes
+import functools
 import math
 
 import torch
@@ -37,18 +38,12 @@ def tree_mask(parents):
     return mask
 
 
-_sizes: dict = {}
-
-
+@functools.lru_cache(maxsize=64)
 def workspace_bytes(q_heads, kv_heads, dim, width) -> int:
     """Device scratch of one call (partial results of split contexts)."""
-    key = (q_heads, kv_heads, dim, width)
-    n = _sizes.get(key)
-    if n is None:
-        size = ctypes.c_size_t()
-        _lib.call("dsv_tree_attention_workspace_size", q_heads, kv_heads, dim, width, ctypes.byref(size))
-        n = _sizes[key] = int(size.value)
-    return n
+    size = ctypes.c_size_t()
+    _lib.call("dsv_tree_attention_workspace_size", q_heads, kv_heads, dim, width, ctypes.byref(size))
+    return int(size.value)
 
 
 def tree_attention(q, k_cache, v_cache, page_table, kv_lens, *, page_size=1, q_indptr=None, max_width=None,
@@ -68,8 +63,10 @@ def tree_attention(q, k_cache, v_cache, page_table, kv_lens, *, page_size=1, q_i
     softmax(scale q.k) v (scale 1/sqrt(dim) unless given), zeros for a row that sees nothing;
     `return_lse` adds the fp32 [rows, q_heads] logsumexp.  Rows of no request are left as they were.
 
-    max_width: a bound on the rows of a request, by which the work is laid out (results do not
-    depend on it); default 64 with a tree_mask, else all rows.  A tree has at most 64 nodes.
+    max_width: a bound on the rows of a request, by which the work is laid out (results depend on it
+    in the order of their sums alone); default 64 with a tree_mask, else all rows, which costs up to a
+    sixth where the requests are many and short (64 requests of 1 row, up to 512 cached, bf16: 81 us
+    against 70 with max_width=1).  A tree has at most 64 nodes.
     workspace: uint8 scratch of `workspace_bytes` (allocated for the call unless given); calls that may
     overlap need one each.  err (int32 [1], optional) collects bit 1: a page outside the cache or
     a length past the page table (those positions are unseen, drafted tokens among them; no token

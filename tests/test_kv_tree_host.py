@@ -270,3 +270,12 @@ def test_every_output_of_accept_tree_has_to_be_aligned(lib, name):
 
     for off in range(1, size):
         assert tree(**{name: 16 + off}) == 4, off
+
+
+def test_sizes_of_workspaces_are_not_kept_for_every_width(lib):
+    """A server asks with another width at nearly every step."""
+    for width in list(range(1, 2000)) + [1, 5, 1999]:
+        size = ctypes.c_size_t()
+        assert lib.dsv_tree_attention_workspace_size(32, 8, 128, width, ctypes.byref(size)) == 0
+        assert attention.workspace_bytes(32, 8, 128, width) == size.value
+    assert attention.workspace_bytes.cache_info().currsize <= 64
