@@ -34,24 +34,26 @@
 //   combine_kernel  joins the partial results of items that a cut went through.
 //
 // Softmax: weights are 2^(s c - ref), c = scale log2(e), ref a running reference that follows the
-// row's maximum but moves only when the maximum has outgrown it by more than 2^8: the accumulator
-// is then rescaled (a TMEM round trip), else left alone.  Any reference gives the same quotient;
-// 2^8 keeps fp16 weights below 2^14.  Sums and the accumulator are fp32; the weights are rounded
-// once to the operand type.
+// row's maximum but moves only when the maximum has outgrown it by more than 2^8 (fp16: 2^5): the
+// accumulator is then rescaled (a TMEM round trip), else left alone.  Any reference gives the same
+// quotient; fp16's lies 2^9 below the maximum, so that a row's largest weight lies in [2^9, 2^14] and
+// a weight below 2^-23 of it, which fp16 holds with fewer bits, is off by at most 2^-34 of it.  Sums
+// and the accumulator are fp32; the weights are rounded once to the operand type.
 //
 // e4m3 caches: codes are exact in fp16, so they are converted between two rings in shared memory
 // and the matrix instructions run on fp16.  q goes to fp16 with a power of two per row.  K
 // scales multiply the scores; V scales multiply the weights.  The products are what is rounded to
 // fp16, so the reference follows the row's largest product: the maximum, over the keys that the row
 // sees, of s c + e, 2^e the first power of two above the key's V scale.  Where the V scales of a tile
-// lie within 2^kNear of each other and of the last tile's (nearly always; one vote), one e serves for
-// all its keys, at most kNear too large, so that the row's largest product lies in [2, 2^14]: products
-// keep fp16's full precision down to 2^-15 of it and are off by at most 2^-26 of it below.  Other
+// lie within 2^kNear of each other and of the last tile's (nearly always; two ballots), one e serves for
+// all its keys, at most kNear too large, so that the row's largest product lies in [4, 2^14]: products
+// keep fp16's full precision down to 2^-16 of it and are off by at most 2^-27 of it below.  Other
 // tiles take an e a key, in a function of its own (far_unit).  e is held within [-90, 120], so that
 // sums of the weights themselves stay within fp32.
 //
-// A near tile costs what it did with one e for the whole context (64 x 16 245 us, 1 x 16 long 87 from 84: the
-// rare forms are calls, as any code beside the loop slowed it, run or not; an e a key for every tile: 277 and 93).
+// A near tile costs what one e for the whole context did (64 x 16 247 us from 245, 1 x 16 long 87 from 84; an e a
+// key for every tile: 277 and 93).  The rare forms are calls: code beside the loop slowed it whether it
+// ran or not.  With V scales that spread over 2^8 in every tile: 338 and 151 us; over 2^3: as without.
 //
 // Masked positions: scores of unseen keys are replaced by -inf, rows of unreadable positions are
 // zeros in shared memory.  A V element of a drafted token that is not finite would reach rows that
@@ -97,8 +99,9 @@ constexpr int kSoftmaxThreads = 256;
 // tiles per CTA below which fewer CTAs take part; the device's time for 1 request of 333 cached
 // positions (8 items of 6 tiles): 1 tile 16.9 us, 2 16.4, 4 18.4, 8 23.5
 constexpr int kMinTiles = 2;
-constexpr float kSlack = 8.0f;             // log2 by which a maximum may outgrow the reference
-constexpr int kNear = 4;                   // e4m3: powers of two between V scales that one e serves
+// log2 by which a maximum may outgrow the reference, and fp16: by which the reference is set below the maximum
+constexpr float kSlack = 8.0f, kHalfSlack = 5.0f, kHalfRoom = 9.0f;
+constexpr int kNear = 6;                   // e4m3: powers of two between V scales that one e serves
 constexpr int kFar = 0x10000;              // a biased exponent near to none
 constexpr int kSpan = 60;                  // see far_unit
 constexpr float kReach = 120.0f, kFarthest = 400.0f;   // log2 of a step of scaling; beyond kFarthest nothing is left in any case
@@ -689,8 +692,8 @@ struct FarResult {
 // accumulator and sum follow in steps of 2^-kReach (three at most; scores that differ by kFarthest
 // leave nothing).  The tiles between scale in one step.  What that flushes to zero (factors below
 // 2^-126) has to be nothing beside the new sum.  A sum is at most (keys) x 2^(14 - e_eff), e_eff the least
-// that e has added to the maximum of a row's scores so far, and the new one at least 2^(2 - e): with
-// 2^31 keys and e <= e_eff + kSpan, 2^(31 + 14 - 2 + kSpan - 126) = 2^-23 of it, and 2^-37 with 2^17
+// that e has added to the maximum of a row's scores so far, and the new one at least 2^(9 - kNear - e): with
+// 2^31 keys and e <= e_eff + kSpan, 2^(31 + 14 - 3 + kSpan - 126) = 2^-24 of it, and 2^-38 with 2^17
 // keys.  So where the V scales have risen by more than kSpan above e_eff, the tiles to come are far
 // as well.
 __device__ __noinline__ FarResult far_unit(uint32_t ts, uint32_t to, int dim, float cm, uint2 vis, const TileInfoScaled& inf, float ref,
@@ -730,8 +733,8 @@ __device__ __noinline__ FarResult far_unit(uint32_t ts, uint32_t to, int dim, fl
     *e_eff = least;                                             // every lane the same
     most += 127 - kNear;                                        // biased; room for one power above these
     e_low = max(most, 36) - 126 > least + kSpan - kNear ? kFar : max(most, 36);
-    target -= 6.0f;
-    for (int k = 0; k < 4 && __any_sync(0xffffffffu, target > ref + kSlack); ++k) {
+    target -= kHalfRoom;
+    for (int k = 0; k < 4 && __any_sync(0xffffffffu, target > ref + kHalfSlack); ++k) {
         float to_ref = fmaxf(ref, target);
         if (k < 3 && to_ref < ref + kFarthest) to_ref = fminf(to_ref, ref + kReach);
         if (used) {                                             // the accumulator holds something
@@ -1458,11 +1461,11 @@ __global__ void __launch_bounds__(kThreads, 1) attn_kernel(const __grid_constant
                         }
                         float target = fmaxf(mx[0], mx[1]) * cm;
                         if constexpr (kFp8) {
-                            target += (float)(e_low + kNear - 126 - 6);
+                            target += (float)(e_low + kNear - 126) - kHalfRoom;
                         } else if constexpr (std::is_same<TO, __half>::value) {
-                            target -= 6.0f;
+                            target -= kHalfRoom;
                         }
-                        if (__any_sync(0xffffffffu, target > ref + kSlack)) {
+                        if (__any_sync(0xffffffffu, target > ref + (std::is_same<TO, __half>::value ? kHalfSlack : kSlack))) {
                             const float to_ref = fmaxf(ref, target);
                             if (tl >= step) {                       // the accumulator holds something
                                 ok = __all_sync(0xffffffffu, wait_or_abort(&sh->s_free[s][b ^ 1], ((ph >> (b ^ 1)) & 1u) ^ 1u, abort));

@@ -462,7 +462,7 @@ int dsv_kv_read(int64_t tokens, const void* slots, int32_t slots_int64, const ds
  * out[row, head] = sum softmax(scale * q . k) v over those, rounded once to dtype; lse [rows,
  * q_heads] fp32 (may be NULL) the natural logsumexp of the scaled scores.  With e4m3
  * the products weight * V scale are rounded to fp16 relative to the largest of those that the row
- * sees (by 2^-11 of themselves, 2^-26 of the largest at least; V scales from 2^-90 to 2^120).  A row that sees
+ * sees (by 2^-11 of themselves, 2^-27 of the largest at least; V scales from 2^-90 to 2^120).  A row that sees
  * nothing gets zeros and -inf.  Query head hq reads KV head hq / (q_heads / heads)
  * (at most 4096 of them each; rows times that number at most 0x7fffff00).
  * dtype (q and out) DSV_BF16 or DSV_F16; the cache has the same type or is e4m3; dim a multiple

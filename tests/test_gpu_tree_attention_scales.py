@@ -149,3 +149,25 @@ def test_v_scales_that_are_not_finite_reach_the_rows_that_see_them(value, dim, g
     clean = c.want()
     bound, _ = R.attention_bounds(*clean, dim=dim, out_dtype=c.kind, weight_half_step=2.0 ** -11)
     assert bool(((out - clean[0]).abs() <= bound + _products_bound(c))[~touched].all())
+
+
+@pytest.mark.parametrize("power,at", [(28, 299), (31, 310), (33, 257), (36, 500)])     # the first three in one tile
+def test_fp16_values_of_next_to_no_weight(power, at):
+    """An fp16 cache: one key carries the weight, another has 2^-power of it but 2^26 times its V."""
+    c = Case([2, 1], [702, 65], heads=4, kv_heads=1, dim=64, kind="fp16", cache="fp16", seed=9)
+    slots = _slots(c, 0, torch.arange(702))
+    c.q[..., 0] = 8.0
+    c.k[slots, 0] = 0.0
+    c.k[slots, 0, 0] = -60 * math.log(2.0)                 # scale 1/8 x 8
+    c.k[slots[300], 0, 0] = 0.0
+    c.k[slots[at], 0, 0] = -(power + 0.53) * math.log(2.0)
+    c.v[slots] = (c.v[slots].float() * 2.0 ** -10).half()
+    c.v[slots[at]] = 60000.0
+    out, lse = (x.double().cpu() for x in c.run())
+    want = c.want()
+    bound, lse_bound = R.attention_bounds(*want, dim=64, out_dtype=c.kind, weight_half_step=2.0 ** -11)
+    # the row's largest weight lies in [2^9, 2^14]: one below fp16's normal numbers is off by up to 2^-25, so by 2^-34
+    # of the largest (at most 1), times its value: 60000 of one key, 2^-8 at most of the 700 others
+    bound[:2] += 2.0 ** -34 * (60000.0 + 700 * 2.0 ** -8)
+    assert bool(((out - want[0]).abs() <= bound).all()), float(((out - want[0]).abs() / bound).max())
+    assert bool(((lse - want[1]).abs() <= lse_bound).all())
