@@ -60,8 +60,9 @@ def tree_attention(q, k_cache, v_cache, page_table, kv_lens, *, page_size=1, q_i
 
     Row i of a request sees every position before its drafted tokens, and drafted token j where
     bit j of tree_mask[row] (int64 [rows]) is set, or without a tree_mask where j <= i.  The result is
-    softmax(scale q.k) v (scale 1/sqrt(dim) unless given), zeros for a row that sees nothing;
-    `return_lse` adds the fp32 [rows, q_heads] logsumexp.  Rows of no request are left as they were.
+    softmax(scale q.k) v (scale 1/sqrt(dim) unless given), zeros for a row that sees nothing (or scores
+    of -inf alone); `return_lse` adds the fp32 [rows, q_heads] logsumexp.  Rows of no request are left
+    as they were.
 
     max_width: a bound on the rows of a request, by which the work is laid out (results depend on it
     in the order of their sums alone); default 64 with a tree_mask, else all rows, which costs up to a

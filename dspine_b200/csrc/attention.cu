@@ -60,18 +60,19 @@
 // do not see it through 0 x inf; tiles with drafted tokens are scanned, such elements zeroed and
 // added back to the rows that do see them.
 //
-// Measured (32 query heads over 8 KV heads of 128 unless said; ragged lengths; caches larger than L2):
-//   64 requests x 1 token, up to 8192 cached, bf16, pages of 16     242 us, 5.0 TB/s: the cache's bytes
+// Measured (32 query heads over 8 KV heads of 128 unless said; ragged lengths; caches larger than L2, three sets of
+// inputs in turn).  Cycles are from a build that reads the clock, which is up to a third slower in all:
+//   64 requests x 1 token, up to 8192 cached, bf16, pages of 16     245 us, 4.9 TB/s: the cache's bytes
 //       (copy bandwidth would take 186), less what segment switches cost (a tenth)
-//   16 requests x trees of up to 64, 64 query heads, up to 16384    365 us, 0.62 PFLOP/s: the softmax
-//       warps' exponentials (a unit of 64 keys: 1700 cycles, 512 of them at least for the ex2 of its
-//       warp, twice for two warps a scheduler; its matrix instructions: 640)
-//   64 requests x 16 tokens, up to 4096 cached, e4m3, pages of 1    243 us, and 1 x 16 tokens, 131071
-//       cached, 4 KV heads 84 us: the loaders' conversion (two warps for K, two for V: 1500 cycles a
-//       tile of the 1750 to 2100 that one takes), beside it the integer pipe (half busy) and shared
-//       memory (970 wavefronts a tile by its threads, 510 more for the matrix operands).  64 x 16 loses a fifth
-//       to segment switches besides
-//   1 request x 1 token, 333 cached                                 24 us a call from Python, the host's time (19 us
+//   16 requests x trees of up to 64, 64 query heads, up to 16384    368 us, 0.62 PFLOP/s: the latency of a unit, whose
+//       phases (scores from TMEM, maximum, exponentials, weights to TMEM) follow one another with two softmax warps a
+//       scheduler: 1390 cycles of work and 630 of waiting for scores for 64 keys; no pipe is above 40%
+//   64 requests x 16 tokens, up to 4096 cached, e4m3, pages of 1    247 us: softmax warps work 3900 cycles on a unit
+//       and wait 600 for its scores, loaders convert 1800 a tile and wait 3200 for a free stage (two tiles a ring): the
+//       chain of conversion, scores, weights and accumulation through short rings; a switch of segments takes 9400
+//   1 request x 16 tokens, 131071 cached, 4 KV heads, e4m3          86 us: work 2400 a unit and 600 of waiting,
+//       conversion 1950 a tile and 500 of waiting: both sides nearly always at work, each by its own latency
+//   1 request x 1 token, 333 cached                                 24 us a call from Python, the host's time (16 us
 //       in attn_kernel when all caches are cold: the chain of waits from the plan to the join)
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -602,8 +603,9 @@ __device__ __noinline__ void bring_queries(const KernelArgs& a, const Walk& w, u
                 unpack2(x[i].z, f[4], f[5], TQ());
                 unpack2(x[i].w, f[6], f[7], TQ());
                 unpack2(top[i], m, none, TQ());
-                // a power of two that brings the row's largest value to [2^13, 2^14): products
-                // stay exact, and values down to 2^-37 of the largest keep a place in fp16.  A
+                // a power of two that brings the row's largest value to [2^13, 2^14): products stay
+                // exact, values down to 2^-27 of the largest keep fp16's precision (a bf16 value is
+                // whole down to 2^-30), those down to 2^-37 a place in fp16.  A
                 // row with a NaN or an infinity is left as it is: its scores are NaN or infinite
                 int e = (int)(__float_as_uint(m) >> 23) - 127;
                 e = m > 0.f && e < 128 ? max(e, -100) : 13;
@@ -698,6 +700,7 @@ struct FarResult {
 // as well.
 __device__ __noinline__ FarResult far_unit(uint32_t ts, uint32_t to, int dim, float cm, uint2 vis, const TileInfoScaled& inf, float ref,
                                            float sum, int e_low, Shared* sh, uint64_t* used, uint32_t parity) {
+    __syncwarp();
     const float *ks = inf.ks, *vs = inf.vs;
     volatile int *e_eff = &sh->e_eff[threadIdx.x >> 5], *abort = &sh->abort;
     auto power = [](float scale) {                              // e of a scale; of one that is not finite the least
@@ -931,8 +934,8 @@ __global__ void __launch_bounds__(kThreads, 1) attn_kernel(const __grid_constant
     tc_fence_after();
     constexpr uint32_t tmem = 0;                           // all 512 columns were allocated
     // Up to 64 rows only the softmax warps of schedulers 0 and 1 have any: the loaders there change
-    // places with the index and the query warp (64 x 16 e4m3, 64 rows: 243.2 us from 246.0; 64 x 1 bf16, 4 rows:
-    // 215.3 from 216.0).  With more rows they would meet on schedulers 2 and 3 alone.
+    // places with the index and the query warp (the change alone, on one set of inputs repeated, which L2 serves in
+    // part: 64 x 16 e4m3, 64 rows: 243.2 us from 246.0; 64 x 1 bf16, 4 rows: 215.3 from 216.0).  With more rows they would meet on schedulers 2 and 3 alone.
     const int role = (long long)t.group * t.width <= 64 && warp >= kIndexWarp && warp < kFirstLoader + 2 ? warp ^ 6 : warp;
     if (role >= kFirstLoader) {
         // ---------------- loaders: rows of K and V by 16-byte copies of the lanes -----------------

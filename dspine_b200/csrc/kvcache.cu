@@ -12,8 +12,8 @@
 // A row is read once and written once.  A lane holds 16 elements because 16 codes are one 16-byte
 // access of the cache: the widest there is, and rows of 128 elements then need 8 lanes, so a warp
 // moves 4 rows at a time.  Measured with 8 heads of 128, e4m3, bf16 rows: 131072 tokens read in
-// 147 us (5.5 TB/s, bound by memory); 32749 written in 51.5 us (4.0 TB/s, bound by issue: 318
-// instructions for the 16 elements of a lane, schedulers 75% busy.  The next row's loads ahead of this
+// 145 us (5.6 TB/s, bound by memory); 32749 written in 51.4 us (4.0 TB/s, bound by issue: 318
+// instructions for the 16 elements of a lane, schedulers 70% busy.  The next row's loads ahead of this
 // one's arithmetic took the same time; arithmetic on pairs took fewer instructions but more
 // registers, 53 us).
 #include <cuda_bf16.h>
@@ -133,7 +133,8 @@ __device__ __forceinline__ uint32_t codes4(float a, float b, float c, float d) {
 // The codes of x / s, IEEE quotients rounded to e4m3.  In a row of finite values a quotient takes a
 // product with r = 1 / s and two corrections by its exact residual (P. Markstein, "Computation of
 // elementary functions on the IBM RISC System/6000 processor", 1990: with r rounded correctly, the
-// first leaves a quotient off by less than a step, the second rounds that one correctly).  s
+// first leaves a quotient off by less than a step, the second rounds that one correctly; fp32 rows need
+// both, for bf16 ones the first is correct already, over all pairs of mantissas).  s
 // within 2^-60 and 2^100 keeps r normal and the residuals of all quotients from 2^-42 on exact (they
 // are multiples of 2^-47 s y); smaller ones are far below half of the smallest code, 2^-10.  The residual is taken as q s - x, so that -0
 // stays -0.

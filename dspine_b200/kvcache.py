@@ -120,7 +120,8 @@ def write_kv(k, v, k_cache, v_cache, slots, *, k_scale=None, v_scale=None, err=N
     go into an e4m3 cache as codes, with their scale amax / 448 in k_scale and v_scale.  Rows may
     be views of a wider projection (any token and head strides of 16-byte steps).  A negative slot
     is skipped; one past the cache is skipped and sets bit 0 of `err` (int32 [1], optional).  The
-    slots of one call should differ: of tokens that share one, any may be kept, or a mixture."""
+    slots of one call should differ: of tokens that share one, any may be kept, or a mixture.  k and v
+    must not be views of the cache itself."""
     c = describe(k_cache, v_cache, k_scale, v_scale)
     dev = k_cache.device
     shape = k.shape

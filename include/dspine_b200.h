@@ -415,7 +415,8 @@ int dsv_rescore_select16(int32_t rows, int32_t cands, int32_t hidden, int32_t vo
  * into: per slot and KV head one K row and one V row of `dim` elements.  dtype DSV_BF16 or
  * DSV_F16 holds the rows as they are; DSV_E4M3 holds codes with one fp32 scale per (slot, head),
  * value = code * scale, quantised by the rule of dsv_fp8_quantize_rows applied to each head's row
- * (scale = amax / 448, 1 for a row of zeros or with a NaN).  No counterpart in the reference
+ * (scale = amax / 448, 1 for a row of zeros or with a NaN; the scale of an fp32 row below 3.1e-43
+ * underflows to 0, its codes are then +-448 and, for zeros, NaN).  No counterpart in the reference
  * (SGLang owns the cache).  K and V have the same strides; dim is a multiple of 16, at most 256;
  * rows start on 16-byte boundaries. */
 typedef struct {
@@ -436,7 +437,7 @@ typedef struct {
  * strides in elements, rows on 16-byte boundaries) to slot slots[n] (int32, or int64 where
  * slots_int64).  A negative slot is skipped; one past the cache is skipped and sets bit 0 of
  * *err (a device word, may be NULL).  Of tokens that share a slot any may be kept, or a mixture
- * of them: the slots of one call should differ.  A cache that is not e4m3 takes rows of its own
+ * of them: the slots of one call should differ.  The rows must not overlap the cache.  A cache that is not e4m3 takes rows of its own
  * type only.  tokens * heads < 2^31. */
 int dsv_kv_write(int64_t tokens, int32_t dtype, const void* k, int64_t k_token_stride,
                  int64_t k_head_stride, const void* v, int64_t v_token_stride,
@@ -462,8 +463,8 @@ int dsv_kv_read(int64_t tokens, const void* slots, int32_t slots_int64, const ds
  * out[row, head] = sum softmax(scale * q . k) v over those, rounded once to dtype; lse [rows,
  * q_heads] fp32 (may be NULL) the natural logsumexp of the scaled scores.  With e4m3
  * the products weight * V scale are rounded to fp16 relative to the largest of those that the row
- * sees (by 2^-11 of themselves, 2^-27 of the largest at least; V scales from 2^-90 to 2^120).  A row that sees
- * nothing gets zeros and -inf.  Query head hq reads KV head hq / (q_heads / heads)
+ * sees (by 2^-11 of themselves, 2^-27 of the largest at least; V scales from 2^-90 to 2^120, K
+ * scales below 2^97).  A row that sees nothing (or scores of -inf alone) gets zeros and -inf.  Query head hq reads KV head hq / (q_heads / heads)
  * (at most 4096 of them each; rows times that number at most 0x7fffff00).
  * dtype (q and out) DSV_BF16 or DSV_F16; the cache has the same type or is e4m3; dim a multiple
  * of 16, at most 128; cache->slots a multiple of page_size; max_pages * page_size at most
