@@ -934,8 +934,9 @@ __global__ void __launch_bounds__(kThreads, 1) attn_kernel(const __grid_constant
     tc_fence_after();
     constexpr uint32_t tmem = 0;                           // all 512 columns were allocated
     // Up to 64 rows only the softmax warps of schedulers 0 and 1 have any: the loaders there change
-    // places with the index and the query warp (the change alone, on one set of inputs repeated, which L2 serves in
-    // part: 64 x 16 e4m3, 64 rows: 243.2 us from 246.0; 64 x 1 bf16, 4 rows: 215.3 from 216.0).  With more rows they would meet on schedulers 2 and 3 alone.
+    // places with the index and the query warp (the change alone, on one set of inputs repeated, which L2
+    // serves in part: 64 x 16 e4m3, 64 rows: 243.2 us from 246.0; 64 x 1 bf16, 4 rows: 215.3 from 216.0).
+    // With more rows they would meet on schedulers 2 and 3 alone.
     const int role = (long long)t.group * t.width <= 64 && warp >= kIndexWarp && warp < kFirstLoader + 2 ? warp ^ 6 : warp;
     if (role >= kFirstLoader) {
         // ---------------- loaders: rows of K and V by 16-byte copies of the lanes -----------------
